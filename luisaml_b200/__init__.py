@@ -7,6 +7,9 @@ Layers:
 * ``lib/liblcml_onnx.so`` the C++ host mirror of LuisaML's operator registry,
   tensor API and NetworkInstance (``include/lcml_onnx.h``), whose operators
   call the C ABI;
+* ``decoder``             the operators of a decoder layer around the FP8 GEMMs
+  (``include/lcml_decoder.h``): RMS norm with an e4m3 output, the paged e4m3
+  key/value cache and the attention over it;
 * this module: torch-tensor helpers over the C ABI (device memory, streams)
   used by tests and bench.py. PyTorch is plumbing here, not the product.
 """
@@ -18,9 +21,19 @@ from . import _capi
 from ._capi import (TENSOR_DYNAMIC_WORKSPACE_BYTES, DTYPE_BFLOAT16, DTYPE_E4M3, DTYPE_FLOAT, EPI_NONE, EPI_RELU, EPI_SILU_MUL, SCALE_AXIS,
                     SCALE_COL, SCALE_ROW, SCALE_TENSOR, GemmDesc, LcmlError, check)
 
-__all__ = ["lib", "check", "LcmlError", "quantize", "quantize_from_amax", "quantize_rows_dynamic",
+_DECODER = ("rmsnorm_quantize", "kv_cache_write", "kv_cache_read", "kv_attention", "kv_attention_workspace_size")
+
+__all__ = [*_DECODER, "lib", "check", "LcmlError", "quantize", "quantize_from_amax", "quantize_rows_dynamic",
            "quantize_tensor_dynamic", "amax", "dequantize", "transpose_u8", "gemm", "gemm_rowquant", "launch_count",
            "device_error"]
+
+
+def __getattr__(name):
+    if name in _DECODER:  # luisaml_b200.decoder imports torch, which this module does only when a call needs it
+        from . import decoder
+        globals().update({n: getattr(decoder, n) for n in _DECODER})
+        return globals()[name]
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
 def lib():

@@ -1,4 +1,5 @@
-"""ctypes binding of the C ABI in include/lcml_fp8.h (liblcml_fp8.so).
+"""ctypes binding of the C ABI in include/lcml_fp8.h and include/lcml_decoder.h
+(liblcml_fp8.so).
 
 This is the binding a Python caller of the reference's operator path would
 add; tests and bench.py go through it so every GPU number is measured across
@@ -82,6 +83,48 @@ class ConvDesc(ctypes.Structure):
     ]
 
 
+class KvCache(ctypes.Structure):
+    """lcml_kv_cache (include/lcml_decoder.h)."""
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+        ("num_pages", ctypes.c_int64),
+        ("page_size", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+        ("scale_block", ctypes.c_int32),
+    ]
+
+
+class KvBatch(ctypes.Structure):
+    """lcml_kv_batch."""
+    _fields_ = [
+        ("batch", ctypes.c_int32), ("table_cols", ctypes.c_int32),
+        ("block_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+        ("cu_tokens", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("total_tokens", ctypes.c_int64),
+    ]
+
+
+class RmsnormDesc(ctypes.Structure):
+    """lcml_rmsnorm_desc."""
+    _fields_ = [
+        ("rows", ctypes.c_int64), ("cols", ctypes.c_int64),
+        ("x", ctypes.c_void_p), ("ldx", ctypes.c_int64), ("residual", ctypes.c_void_p), ("ldr", ctypes.c_int64),
+        ("h_out", ctypes.c_void_p), ("ldh", ctypes.c_int64), ("weight", ctypes.c_void_p),
+        ("x_dtype", ctypes.c_int), ("weight_dtype", ctypes.c_int), ("eps", ctypes.c_float),
+        ("scale", ctypes.c_void_p), ("scale_out", ctypes.c_void_p), ("q", ctypes.c_void_p),
+    ]
+
+
+class KvAttentionDesc(ctypes.Structure):
+    """lcml_kv_attention_desc."""
+    _fields_ = [
+        ("cache", ctypes.POINTER(KvCache)), ("batch", ctypes.POINTER(KvBatch)),
+        ("q", ctypes.c_void_p), ("q_token_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64),
+        ("out", ctypes.c_void_p), ("out_token_stride", ctypes.c_int64), ("out_head_stride", ctypes.c_int64),
+        ("lse", ctypes.c_void_p), ("q_heads", ctypes.c_int32), ("dtype", ctypes.c_int),
+        ("max_tokens", ctypes.c_int64), ("softmax_scale", ctypes.c_float), ("softcap", ctypes.c_float),
+        ("window", ctypes.c_int32), ("causal", ctypes.c_int), ("workspace", ctypes.c_void_p), ("variant", ctypes.c_int),
+    ]
+
+
 _c_i64 = ctypes.c_int64
 _vp = ctypes.c_void_p
 _ci = ctypes.c_int
@@ -141,12 +184,19 @@ PROTOTYPES = {
                        _ci, _c_i64, _vp],
     "lcml_global_avgpool": [_vp, _ci, _vp, _c_i64, _c_i64, _c_i64, _ci, _vp, _vp],
     "lcml_cast": [_vp, _ci, _vp, _ci, _c_i64, _vp],
+    "lcml_rmsnorm_quantize": [ctypes.POINTER(RmsnormDesc), _vp],
+    "lcml_kv_cache_write": [ctypes.POINTER(KvCache), ctypes.POINTER(KvBatch), _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64,
+                            _ci, _vp],
+    "lcml_kv_cache_read": [ctypes.POINTER(KvCache), ctypes.POINTER(KvBatch), _vp, _vp, _ci, _vp],
+    "lcml_kv_attention_workspace_size": [ctypes.POINTER(KvAttentionDesc)],
+    "lcml_kv_attention": [ctypes.POINTER(KvAttentionDesc), _vp],
 }
 _RESTYPES = {
     "lcml_last_error": ctypes.c_char_p,
     "lcml_launch_count": ctypes.c_uint64,
     "lcml_fp8_conv_workspace_size": ctypes.c_int64,
     "lcml_fp8_conv_packed_k": ctypes.c_int64,
+    "lcml_kv_attention_workspace_size": ctypes.c_int64,
 }
 
 _lib = None

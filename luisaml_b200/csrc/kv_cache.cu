@@ -1,0 +1,306 @@
+// The paged e4m3 key/value cache: quantizing write and read back
+// (lcml_kv_cache_write, lcml_kv_cache_read).
+//
+// Work unit: one block of scale_block positions of one sequence, the span of
+// one scale. Sequence b's n tokens touch at most floor(n / block) + 2 blocks,
+// so its units start at floor(cu[b] / block) + 2 b (increasing by at least
+// that many per sequence): the grid's size follows from host-known totals and
+// each CTA finds its sequence by one search in cu_tokens, whatever the
+// lengths on the device. A CTA takes one unit and a share of its heads (K and
+// V), so the look-ups (sequence, length, page) are paid once per unit.
+//
+// Bound: HBM for prompts; for a decode step the chain of dependent look-ups
+// (cu -> length -> page -> codes and scales) of a few L2 latencies.
+#include "lcml_decoder.cuh"
+
+namespace lcml {
+
+int check_cache(const lcml_kv_cache *c, const char *what) {
+    LCML_CHECK_ARG(c != nullptr, "%s: null cache", what);
+    LCML_CHECK_ARG(c->num_pages >= 0 && c->kv_heads > 0 && c->page_size > 0, "%s: bad cache extents", what);
+    LCML_CHECK_ARG(c->head_dim == 64 || c->head_dim == 128 || c->head_dim == 256, "%s: head_dim %d is not 64, 128 or 256", what,
+                   c->head_dim);
+    LCML_CHECK_ARG(c->scale_block > 0 && c->scale_block % 16 == 0 && c->page_size % c->scale_block == 0,
+                   "%s: scale_block %d is not a multiple of 16 that divides page_size %d", what, c->scale_block, c->page_size);
+    LCML_CHECK_ARG(static_cast<int64_t>(c->scale_block) * c->head_dim <= 32768, "%s: scale_block * head_dim exceeds 32768", what);
+    LCML_CHECK_ARG(c->kv_heads <= 4096 && c->page_size <= 65536 && c->num_pages <= 0x7fffffff, "%s: cache extent too large", what);
+    if (c->num_pages > 0) {
+        LCML_CHECK_ARG(c->k && c->v && c->k_scale && c->v_scale, "%s: null cache pointer", what);
+        LCML_CHECK_ARG(aligned(c->k, 16) && aligned(c->v, 16) && aligned(c->k_scale, 4) && aligned(c->v_scale, 4),
+                       "%s: cache pointers must be 16-byte (codes) and 4-byte (scales) aligned", what);
+    }
+    return LCML_OK;
+}
+
+int check_batch(const lcml_kv_batch *b, const char *what) {
+    LCML_CHECK_ARG(b != nullptr, "%s: null batch", what);
+    LCML_CHECK_ARG(b->batch >= 0 && b->table_cols >= 0 && b->total_tokens >= 0, "%s: negative extent", what);
+    LCML_CHECK_ARG(b->total_tokens <= 0x7fffffff, "%s: too many tokens", what);
+    LCML_CHECK_ARG(b->table_stride >= b->table_cols, "%s: table_stride is less than table_cols", what);
+    if (b->batch > 0) {
+        LCML_CHECK_ARG(b->cu_tokens && b->lengths && (b->block_table || b->table_cols == 0), "%s: null batch pointer", what);
+        LCML_CHECK_ARG(aligned(b->cu_tokens, 4) && aligned(b->lengths, 4) && aligned(b->block_table, 4),
+                       "%s: a batch pointer is not 4-byte aligned", what);
+    }
+    return LCML_OK;
+}
+
+namespace {
+
+constexpr int kUnitThreads = 1024;  // at most: scale_block * head_dim / 32 threads handle a unit
+
+// One unit as a CTA sees it.
+struct Unit {
+    int64_t page;      // -1: nothing to do
+    int first;         // position of the block's first slot
+    int lo, hi;        // the call's tokens in the block, as slots [lo, hi)
+    int64_t token;     // packed index of the token in slot lo
+    int old;           // slots [0, old) hold earlier tokens
+    int slot;          // the block's first slot within its page
+};
+
+__device__ __forceinline__ Unit find_unit(const lcml_kv_cache &c, const lcml_kv_batch &b, int64_t u, int *err) {
+    Unit r;
+    r.page = -1;
+    const int blk = c.scale_block;
+    const int s = find_sequence(b.cu_tokens, b.batch, u, 1, blk, 2);
+    const int t0 = __ldg(b.cu_tokens + s), t1 = min(static_cast<int64_t>(__ldg(b.cu_tokens + s + 1)), b.total_tokens);
+    const int start = __ldg(b.lengths + s);
+    const int64_t i = u - (t0 / blk + 2 * static_cast<int64_t>(s));  // the sequence's i-th block
+    const int64_t first = (static_cast<int64_t>(start) / blk + i) * blk;
+    if (t0 < 0 || start < 0 || first >= static_cast<int64_t>(start) + (t1 - t0)) return r;
+    r.first = static_cast<int>(first);
+    r.lo = max(0, start - r.first);
+    r.hi = static_cast<int>(min(static_cast<int64_t>(blk), start + static_cast<int64_t>(t1 - t0) - first));
+    r.old = r.lo;
+    r.token = t0 + (first + r.lo - start);
+    const int64_t col = first / c.page_size;
+    r.slot = static_cast<int>(first % c.page_size);
+    const int64_t page = col < b.table_cols ? __ldg(b.block_table + s * b.table_stride + col) : -1;
+    if (page < 0 || page >= c.num_pages) {
+        if (threadIdx.x == 0) record_device_error(err, kDevBadPage);
+        return r;
+    }
+    r.page = page;
+    return r;
+}
+
+struct WriteArgs {
+    lcml_kv_cache c;
+    lcml_kv_batch b;
+    const void *x[2];
+    int64_t token_stride[2], head_stride[2];
+    int *err;
+};
+
+// |x| as ordered bits, non-finite values as 0.
+__device__ __forceinline__ uint32_t abs_bits_finite(float x) {
+    const uint32_t a = __float_as_uint(x) & 0x7fffffffu;
+    return a >= 0x7f800000u ? 0u : a;
+}
+
+constexpr float kMinScale = 7.888609052210118e-31f;  // 2^-100
+
+// The unit's new values stay in registers (kVpt vectors of 8 per thread)
+// between the maximum and the encoding, so they are read once.
+constexpr int kVpt = 4;
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kUnitThreads) k_kv_cache_write(WriteArgs a) {
+    griddep_launch_dependents();
+    griddep_wait();
+    __shared__ uint32_t red[2][32];
+    const Unit un = find_unit(a.c, a.b, blockIdx.x, a.err);
+    if (un.page < 0) return;
+    const int hk = a.c.kv_heads, d = a.c.head_dim, blk = a.c.scale_block, per_row = d >> 3;
+    const int shift = d == 64 ? 3 : (d == 128 ? 4 : 5);  // per_row = 1 << shift
+    const int nv = (un.hi - un.lo) * per_row;            // vectors of new values
+    const int w = threadIdx.x >> 5, l = threadIdx.x & 31, nw = blockDim.x >> 5;
+    int turn = 0;
+    for (int item = blockIdx.y; item < 2 * hk; item += gridDim.y, turn ^= 1) {
+        const int kv = item >= hk ? 1 : 0, head = item - kv * hk;
+        const T *x = static_cast<const T *>(a.x[kv]);
+        x += un.token * a.token_stride[kv] + head * a.head_stride[kv];
+        const int64_t base = (un.page * hk + head) * a.c.page_size + un.slot;
+        uint8_t *codes = (kv ? a.c.v : a.c.k) + base * d;
+        float *scale = (kv ? a.c.v_scale : a.c.k_scale) + base / blk;
+        const float s_old = un.old > 0 ? *scale : 0.0f;
+        float v[kVpt][8];
+        uint32_t mx = 0;
+#pragma unroll
+        for (int j = 0; j < kVpt; ++j) {
+            const int i = threadIdx.x + j * blockDim.x;
+            if (i < nv) {
+                const T *p = x + (i >> shift) * a.token_stride[kv] + ((i & (per_row - 1)) << 3);
+                if constexpr (VEC) {
+                    load_vec<T, 8>(p, v[j]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[j][e] = Elem<T>::load(p + e);
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) mx = max(mx, abs_bits_finite(v[j][e]));
+            }
+        }
+        mx = __reduce_max_sync(0xffffffffu, mx);
+        if (nw > 1) {  // two buffers in turn: one barrier per item
+            if (l == 0) red[turn][w] = mx;
+            __syncthreads();
+            mx = __reduce_max_sync(0xffffffffu, l < nw ? red[turn][l] : 0u);
+        }
+        const float amax = __uint_as_float(mx);
+        float s = amax > 0.0f ? fmaxf(__fdiv_rn(amax, 448.0f), kMinScale) : 0.0f;
+        const bool grew = un.old > 0 && s > s_old;
+        s = fmaxf(s, s_old);
+        const float div = s > 0.0f ? s : 1.0f;
+        const float r = __frcp_rn(div);
+        const bool ok = scale_fast_ok(div, r);
+#pragma unroll
+        for (int j = 0; j < kVpt; ++j) {
+            const int i = threadIdx.x + j * blockDim.x;
+            if (i < nv) {
+                uint32_t q[2];
+                quantize_block_fast<8>(v[j], div, r, ok, q);
+                *reinterpret_cast<uint2 *>(codes + (un.lo + (i >> shift)) * d + ((i & (per_row - 1)) << 3)) = make_uint2(q[0], q[1]);
+            }
+        }
+        if (grew) {  // the earlier codes move to the new scale
+            for (int i = threadIdx.x; i < un.old * per_row; i += blockDim.x) {
+                uint2 *p = reinterpret_cast<uint2 *>(codes) + i;
+                const uint2 c = *p;
+                float f[8];
+                e4m3x2_decode(c.x & 0xffffu, f[0], f[1]);
+                e4m3x2_decode(c.x >> 16, f[2], f[3]);
+                e4m3x2_decode(c.y & 0xffffu, f[4], f[5]);
+                e4m3x2_decode(c.y >> 16, f[6], f[7]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] *= s_old;
+                uint32_t q[2];
+                quantize_block_fast<8>(f, div, r, ok, q);
+                *p = make_uint2(q[0], q[1]);
+            }
+        }
+        // every thread has its s_old before the barrier above (nw > 1) or in lockstep (one warp)
+        if (nw == 1) __syncwarp();
+        if (threadIdx.x == 0) *scale = s;
+    }
+}
+
+struct ReadArgs {
+    lcml_kv_cache c;
+    lcml_kv_batch b;
+    void *y[2];
+    int *err;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kUnitThreads) k_kv_cache_read(ReadArgs a) {
+    griddep_launch_dependents();
+    griddep_wait();
+    const Unit un = find_unit(a.c, a.b, blockIdx.x, a.err);
+    if (un.page < 0) return;
+    const int hk = a.c.kv_heads, d = a.c.head_dim, blk = a.c.scale_block;
+    const int shift = d == 64 ? 3 : (d == 128 ? 4 : 5), per_row = 1 << shift;
+    const int nv = (un.hi - un.lo) * per_row;
+    for (int item = blockIdx.y; item < 2 * hk; item += gridDim.y) {
+        const int kv = item >= hk ? 1 : 0, head = item - kv * hk;
+        if (a.y[kv] == nullptr) continue;
+        T *y = static_cast<T *>(a.y[kv]) + (un.token * hk + head) * d;
+        const int64_t base = (un.page * hk + head) * a.c.page_size + un.slot;
+        const uint8_t *codes = (kv ? a.c.v : a.c.k) + (base + un.lo) * d;
+        const float s = __ldg((kv ? a.c.v_scale : a.c.k_scale) + base / blk);
+        for (int i0 = threadIdx.x; i0 < nv; i0 += 4 * blockDim.x) {
+            uint2 c[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int i = i0 + j * blockDim.x;
+                if (i < nv) c[j] = __ldg(reinterpret_cast<const uint2 *>(codes) + i);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int i = i0 + j * blockDim.x;
+                if (i < nv) {
+                    float f[8];
+                    e4m3x2_decode(c[j].x & 0xffffu, f[0], f[1]);
+                    e4m3x2_decode(c[j].x >> 16, f[2], f[3]);
+                    e4m3x2_decode(c[j].y & 0xffffu, f[4], f[5]);
+                    e4m3x2_decode(c[j].y >> 16, f[6], f[7]);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) f[e] *= s;
+                    store_vec<T, 8>(y + static_cast<int64_t>(i >> shift) * hk * d + ((i & (per_row - 1)) << 3), f);
+                }
+            }
+        }
+    }
+}
+
+// grid.x: units; grid.y: how many CTAs share a unit's 2 * kv_heads items.
+// Enough CTAs to fill the machine a few times over when the units alone do
+// not; otherwise one CTA per unit, which pays the look-ups once.
+dim3 unit_grid(const lcml_kv_cache *c, const lcml_kv_batch *b) {
+    const int64_t units = b->total_tokens / c->scale_block + 2 * static_cast<int64_t>(b->batch);
+    const int64_t want = 8 * static_cast<int64_t>(sm_count());
+    int64_t y = (want + units - 1) / units;
+    if (y > 2 * c->kv_heads) y = 2 * c->kv_heads;
+    return dim3(static_cast<unsigned>(units), static_cast<unsigned>(y < 1 ? 1 : y));
+}
+
+unsigned unit_threads(const lcml_kv_cache *c) { return static_cast<unsigned>(c->scale_block * c->head_dim / (8 * kVpt)); }
+
+template <typename T>
+int launch_write(const lcml_kv_cache *c, const lcml_kv_batch *b, const WriteArgs &a, bool vec, cudaStream_t st) {
+    return launch_dependent(vec ? k_kv_cache_write<T, true> : k_kv_cache_write<T, false>, unit_grid(c, b), unit_threads(c), 0, st,
+                            "kv_cache_write", a);
+}
+
+}// namespace
+}// namespace lcml
+
+using namespace lcml;
+
+extern "C" {
+
+int lcml_kv_cache_write(const lcml_kv_cache *cache, const lcml_kv_batch *batch, const void *k, int64_t k_token_stride,
+                        int64_t k_head_stride, const void *v, int64_t v_token_stride, int64_t v_head_stride, int dtype,
+                        lcml_stream_t stream) {
+    int rc = check_cache(cache, "lcml_kv_cache_write");
+    if (rc == LCML_OK) rc = check_batch(batch, "lcml_kv_cache_write");
+    if (rc != LCML_OK) return rc;
+    LCML_CHECK_ARG(dtype == LCML_DTYPE_FLOAT || dtype == LCML_DTYPE_FLOAT16 || dtype == LCML_DTYPE_BFLOAT16,
+                   "lcml_kv_cache_write: dtype %d unsupported", dtype);
+    if (batch->batch == 0 || batch->total_tokens == 0) return LCML_OK;
+    LCML_CHECK_ARG(k && v, "lcml_kv_cache_write: null pointer");
+    LCML_CHECK_ARG(k_token_stride >= 0 && k_head_stride >= 0 && v_token_stride >= 0 && v_head_stride >= 0,
+                   "lcml_kv_cache_write: negative stride");
+    const int64_t es = dtype == LCML_DTYPE_FLOAT ? 4 : 2;
+    LCML_CHECK_ARG(aligned(k, es) && aligned(v, es), "lcml_kv_cache_write: k or v is not aligned to its element size");
+    const int64_t e16 = 16 / es;
+    const bool vec = aligned(k, 16) && aligned(v, 16) && k_token_stride % e16 == 0 && k_head_stride % e16 == 0 &&
+                     v_token_stride % e16 == 0 && v_head_stride % e16 == 0;
+    const WriteArgs a{*cache, *batch, {k, v}, {k_token_stride, v_token_stride}, {k_head_stride, v_head_stride}, device_error_word()};
+    cudaStream_t st = to_cuda(stream);
+    if (dtype == LCML_DTYPE_FLOAT) return launch_write<float>(cache, batch, a, vec, st);
+    if (dtype == LCML_DTYPE_FLOAT16) return launch_write<__half>(cache, batch, a, vec, st);
+    return launch_write<__nv_bfloat16>(cache, batch, a, vec, st);
+}
+
+int lcml_kv_cache_read(const lcml_kv_cache *cache, const lcml_kv_batch *batch, void *k, void *v, int dtype,
+                       lcml_stream_t stream) {
+    int rc = check_cache(cache, "lcml_kv_cache_read");
+    if (rc == LCML_OK) rc = check_batch(batch, "lcml_kv_cache_read");
+    if (rc != LCML_OK) return rc;
+    LCML_CHECK_ARG(dtype == LCML_DTYPE_FLOAT || dtype == LCML_DTYPE_FLOAT16 || dtype == LCML_DTYPE_BFLOAT16,
+                   "lcml_kv_cache_read: dtype %d unsupported", dtype);
+    if (batch->batch == 0 || batch->total_tokens == 0) return LCML_OK;
+    LCML_CHECK_ARG(k || v, "lcml_kv_cache_read: null pointers");
+    LCML_CHECK_ARG(aligned(k, 16) && aligned(v, 16), "lcml_kv_cache_read: k and v must be 16-byte aligned");
+    const ReadArgs a{*cache, *batch, {k, v}, device_error_word()};
+    cudaStream_t st = to_cuda(stream);
+    const dim3 grid = unit_grid(cache, batch);
+    const unsigned threads = unit_threads(cache);
+    if (dtype == LCML_DTYPE_FLOAT) return launch_dependent(k_kv_cache_read<float>, grid, threads, 0, st, "kv_cache_read", a);
+    if (dtype == LCML_DTYPE_FLOAT16) return launch_dependent(k_kv_cache_read<__half>, grid, threads, 0, st, "kv_cache_read", a);
+    return launch_dependent(k_kv_cache_read<__nv_bfloat16>, grid, threads, 0, st, "kv_cache_read", a);
+}
+
+}// extern "C"

@@ -1,0 +1,233 @@
+// RMS norm with the residual's addition and an e4m3 output
+// (lcml_rmsnorm_quantize).
+//
+// One CTA per row; the row stays in registers as h * w between the reduction
+// and the quantization, so x and the residual are read once. With
+//   y = h w r,  r = 1 / sqrt(mean(h^2) + eps) > 0,
+// max|y| = r max|h w|, so the sum of squares and the maximum are reduced
+// together: one block reduction per row, not two.
+//
+// Bound: HBM (x + residual + h + 1 byte per element) for many rows, the
+// latency of one load, one block reduction and one store for few.
+#include "lcml_decoder.cuh"
+
+namespace lcml {
+namespace {
+
+struct NormArgs {
+    int64_t cols, ldx, ldr, ldh;
+    const void *x, *residual;
+    void *h_out;
+    const void *weight;
+    float eps;
+    const float *scale;
+    float *scale_out;
+    uint8_t *q;
+};
+
+// Block-wide (sum, max): every thread gets both.
+__device__ __forceinline__ void block_sum_max(float &sum, uint32_t &mx) {
+    __shared__ float red_s[32];
+    __shared__ uint32_t red_m[32];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    }
+    const int w = threadIdx.x >> 5, l = threadIdx.x & 31, nw = blockDim.x >> 5;
+    if (nw == 1) return;
+    if (l == 0) {
+        red_s[w] = sum;
+        red_m[w] = mx;
+    }
+    __syncthreads();
+    sum = l < nw ? red_s[l] : 0.0f;
+    mx = l < nw ? red_m[l] : 0u;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    }
+}
+
+// E elements per access (E = 1: rows of any alignment), VPT accesses per
+// thread: cols <= E * VPT * blockDim.x.
+template <typename T, typename W, int E, int VPT>
+__global__ void __launch_bounds__(1024) k_rmsnorm_quantize(NormArgs a) {
+    griddep_launch_dependents();  // the GEMM behind may start its set-up
+    const int64_t row = blockIdx.x;
+    const int nv = static_cast<int>(a.cols / E);
+    float v[VPT * E];
+    griddep_wait();
+    const T *x = static_cast<const T *>(a.x) + row * a.ldx;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        const int i = threadIdx.x + j * blockDim.x;
+        if (i < nv) load_vec<T, E>(x + static_cast<int64_t>(i) * E, v + j * E);
+    }
+    if (a.residual != nullptr) {
+        const T *r = static_cast<const T *>(a.residual) + row * a.ldr;
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const int i = threadIdx.x + j * blockDim.x;
+            float t[E];
+            if (i < nv) {
+                load_vec<T, E>(r + static_cast<int64_t>(i) * E, t);
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[j * E + e] += t[e];
+            }
+        }
+    }
+    float sum = 0.0f;
+    uint32_t mx = 0;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        const int i = threadIdx.x + j * blockDim.x;
+        if (i < nv) {
+            if (a.h_out != nullptr)
+                store_vec<T, E>(static_cast<T *>(a.h_out) + row * a.ldh + static_cast<int64_t>(i) * E, v + j * E);
+            float w[E];
+            load_vec<W, E>(static_cast<const W *>(a.weight) + static_cast<int64_t>(i) * E, w);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int k = j * E + e;
+                sum = fmaf(v[k], v[k], sum);
+                v[k] *= w[e];
+                mx = max(mx, abs_bits_nan0(v[k]));
+            }
+        }
+    }
+    block_sum_max(sum, mx);
+    const float r = rsqrtf(sum / static_cast<float>(a.cols) + a.eps);
+    const float s = a.scale != nullptr ? __ldg(a.scale) : scale_from_amax(__uint_as_float(mx) * r);
+    if (a.scale_out != nullptr && threadIdx.x == 0) a.scale_out[row] = s;
+    const float rs = __frcp_rn(s);
+    const bool ok = scale_fast_ok(s, rs);
+    uint8_t *q = a.q + row * a.cols;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        const int i = threadIdx.x + j * blockDim.x;
+        if (i < nv) {
+            float y[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) y[e] = v[j * E + e] * r;
+            if constexpr (E == 1) {
+                q[i] = static_cast<uint8_t>(quantize2_fast(y[0], y[0], s, rs, ok));
+            } else {
+                uint32_t c[E / 4];
+                quantize_block_fast<E>(y, s, rs, ok, c);
+                if constexpr (E == 8) *reinterpret_cast<uint2 *>(q + static_cast<int64_t>(i) * 8) = make_uint2(c[0], c[1]);
+                else *reinterpret_cast<uint32_t *>(q + static_cast<int64_t>(i) * 4) = c[0];
+            }
+        }
+    }
+}
+
+// Rows too long for the registers of one CTA: three passes over the row (the
+// second and third mostly from L1 / L2). h_out may alias x or residual, so h
+// is written in the last pass.
+template <typename T, typename W>
+__global__ void __launch_bounds__(1024) k_rmsnorm_quantize_long(NormArgs a) {
+    griddep_launch_dependents();
+    griddep_wait();
+    const int64_t row = blockIdx.x;
+    const T *x = static_cast<const T *>(a.x) + row * a.ldx;
+    const T *rp = a.residual != nullptr ? static_cast<const T *>(a.residual) + row * a.ldr : nullptr;
+    const W *w = static_cast<const W *>(a.weight);
+    auto h = [&](int64_t c) { return Elem<T>::load(x + c) + (rp != nullptr ? Elem<T>::load(rp + c) : 0.0f); };
+    float sum = 0.0f;
+    uint32_t mx = 0;
+    for (int64_t c = threadIdx.x; c < a.cols; c += blockDim.x) {
+        const float v = h(c);
+        sum = fmaf(v, v, sum);
+        mx = max(mx, abs_bits_nan0(v * Elem<W>::load(w + c)));
+    }
+    block_sum_max(sum, mx);
+    const float r = rsqrtf(sum / static_cast<float>(a.cols) + a.eps);
+    const float s = a.scale != nullptr ? __ldg(a.scale) : scale_from_amax(__uint_as_float(mx) * r);
+    if (a.scale_out != nullptr && threadIdx.x == 0) a.scale_out[row] = s;
+    for (int64_t c = threadIdx.x; c < a.cols; c += blockDim.x) {
+        const float v = h(c);
+        a.q[row * a.cols + c] = static_cast<uint8_t>(quantize1(v * Elem<W>::load(w + c) * r, s));
+        if (a.h_out != nullptr) static_cast<T *>(a.h_out)[row * a.ldh + c] = Elem<T>::from(v);
+    }
+}
+
+template <typename T, typename W, int E>
+int launch_norm(const lcml_rmsnorm_desc *d, const NormArgs &a, cudaStream_t st) {
+    const dim3 grid(static_cast<unsigned>(d->rows));
+    const int64_t nv = d->cols / E;
+    // Few rows: one access per thread, the shortest chain from load to store.
+    // Many rows: more accesses in flight per thread and smaller reductions.
+    const int want = d->rows <= 2 * sm_count() ? 1024 : 256;
+    constexpr int kMost = E == 1 ? 16 : (E * static_cast<int>(sizeof(T)) == 16 ? 4 : 8);
+    int vpt = 1;
+    while (vpt < kMost && nv > static_cast<int64_t>(vpt) * want) vpt *= 2;
+    int64_t threads = ((nv + vpt - 1) / vpt + 31) / 32 * 32;
+    if (threads > 1024) {
+        return launch_dependent(k_rmsnorm_quantize_long<T, W>, grid, 1024, 0, st, "rmsnorm_quantize_long", a);
+    }
+    void (*kern)(NormArgs) = nullptr;
+    switch (vpt) {
+        case 1: kern = k_rmsnorm_quantize<T, W, E, 1>; break;
+        case 2: kern = k_rmsnorm_quantize<T, W, E, 2>; break;
+        case 4: kern = k_rmsnorm_quantize<T, W, E, 4>; break;
+        case 8:
+            if constexpr (kMost >= 8) kern = k_rmsnorm_quantize<T, W, E, 8>;
+            break;
+        case 16:
+            if constexpr (kMost >= 16) kern = k_rmsnorm_quantize<T, W, E, 16>;
+            break;
+    }
+    return launch_dependent(kern, grid, static_cast<unsigned>(threads), 0, st, "rmsnorm_quantize", a);
+}
+
+template <typename T, typename W>
+int dispatch_norm(const lcml_rmsnorm_desc *d, const NormArgs &a, cudaStream_t st) {
+    auto fits = [&](int e) {
+        const int64_t b = static_cast<int64_t>(e) * static_cast<int64_t>(sizeof(T));
+        const uintptr_t al = static_cast<uintptr_t>(b < 16 ? b : 16);
+        return d->cols % e == 0 && d->ldx % e == 0 && aligned(d->x, al) && (!d->residual || (d->ldr % e == 0 && aligned(d->residual, al))) &&
+               (!d->h_out || (d->ldh % e == 0 && aligned(d->h_out, al))) && aligned(d->weight, e * sizeof(W) < 16 ? e * sizeof(W) : 16) &&
+               aligned(d->q, static_cast<uintptr_t>(e));
+    };
+    if constexpr (sizeof(T) == 2) {
+        if (fits(8)) return launch_norm<T, W, 8>(d, a, st);
+    }
+    if (fits(4)) return launch_norm<T, W, 4>(d, a, st);
+    return launch_norm<T, W, 1>(d, a, st);
+}
+
+}// namespace
+}// namespace lcml
+
+using namespace lcml;
+
+extern "C" int lcml_rmsnorm_quantize(const lcml_rmsnorm_desc *d, lcml_stream_t stream) {
+    LCML_CHECK_ARG(d != nullptr, "lcml_rmsnorm_quantize: null descriptor");
+    LCML_CHECK_ARG(d->rows >= 0 && d->cols >= 0, "lcml_rmsnorm_quantize: negative extent");
+    LCML_CHECK_ARG(d->x_dtype == LCML_DTYPE_FLOAT || d->x_dtype == LCML_DTYPE_FLOAT16 || d->x_dtype == LCML_DTYPE_BFLOAT16,
+                   "lcml_rmsnorm_quantize: x_dtype %d unsupported", d->x_dtype);
+    LCML_CHECK_ARG(d->weight_dtype == d->x_dtype || d->weight_dtype == LCML_DTYPE_FLOAT,
+                   "lcml_rmsnorm_quantize: weight_dtype %d is neither x's type nor FLOAT", d->weight_dtype);
+    LCML_CHECK_ARG(d->eps >= 0.0f, "lcml_rmsnorm_quantize: eps is negative or NaN");
+    if (d->rows == 0 || d->cols == 0) return LCML_OK;
+    LCML_CHECK_ARG((d->scale != nullptr) != (d->scale_out != nullptr),
+                   "lcml_rmsnorm_quantize: give exactly one of scale and scale_out");
+    LCML_CHECK_ARG(d->x && d->weight && d->q, "lcml_rmsnorm_quantize: null pointer");
+    LCML_CHECK_ARG(d->rows <= 0x7fffffff && d->cols <= 0x7fffffff, "lcml_rmsnorm_quantize: extent over 2^31 - 1");
+    LCML_CHECK_ARG(d->ldx >= d->cols && (!d->residual || d->ldr >= d->cols) && (!d->h_out || d->ldh >= d->cols),
+                   "lcml_rmsnorm_quantize: a row stride is less than cols %lld", (long long)d->cols);
+    const uintptr_t es = d->x_dtype == LCML_DTYPE_FLOAT ? 4 : 2, ws = d->weight_dtype == LCML_DTYPE_FLOAT ? 4 : 2;
+    LCML_CHECK_ARG(aligned(d->x, es) && (!d->residual || aligned(d->residual, es)) && (!d->h_out || aligned(d->h_out, es)) &&
+                       aligned(d->weight, ws) && (!d->scale || aligned(d->scale, 4)) && (!d->scale_out || aligned(d->scale_out, 4)),
+                   "lcml_rmsnorm_quantize: a pointer is not aligned to its element size");
+    const NormArgs a{d->cols, d->ldx, d->ldr, d->ldh, d->x, d->residual, d->h_out, d->weight, d->eps, d->scale, d->scale_out, d->q};
+    cudaStream_t st = to_cuda(stream);
+    const bool wf = d->weight_dtype == LCML_DTYPE_FLOAT;
+    switch (d->x_dtype) {
+        case LCML_DTYPE_FLOAT: return dispatch_norm<float, float>(d, a, st);
+        case LCML_DTYPE_FLOAT16: return wf ? dispatch_norm<__half, float>(d, a, st) : dispatch_norm<__half, __half>(d, a, st);
+        default: return wf ? dispatch_norm<__nv_bfloat16, float>(d, a, st) : dispatch_norm<__nv_bfloat16, __nv_bfloat16>(d, a, st);
+    }
+}
