@@ -31,6 +31,7 @@ constexpr int kRows = 16;          // rows per tile
 constexpr int kStep = 16;          // keys per warp step
 constexpr int kMinChunk = 64;      // steps: below this a split costs more than it gains
 constexpr int kTargetPerSm = 2;
+constexpr int kTcRows = 128;       // rows of a sequence from which the tensor-core kernel takes it
 
 template <int D>
 struct Shape {
@@ -764,7 +765,19 @@ int lcml_kv_attention(const lcml_kv_attention_desc *d, lcml_stream_t stream) {
                d->softcap,        d->softcap > 0.0f ? d->softmax_scale / d->softcap : 0.0f, d->window,
                d->causal ? 1 : 0, d->max_tokens,      device_error_word()};
     cudaStream_t st = to_cuda(stream);
-    const int max_rows = 0x7fffffff;
+    // Rows a sequence must have for the tensor-core kernel; the streaming
+    // kernel takes the others. One launch where the bound or the variant says
+    // that one kernel serves every sequence.
+    const bool fits = kv_attention_tc_fits(d);
+    LCML_CHECK_ARG(d->variant != 2 || fits, "lcml_kv_attention: variant 2 does not serve this call");
+    const int64_t most = (d->max_tokens < d->batch->total_tokens ? d->max_tokens : d->batch->total_tokens) * a.group;
+    int min_rows = fits && d->variant != 1 ? (d->variant == 2 ? 0 : kTcRows) : 0x7fffffff;
+    if (most < min_rows) min_rows = 0x7fffffff;
+    if (min_rows != 0x7fffffff) {
+        const int rc2 = kv_attention_tc(d, a, min_rows, st);
+        if (rc2 != LCML_OK || min_rows == 0 || d->batch->batch == 1) return rc2;
+    }
+    const int max_rows = min_rows == 0x7fffffff ? min_rows : min_rows - 1;
     switch (d->cache->head_dim) {
         case 64: return launch_stream<64>(d, a, max_rows, st);
         case 128: return launch_stream<128>(d, a, max_rows, st);

@@ -1,0 +1,717 @@
+// Attention over the paged e4m3 cache: the tensor-core kernel for long runs of
+// queries (prompts and chunks).
+//
+// One CTA per (sequence, cache head, 256 rows), rows = query * group + head as
+// in kv_attention.cu, as two tiles of 128 rows that share every key and value
+// tile of 128 tokens. Per tile t and key tile j:
+//   S_t = sum over parts p of Q_t,p K_j^T    tcgen05 kind::f8f6f4, fp32 in TMEM
+//   P_t = 2^(S_t scale + log2 s_v - m)       one thread per row, halves in TMEM over S_t
+//   O_t += P_t V_j                           tcgen05 kind::f16, A from TMEM
+// Keys go from global memory to the MMA as they are: a row of q, times a power
+// of two, is split into e4m3 parts hi + lo (+ lo2) whose sum is q exactly (a
+// bf16 has 8 significant bits, two e4m3 parts with 4 each and a sign carry
+// them; an fp16 takes three), down to 2^-17 of the row's largest element. Two
+// e4m3 products cost what one 16-bit product does, and no key is converted.
+// Values are converted to halves (exact) by one warpgroup, from global memory
+// into the MN-major 128-byte-swizzled layout of the B operand: the weights
+// need more range than e4m3 has.
+//
+// Roles (16 warps): 0-3 and 4-7 softmax of tile 0 and 1 (a row per thread, no
+// shuffles), 8-11 value conversion, 12 look-ups and TMA of the keys, 13 MMA
+// issue. The MMA order PV_0(j) QK_0(j+1) PV_1(j) QK_1(j+1) lets one tile's
+// softmax run under the other's products.
+//
+// Bound: the tensor cores (4 head_dim FLOP per visible pair) and the
+// exponentials, 16 a clock per SM: equal at head_dim 128, twice the products'
+// time at 64.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <cstring>
+#include <mutex>
+
+#include "lcml_attention.cuh"
+
+namespace lcml {
+namespace {
+
+constexpr int kTile = 128;                // rows per tile, keys per tile
+constexpr int kBlockRows = 2 * kTile;     // rows per CTA
+constexpr int kThreads = 512;
+constexpr int kGroups = kTile / 16;       // 16-token groups of a key tile: one pair of scales each
+constexpr int kInfoStages = 4;
+constexpr int kVStages = 2;
+
+// Registers per thread by role; 256 * 192 + 128 * 80 + 128 * 48 = 512 * 128,
+// the block's allocation at launch.
+constexpr int kSoftmaxRegs = 192, kConvertRegs = 80, kOtherRegs = 48;
+
+struct alignas(16) GroupInfo {
+    float k_scale, log2_v, inv_v;
+    int row;  // cache row of the group's first token, -1: no token
+};
+
+template <int D, int NP>
+struct Shape {
+    static constexpr int kKStages = NP == 2 ? 3 : 2;
+    static constexpr int kQPart = kTile * D;              // one part of one tile
+    static constexpr int kQ = 2 * NP * kQPart;
+    static constexpr int kK = kTile * D;                  // one stage
+    static constexpr int kV = kTile * D * 2;              // one stage, halves
+    static constexpr int kOffK = kQ;
+    static constexpr int kOffV = kOffK + kKStages * kK;
+    static constexpr int kSmem = kOffV + kVStages * kV + 1024;  // + alignment of the base
+};
+
+struct Shared {
+    uint64_t k_full[3], k_empty[3], v_full[kVStages], v_empty[kVStages], info_full[kInfoStages], info_empty[kInfoStages];
+    uint64_t s_full[2], p_full[2], o_full[2];
+    uint32_t tmem;
+    int nan_seen;
+    GroupInfo info[kInfoStages][kGroups];
+    float row_factor[kBlockRows];
+};
+
+template <int N>
+__device__ __forceinline__ void reg_inc() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void reg_dec() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// D[tmem] (+)= A[tmem] * B[smem], halves -> f32.
+__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+        "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
+        "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// B operand of P V: [token][d] with d contiguous (MN-major), halves, 128-byte
+// swizzle: blocks of 64 d (128-byte rows, one per token, 8-token groups 1024
+// bytes apart: the stride of K) of kTile tokens each (16 KiB apart: the stride
+// of N).
+__device__ __forceinline__ uint64_t sdesc_v(uint32_t smem_addr) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((smem_addr & 0x3ffffu) >> 4);
+    d |= static_cast<uint64_t>((kTile * 128) >> 4) << 16;
+    d |= static_cast<uint64_t>(1024u >> 4) << 32;
+    d |= static_cast<uint64_t>(1u) << 46;
+    d |= static_cast<uint64_t>(2u) << 61;
+    return d;
+}
+
+// kind::f16 with fp16 A and B, f32 D, A K-major, B MN-major.
+constexpr uint32_t idesc_f16(uint32_t m, uint32_t n) { return (1u << 4) | (1u << 16) | ((n >> 3) << 17) | ((m >> 4) << 24); }
+
+// Byte offset of 16-byte chunk `chunk` of row `row` in a K-major tile of
+// D-byte rows with the D-byte swizzle (D = 128: chunk ^ row % 8, 64: chunk ^
+// row / 2 % 4).
+template <int D>
+__device__ __forceinline__ uint32_t kmajor_offset(int row, int chunk) {
+    return D == 128 ? row * 128 + ((chunk ^ (row & 7)) << 4) : row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
+}
+
+// The CTA's work, known to every thread.
+struct Work {
+    int seq, head, rows;      // rows in this block (<= kBlockRows)
+    int row0;                 // first row within the sequence
+    int t0, n, len, pos0;     // packed first token, queries, tokens held, position of query 0
+    int tile_lo, tiles;       // first key tile and how many
+};
+
+template <int D, int NP, bool CAP>
+__global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_constant__ CUtensorMap k_map, AttnArgs a, int box_rows,
+                                                                 int min_rows) {
+    using S = Shape<D, NP>;
+    extern __shared__ uint8_t raw[];
+    __shared__ Shared sh;
+    const uint32_t smem = (smem_u32(raw) + 1023u) & ~1023u;
+
+    griddep_launch_dependents();
+    griddep_wait();
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    // Units are handed out from the last one: within a sequence the last rows
+    // see the most keys, and the longest units should not start last.
+    Work w;
+    {
+        w.head = blockIdx.x % a.c.kv_heads;
+        const int64_t u = (gridDim.x - 1 - blockIdx.x) / a.c.kv_heads;
+        w.seq = find_sequence(a.b.cu_tokens, a.b.batch, u, a.group, kBlockRows, 1);
+        w.t0 = __ldg(a.b.cu_tokens + w.seq);
+        const int t1 = static_cast<int>(min(static_cast<int64_t>(__ldg(a.b.cu_tokens + w.seq + 1)), a.b.total_tokens));
+        const int len = max(0, __ldg(a.b.lengths + w.seq));
+        w.n = w.t0 >= 0 ? max(0, t1 - w.t0) : 0;
+        w.len = static_cast<int>(min(static_cast<int64_t>(len), static_cast<int64_t>(a.b.table_cols) * a.c.page_size));
+        if ((w.len < len || w.n > a.max_tokens) && threadIdx.x == 0) record_device_error(a.err, kDevBadBatch);
+        w.pos0 = w.len - w.n;
+        const int64_t block = u - (static_cast<int64_t>(w.t0) * a.group / kBlockRows + w.seq);
+        const int64_t all = static_cast<int64_t>(w.n) * a.group;
+        if (block * kBlockRows >= all || all < min_rows || w.t0 < 0) return;  // the whole CTA
+        w.row0 = static_cast<int>(block * kBlockRows);
+        w.rows = static_cast<int>(min(static_cast<int64_t>(kBlockRows), all - w.row0));
+        const int qa = w.row0 / a.group, qz = (w.row0 + w.rows - 1) / a.group;
+        const int hi = a.causal ? min(w.pos0 + qz, w.len - 1) : w.len - 1;  // the last key any row sees
+        const int lo = a.window > 0 ? max(0, w.pos0 + qa - a.window + 1) : 0;
+        w.tile_lo = lo / kTile;
+        w.tiles = hi >= lo ? hi / kTile - w.tile_lo + 1 : 0;
+    }
+    const bool two = w.rows > kTile;
+
+    if (warp == 12) {
+        if (lane == 0) {
+            for (int i = 0; i < S::kKStages; ++i) {
+                mbar_init(&sh.k_full[i], 1);
+                mbar_init(&sh.k_empty[i], 1);
+            }
+            for (int i = 0; i < kVStages; ++i) {
+                mbar_init(&sh.v_full[i], 4);
+                mbar_init(&sh.v_empty[i], 1);
+            }
+            for (int i = 0; i < kInfoStages; ++i) {
+                mbar_init(&sh.info_full[i], 1);
+                mbar_init(&sh.info_empty[i], two ? 12 : 8);
+            }
+            for (int i = 0; i < 2; ++i) {
+                mbar_init(&sh.s_full[i], 1);
+                mbar_init(&sh.p_full[i], 4);
+                mbar_init(&sh.o_full[i], 1);
+            }
+            sh.nan_seen = 0;
+            fence_mbar_init();
+        }
+        tma_prefetch_desc(&k_map);
+    }
+    if (warp == 13) {
+        tmem_alloc(&sh.tmem, 512);
+        tmem_relinquish();
+    }
+
+    // Q -> e4m3 parts. A lane takes 4 elements of a row: 32 lanes a row at
+    // head_dim 128, 16 at 64. Rows past the block's end are zeros.
+    {
+        constexpr int LPR = D / 4, RPW = 32 / LPR;
+        const int part_lane = lane % LPR;
+        const bool vec = aligned(a.q, 8) && a.q_token_stride % 4 == 0 && a.q_head_stride % 4 == 0;
+        const int most = two ? kBlockRows : kTile;
+        for (int r = warp * RPW + lane / LPR; r < most; r += (kThreads / 32) * RPW) {
+            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (r < w.rows) {
+                const int row = w.row0 + r;
+                const int64_t off = (w.t0 + static_cast<int64_t>(row / a.group)) * a.q_token_stride +
+                                    (static_cast<int64_t>(w.head) * a.group + row % a.group) * a.q_head_stride + part_lane * 4;
+                uint16_t e[4];
+                const uint16_t *p = static_cast<const uint16_t *>(a.q) + off;
+                if (vec) {
+                    const uint2 t = __ldg(reinterpret_cast<const uint2 *>(p));
+                    memcpy(e, &t, 8);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) e[i] = p[i];
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    v[i] = a.bf16 ? __uint_as_float(static_cast<uint32_t>(e[i]) << 16) : __half2float(__ushort_as_half(e[i]));
+            }
+            uint32_t mx = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx = max(mx, abs_bits_nan0(v[i]));
+#pragma unroll
+            for (int o = LPR / 2; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            // times 2^(7 - e): the largest element comes to [128, 256); infinities stay (and saturate)
+            int e = static_cast<int>(mx >> 23);
+            e = mx == 0 ? 127 : min(max(e, 8), 253);
+            const float up = __uint_as_float(static_cast<uint32_t>(254 - e) << 23) * 128.0f;
+            if (part_lane == 0) sh.row_factor[r] = __uint_as_float(static_cast<uint32_t>(e) << 23) * 0.0078125f;
+            bool special = false;
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[i] = v[i] * up;
+                special |= !(fabsf(x[i]) < INFINITY);
+            }
+            const int t = r >> 7, tr = r & 127;
+#pragma unroll
+            for (int p = 0; p < NP; ++p) {
+                uint32_t c = cvt_e4m3x2(x[0], x[1]) | (cvt_e4m3x2(x[2], x[3]) << 16);
+                if (special) c = 0x7f7f7f7fu;  // a row with an infinity or NaN has NaN scores
+                const uint32_t at = smem + (t * NP + p) * S::kQPart + kmajor_offset<D>(tr, part_lane >> 2) + (part_lane & 3) * 4;
+                asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(c) : "memory");
+                if (p + 1 < NP) {
+                    float f[4];
+                    e4m3x2_decode(c & 0xffffu, f[0], f[1]);
+                    e4m3x2_decode(c >> 16, f[2], f[3]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i] -= f[i];
+                }
+            }
+        }
+        fence_proxy_async_smem();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;
+    const int n = w.tiles;
+
+    if (warp >= 12) {
+        reg_dec<kOtherRegs>();
+        if (warp == 12) {
+            // Look-ups run two tiles ahead of their use: table entries for
+            // j + 2 and scales for j + 1 are in flight while j is published.
+            const int32_t *table = a.b.block_table + w.seq * a.b.table_stride;
+            auto entry = [&](int j) -> int {  // page of group `lane` of tile j, -1: none
+                const int64_t pos = static_cast<int64_t>(w.tile_lo + j) * kTile + lane * 16;
+                if (lane >= kGroups || j >= n || pos >= w.len) return -1;
+                return __ldg(table + pos / a.c.page_size);
+            };
+            auto row_of = [&](int j, int page) -> int {
+                const int64_t pos = static_cast<int64_t>(w.tile_lo + j) * kTile + lane * 16;
+                if (lane >= kGroups || j >= n || pos >= w.len) return -1;
+                if (page < 0 || page >= a.c.num_pages) {
+                    record_device_error(a.err, kDevBadPage);
+                    return -1;
+                }
+                return static_cast<int>((static_cast<int64_t>(page) * a.c.kv_heads + w.head) * a.c.page_size + pos % a.c.page_size);
+            };
+            int row = row_of(0, entry(0));
+            float ks = row >= 0 ? __ldg(a.c.k_scale + row / a.c.scale_block) : 0.0f, vs = row >= 0 ? __ldg(a.c.v_scale + row / a.c.scale_block) : 1.0f;
+            int next_page = entry(1);
+            const int groups_per_box = box_rows / 16;
+            int issued = 0;
+            for (int j = 0; j < n; ++j) {
+                const int later_page = entry(j + 2);
+                const int next_row = row_of(j + 1, next_page);
+                float next_ks = 0.0f, next_vs = 1.0f;
+                if (next_row >= 0) {
+                    next_ks = __ldg(a.c.k_scale + next_row / a.c.scale_block);
+                    next_vs = __ldg(a.c.v_scale + next_row / a.c.scale_block);
+                }
+                const int st = j % kInfoStages;
+                if (!__all_sync(0xffffffffu, mbar_wait(&sh.info_empty[st], ((j / kInfoStages) & 1) ^ 1, a.err, kDevTimeoutProducer))) break;
+                if (lane < kGroups) {
+                    const float sv = value_scale(vs);
+                    sh.info[st][lane] = GroupInfo{row >= 0 ? ks : 0.0f, __log2f(sv), __fdividef(1.0f, sv), row};
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.info_full[st]);
+                const int kst = j % S::kKStages;
+                if (!__all_sync(0xffffffffu, mbar_wait(&sh.k_empty[kst], ((j / S::kKStages) & 1) ^ 1, a.err, kDevTimeoutProducer))) break;
+                const bool lead = lane < kGroups && lane % groups_per_box == 0 && row >= 0;  // a box's first group has a token
+                const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, lead));
+                if (lane == 0) mbar_arrive_expect_tx(&sh.k_full[kst], boxes * box_rows * D);
+                __syncwarp();
+                if (lead)
+                    asm volatile(
+                        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
+                            smem + S::kOffK + kst * S::kK + lane * 16 * D),
+                        "l"(&k_map), "r"(smem_u32(&sh.k_full[kst])), "r"(0), "r"(row)
+                        : "memory");
+                issued = j + 1;
+                row = next_row;
+                ks = next_ks;
+                vs = next_vs;
+                next_page = later_page;
+            }
+            // no copy is in flight when the CTA ends (only a given-up wait leaves any)
+            for (int j = max(0, issued - S::kKStages); j < issued; ++j)
+                mbar_wait(&sh.k_full[j % S::kKStages], (j / S::kKStages) & 1, a.err, kDevTimeoutDrain);
+        } else if (warp == 13 && lane == 0 && n > 0) {
+            constexpr uint32_t kIdescS = idesc_e4m3_f32(kTile, kTile, 0), kIdescO = idesc_f16(kTile, D);
+            auto qk = [&](int t, int j) {
+                const uint32_t kb = smem + S::kOffK + (j % S::kKStages) * S::kK;
+#pragma unroll
+                for (int p = 0; p < NP; ++p)
+#pragma unroll
+                    for (int k = 0; k < D / 32; ++k)
+                        umma_f8f6f4(tmem + t * kTile, sdesc_kmajor<D>(smem + (t * NP + p) * S::kQPart + k * 32), sdesc_kmajor<D>(kb + k * 32), kIdescS,
+                                    p + k > 0);
+                umma_commit(&sh.s_full[t]);
+            };
+            bool ok = mbar_wait(&sh.k_full[0], 0, a.err, kDevTimeoutMma);
+            tc_fence_after();
+            if (ok) {
+                qk(0, 0);
+                if (two) qk(1, 0);
+                umma_commit(&sh.k_empty[0]);
+            }
+            for (int j = 0; j < n && ok; ++j) {
+                const int vst = j % kVStages;
+                const uint32_t vb = smem + S::kOffV + vst * S::kV;
+                ok = mbar_wait(&sh.v_full[vst], (j / kVStages) & 1, a.err, kDevTimeoutMma);
+                for (int t = 0; t < (two ? 2 : 1) && ok; ++t) {
+                    ok = mbar_wait(&sh.p_full[t], j & 1, a.err, kDevTimeoutMma);
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int k = 0; k < kTile / 16; ++k)
+                        umma_f16_ts(tmem + 2 * kTile + t * D, tmem + t * kTile + k * 8, sdesc_v(vb + k * 2048), kIdescO, j > 0 || k > 0);
+                    const bool last_tile = t == (two ? 1 : 0);
+                    if (last_tile) umma_commit(&sh.v_empty[vst]);
+                    if (j + 1 < n) {
+                        const int kst = (j + 1) % S::kKStages;
+                        if (t == 0) ok = mbar_wait(&sh.k_full[kst], ((j + 1) / S::kKStages) & 1, a.err, kDevTimeoutMma);
+                        if (!ok) break;
+                        tc_fence_after();
+                        qk(t, j + 1);
+                        if (last_tile) umma_commit(&sh.k_empty[kst]);
+                    } else {
+                        umma_commit(&sh.o_full[t]);
+                    }
+                }
+            }
+        }
+    } else if (warp >= 8) {
+        reg_dec<kConvertRegs>();
+        // A thread takes 16 codes of every kRowsPer-th token: global -> two
+        // 16-byte stores of halves, the loads one tile ahead of the stores.
+        constexpr int CH = D / 16;                 // 16-code chunks of a token
+        constexpr int kPer = kTile * CH / 128;     // per thread and tile
+        constexpr int kRowsPer = 128 / CH;         // tokens covered by the warpgroup at once
+        const int wt = threadIdx.x - 256, ch = wt % CH, tok0 = wt / CH;
+        uint4 codes[kPer];
+        auto fetch = [&](int j) -> bool {
+            const int st = j % kInfoStages;
+            if (!__all_sync(0xffffffffu, mbar_wait(&sh.info_full[st], (j / kInfoStages) & 1, a.err, kDevTimeoutProducer))) return false;
+            const int64_t base = static_cast<int64_t>(w.tile_lo + j) * kTile;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const int tok = tok0 + i * kRowsPer;
+                const int row = sh.info[st][tok >> 4].row;
+                codes[i] = make_uint4(0, 0, 0, 0);
+                if (row >= 0 && base + tok < w.len)
+                    codes[i] = __ldg(reinterpret_cast<const uint4 *>(a.c.v + (static_cast<int64_t>(row) + (tok & 15)) * D) + ch);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.info_empty[st]);
+            return true;
+        };
+        bool ok = n > 0 && fetch(0);
+        for (int j = 0; j < n && ok; ++j) {
+            const int vst = j % kVStages;
+            ok = __all_sync(0xffffffffu, mbar_wait(&sh.v_empty[vst], ((j / kVStages) & 1) ^ 1, a.err, kDevTimeoutProducer));
+            if (!ok) break;
+            const uint32_t vb = smem + S::kOffV + vst * S::kV;
+            uint32_t nan = 0;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const uint32_t cw[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
+#pragma unroll
+                for (int q = 0; q < 4; ++q) nan |= (cw[q] & 0x7f7f7f7fu) + 0x01010101u;
+            }
+            if (__any_sync(0xffffffffu, (nan & 0x80808080u) != 0)) {
+                // NaN codes: zeros here, so 0 * NaN reaches no row that does
+                // not see them; the rows that do get theirs at the end
+                sh.nan_seen = 1;
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) {
+                    uint32_t *cw = reinterpret_cast<uint32_t *>(&codes[i]);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) cw[q] &= ~(((((cw[q] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const int tok = tok0 + i * kRowsPer;
+                const uint32_t cw[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
+                uint32_t h[8];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    h[2 * q] = e4m3x2_to_half2(cw[q] & 0xffffu);
+                    h[2 * q + 1] = e4m3x2_to_half2(cw[q] >> 16);
+                }
+                const uint32_t row = vb + (ch >> 2) * (kTile * 128) + tok * 128;
+                // lanes of the second 64 d store their halves in the other order: no two lanes of a
+                // quarter warp meet in a bank
+                const int flip = D == 128 ? ch >> 2 : 0;
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    const int half = s ^ flip;
+                    const uint32_t at = row + ((((ch & 3) * 2 + half) ^ (tok & 7)) << 4);
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(half ? h[4] : h[0]), "r"(half ? h[5] : h[1]),
+                                 "r"(half ? h[6] : h[2]), "r"(half ? h[7] : h[3])
+                                 : "memory");
+                }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.v_full[vst]);
+            if (j + 1 < n) ok = fetch(j + 1);
+        }
+    } else {
+        reg_inc<kSoftmaxRegs>();
+        const int t = warp >> 2;
+        if (t == 0 || two) {
+            const int r = threadIdx.x;  // row of the block
+            const int row = w.row0 + r;
+            const bool live = r < w.rows;  // the others (zero queries) are computed and dropped
+            const int pos = w.pos0 + row / a.group;
+            const int last = a.causal ? min(pos, w.len - 1) : w.len - 1;
+            const int first = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+            const float factor = sh.row_factor[r] * (CAP ? a.inv_cap : a.scale_log2);
+            const uint32_t lane_base = static_cast<uint32_t>(warp & 3) << 21;  // TMEM lanes 32 (warp % 4) ..
+            const uint32_t ts = tmem + lane_base + t * kTile, to = tmem + lane_base + 2 * kTile + t * D;
+            float m = -INFINITY, l = 0.0f;
+            bool ok = true;
+            for (int j = 0; j < n; ++j) {
+                const int st = j % kInfoStages;
+                ok = mbar_wait(&sh.info_full[st], (j / kInfoStages) & 1, a.err, kDevTimeoutEpilogue) &&
+                     mbar_wait(&sh.s_full[t], j & 1, a.err, kDevTimeoutEpilogue);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_fence_after();
+                uint32_t sr[4][32];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) tmem_ld_32x32b_x32(ts + q * 32, sr[q]);
+                tmem_wait_ld();
+                const int base = (w.tile_lo + j) * kTile;
+                const bool whole = __all_sync(0xffffffffu, first <= base && last >= base + kTile - 1);
+                const bool scaled = CAP || !whole;  // scores brought to log2 units element by element
+                float top = -INFINITY;
+                if (!scaled) {
+#pragma unroll
+                    for (int g = 0; g < kGroups; ++g) {
+                        const GroupInfo gi = sh.info[st][g];
+                        float mx = __uint_as_float(sr[g >> 1][(g & 1) * 16]);
+#pragma unroll
+                        for (int e = 1; e < 16; ++e) mx = fmaxf(mx, __uint_as_float(sr[g >> 1][(g & 1) * 16 + e]));
+                        top = fmaxf(top, fmaf(mx, gi.k_scale * factor, gi.log2_v));
+                    }
+                } else {
+#pragma unroll
+                    for (int g = 0; g < kGroups; ++g) {
+                        const GroupInfo gi = sh.info[st][g];
+                        const float f = gi.k_scale * factor;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const int k = base + g * 16 + e;
+                            const float x = __uint_as_float(sr[g >> 1][(g & 1) * 16 + e]);
+                            float y = CAP ? cap_score(x, f, a.cap) + gi.log2_v : fmaf(x, f, gi.log2_v);
+                            y = k >= first && k <= last ? y : -INFINITY;
+                            sr[g >> 1][(g & 1) * 16 + e] = __float_as_uint(y);
+                            top = fmaxf(top, y);
+                        }
+                    }
+                }
+                // The reference maximum moves only when a score passes it by
+                // 2^8: most tiles leave O alone. The S of this tile being full
+                // means that the previous P V is done.
+                if (__any_sync(0xffffffffu, top > m + 8.0f)) {
+                    const float nm = fmaxf(m, top);
+                    const float f = nm == m ? 1.0f : exp2_approx(m - nm);
+                    m = nm;
+                    l *= f;
+                    if (j > 0) {
+#pragma unroll
+                        for (int q = 0; q < D / 32; ++q) {
+                            uint32_t o[32];
+                            tmem_ld_32x32b_x32(to + q * 32, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            tmem_st_32x32b_x32(to + q * 32, o);
+                        }
+                    }
+                }
+                const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    uint32_t p[16];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const GroupInfo gi = sh.info[st][q * 2 + h];
+                        const float f = scaled ? 1.0f : gi.k_scale * factor;
+                        const float b = (scaled ? 0.0f : gi.log2_v) - ref;
+                        float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+                        for (int e = 0; e < 16; e += 2) {
+                            float x0, x1;
+                            fma2(x0, x1, __uint_as_float(sr[q][h * 16 + e]), __uint_as_float(sr[q][h * 16 + e + 1]), f, f, b, b);
+                            x0 = exp2_approx(x0);
+                            x1 = exp2_approx(x1);
+                            s0 += x0;
+                            s1 += x1;
+                            const __half2 hp = __floats2half2_rn(x0, x1);
+                            p[h * 8 + e / 2] = *reinterpret_cast<const uint32_t *>(&hp);
+                        }
+                        l = fmaf(s0 + s1, gi.inv_v, l);
+                    }
+                    tmem_st_32x32b_x16(ts + q * 16, p);
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&sh.p_full[t]);
+                    mbar_arrive(&sh.info_empty[st]);
+                }
+            }
+            if (ok && n > 0) ok = mbar_wait(&sh.o_full[t], 0, a.err, kDevTimeoutEpilogue);
+            ok = __all_sync(0xffffffffu, ok);
+            tc_fence_after();
+            // one row per thread: D halves, 16 bytes at a time where aligned
+            const int64_t token = w.t0 + static_cast<int64_t>(row / a.group);
+            const int qh = w.head * a.group + row % a.group;
+            uint16_t *out = static_cast<uint16_t *>(a.out) + token * a.out_token_stride + qh * a.out_head_stride;
+            const bool vec = aligned(a.out, 16) && a.out_token_stride % 8 == 0 && a.out_head_stride % 8 == 0;
+            const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+            for (int q = 0; q < D / 32; ++q) {
+                uint32_t o[32];
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = 0;
+                if (ok && n > 0) {
+                    tmem_ld_32x32b_x32(to + q * 32, o);
+                    tmem_wait_ld();
+                }
+                uint32_t pk[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float y0 = l != 0.0f ? __uint_as_float(o[2 * e]) * inv : 0.0f, y1 = l != 0.0f ? __uint_as_float(o[2 * e + 1]) * inv : 0.0f;
+                    if (a.bf16) {
+                        const __nv_bfloat162 b = __floats2bfloat162_rn(y0, y1);
+                        pk[e] = *reinterpret_cast<const uint32_t *>(&b);
+                    } else {
+                        const __half2 b = __floats2half2_rn(y0, y1);
+                        pk[e] = *reinterpret_cast<const uint32_t *>(&b);
+                    }
+                }
+                if (vec && live && ok) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) reinterpret_cast<uint4 *>(out + q * 32)[e] = make_uint4(pk[4 * e], pk[4 * e + 1], pk[4 * e + 2], pk[4 * e + 3]);
+                } else if (live && ok) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        out[q * 32 + 2 * e] = static_cast<uint16_t>(pk[e]);
+                        out[q * 32 + 2 * e + 1] = static_cast<uint16_t>(pk[e] >> 16);
+                    }
+                }
+                __syncwarp();
+            }
+            if (live && ok && a.lse != nullptr)
+                a.lse[token * (static_cast<int64_t>(a.c.kv_heads) * a.group) + qh] = l == 0.0f ? -INFINITY : kLn2 * (m + log2f(l));
+        }
+    }
+
+    __syncwarp();  // lane 0 of the MMA warp comes last
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 13) tmem_dealloc(tmem, 512);
+
+    // Values with NaN codes were met (and counted as zeros): give the rows
+    // that see them their NaN, column by column, from the cache itself.
+    if (sh.nan_seen && static_cast<int>(threadIdx.x) < w.rows) {
+        const int row = w.row0 + threadIdx.x;
+        const int pos = w.pos0 + row / a.group;
+        const int last = a.causal ? min(pos, w.len - 1) : w.len - 1, first = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+        const int32_t *table = a.b.block_table + w.seq * a.b.table_stride;
+        uint16_t *out = static_cast<uint16_t *>(a.out) + (w.t0 + static_cast<int64_t>(row / a.group)) * a.out_token_stride +
+                        (w.head * a.group + row % a.group) * a.out_head_stride;
+        for (int k = first; k <= last; ++k) {
+            const int64_t page = __ldg(table + k / a.c.page_size);
+            if (page < 0 || page >= a.c.num_pages) continue;
+            const uint32_t *v = reinterpret_cast<const uint32_t *>(a.c.v + ((page * a.c.kv_heads + w.head) * a.c.page_size + k % a.c.page_size) * D);
+            for (int i = 0; i < D / 4; ++i) {
+                const uint32_t bad = ((__ldg(v + i) & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+                if (bad != 0)
+                    for (int b = 0; b < 4; ++b)
+                        if (bad >> (8 * b + 7) & 1u) out[i * 4 + b] = 0x7fff;  // NaN in both types
+            }
+        }
+    }
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q{};
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    });
+    return fn;
+}
+
+// Key boxes: the largest power of two of tokens that divides a page and a
+// tile, so no box crosses a page.
+int box_rows_of(const lcml_kv_cache *c) {
+    int r = 16;
+    while (r < kTile && c->page_size % (2 * r) == 0) r *= 2;
+    return r;
+}
+
+template <int D, int NP, bool CAP>
+int launch_tc(const lcml_kv_attention_desc *d, const AttnArgs &a, int min_rows, cudaStream_t st) {
+    using S = Shape<D, NP>;
+    auto fn = encode_fn();
+    if (!fn) return set_error(LCML_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    CUtensorMap map;
+    memset(&map, 0, sizeof(map));
+    const int box = box_rows_of(d->cache);
+    cuuint64_t dims[2] = {D, static_cast<cuuint64_t>(d->cache->num_pages) * d->cache->kv_heads * d->cache->page_size};
+    cuuint64_t strides[1] = {D};
+    cuuint32_t bx[2] = {D, static_cast<cuuint32_t>(box)};
+    cuuint32_t es[2] = {1, 1};
+    const CUresult r = fn(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, d->cache->k, dims, strides, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(LCML_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+    auto kern = k_kv_attention_tc<D, NP, CAP>;
+    const int rc = ensure_max_smem(reinterpret_cast<const void *>(kern), S::kSmem, "kv_attention_tc");
+    if (rc != LCML_OK) return rc;
+    const int64_t units = (d->batch->total_tokens * a.group / kBlockRows + d->batch->batch) * d->cache->kv_heads;
+    LCML_CHECK_ARG(units <= 0x7fffffff, "lcml_kv_attention: too much work for one call");
+    return launch_dependent(kern, dim3(static_cast<unsigned>(units)), kThreads, S::kSmem, st, "kv_attention_tc", map, a, box, min_rows);
+}
+
+template <int D>
+int dispatch_tc(const lcml_kv_attention_desc *d, const AttnArgs &a, int min_rows, cudaStream_t st) {
+    if (a.bf16) return a.cap != 0.0f ? launch_tc<D, 2, true>(d, a, min_rows, st) : launch_tc<D, 2, false>(d, a, min_rows, st);
+    return a.cap != 0.0f ? launch_tc<D, 3, true>(d, a, min_rows, st) : launch_tc<D, 3, false>(d, a, min_rows, st);
+}
+
+}// namespace
+
+// Cache rows are 32-bit TMA coordinates; a negative softmax_scale would turn
+// the maximum of a group into its minimum.
+bool kv_attention_tc_fits(const lcml_kv_attention_desc *d) {
+    const lcml_kv_cache *c = d->cache;
+    return (c->head_dim == 64 || c->head_dim == 128) && d->softmax_scale >= 0.0f && c->num_pages > 0 &&
+           c->num_pages * c->kv_heads * c->page_size <= 0x7fffffff;
+}
+
+int kv_attention_tc(const lcml_kv_attention_desc *d, const AttnArgs &a, int min_rows, cudaStream_t st) {
+    return d->cache->head_dim == 64 ? dispatch_tc<64>(d, a, min_rows, st) : dispatch_tc<128>(d, a, min_rows, st);
+}
+
+}// namespace lcml

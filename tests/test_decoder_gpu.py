@@ -385,17 +385,27 @@ def test_decode_split_over_many_chunks(dev, dtype):
     _attend(dev, [1] * 40, [9000] + [37 * i for i in range(39)], 1, 2, 64, 32, 16, dtype)
 
 
-@pytest.mark.parametrize("variant", [0, 1])
+@pytest.mark.parametrize("variant", [0, 1, 2])
 @pytest.mark.parametrize("kw", [{}, {"window": 1}, {"window": 37}, {"window": 300, "softcap": 20.0}, {"softcap": 3.0}, {"causal": False}, {"scale": 0.3}])
 @pytest.mark.parametrize("dim,group,dtype", [(64, 5, "f16"), (128, 2, "bf16"), (256, 1, "bf16")])
 def test_runs_of_queries(dev, dim, group, dtype, kw, variant):
     """several queries a sequence: verifying steps, chunks behind a prefix, whole prompts"""
+    if variant == 2 and dim == 256:
+        pytest.skip("the tensor-core kernel serves head_dim 64 and 128")
     _attend(dev, [4, 1, 130, 0, 33, 300], [700, 1, 130, 9, 1000, 301], 2, group, dim, 48, 16, dtype, variant=variant, **kw)
 
 
-def test_rows_that_see_nothing(dev):
+@pytest.mark.parametrize("dim,page,block,group,dtype", [(128, 64, 64, 4, "bf16"), (128, 16, 16, 1, "f16"), (64, 256, 32, 8, "bf16"), (64, 80, 16, 3, "f16")])
+def test_prompts(dev, dim, page, block, group, dtype):
+    """the tensor-core kernel over several row blocks and key tiles, boxes of every height"""
+    _attend(dev, [700, 129, 1, 385], [700, 1500, 64, 385], 2, group, dim, page, block, dtype, variant=2)
+    _attend(dev, [513], [2049], 1, group, dim, page, block, dtype, variant=2, window=200, softcap=30.0)
+
+
+@pytest.mark.parametrize("variant", [0, 2])
+def test_rows_that_see_nothing(dev, variant):
     """more queries than tokens, and sequences that hold none"""
-    cache, q, out = _attend(dev, [5, 3, 1], [2, 0, 0], 2, 2, 64, 16, 16, "bf16")
+    cache, q, out = _attend(dev, [5, 3, 1], [2, 0, 0], 2, 2, 64, 16, 16, "bf16", variant=variant)
     assert (out[:3] == 0).all() and (out[5:] == 0).all()
 
 
@@ -423,7 +433,7 @@ def test_large_and_small_queries(dev):
         _check_attention(cache, q, [1, 1], lens, out, scale=1.0 / (8 * spread))
 
 
-@pytest.mark.parametrize("variant", [0, 1])
+@pytest.mark.parametrize("variant", [0, 1, 2])
 @pytest.mark.parametrize("dim", [64, 128])
 def test_nan_only_where_it_is_seen(dev, dim, variant):
     """A NaN in a later token's key or value does not reach earlier queries; those that see it get NaN where the plain form does."""
