@@ -112,19 +112,29 @@ __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Shared-memory descriptors as {low, high} words. Only the start address (low
+// 14 bits, in 16-byte units) changes between the steps of a tile, so a step is
+// one 32-bit add.
+__device__ __forceinline__ uint64_t desc_at(uint32_t low, uint32_t high) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(low), "r"(high));
+    return d;
+}
+// K-major operand of D-byte rows, D-byte swizzle (sdesc_kmajor<D>).
+template <int D>
+__device__ __forceinline__ uint32_t kmajor_low(uint32_t smem_addr) {
+    return (smem_addr >> 4) | (1u << 16);
+}
+template <int D>
+constexpr uint32_t kmajor_high() {
+    return ((D == 128 ? 1024u : 512u) >> 4) | (1u << 14) | ((D == 128 ? 2u : 4u) << 29);
+}
 // B operand of P V: [token][d] with d contiguous (MN-major), halves, 128-byte
 // swizzle: blocks of 64 d (128-byte rows, one per token, 8-token groups 1024
 // bytes apart: the stride of K) of kTile tokens each (16 KiB apart: the stride
 // of N).
-__device__ __forceinline__ uint64_t sdesc_v(uint32_t smem_addr) {
-    uint64_t d = 0;
-    d |= static_cast<uint64_t>((smem_addr & 0x3ffffu) >> 4);
-    d |= static_cast<uint64_t>((kTile * 128) >> 4) << 16;
-    d |= static_cast<uint64_t>(1024u >> 4) << 32;
-    d |= static_cast<uint64_t>(1u) << 46;
-    d |= static_cast<uint64_t>(2u) << 61;
-    return d;
-}
+__device__ __forceinline__ uint32_t values_low(uint32_t smem_addr) { return (smem_addr >> 4) | (((kTile * 128u) >> 4) << 16); }
+constexpr uint32_t kValuesHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
 
 // kind::f16 with fp16 A and B, f32 D, A K-major, B MN-major.
 constexpr uint32_t idesc_f16(uint32_t m, uint32_t n) { return (1u << 4) | (1u << 16) | ((n >> 3) << 17) | ((m >> 4) << 24); }
@@ -135,6 +145,37 @@ constexpr uint32_t idesc_f16(uint32_t m, uint32_t n) { return (1u << 4) | (1u <<
 template <int D>
 __device__ __forceinline__ uint32_t kmajor_offset(int row, int chunk) {
     return D == 128 ? row * 128 + ((chunk ^ (row & 7)) << 4) : row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
+}
+
+// a + b on two fp32 lanes.
+__device__ __forceinline__ void add2(float &d0, float &d1, float a0, float a1, float b0, float b1) {
+    asm("{\n\t.reg .b64 ra, rb, rd;\n\t"
+        "mov.b64 ra, {%2, %3};\n\t"
+        "mov.b64 rb, {%4, %5};\n\t"
+        "add.rn.f32x2 rd, ra, rb;\n\t"
+        "mov.b64 {%0, %1}, rd;\n\t}"
+        : "=f"(d0), "=f"(d1)
+        : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+
+// Maximum and sum of 16 values as trees: one warp per scheduler and tile has
+// to find its parallelism within the row.
+__device__ __forceinline__ float max16(const uint32_t *r) {
+    auto v = [&](int i) { return __uint_as_float(r[i]); };
+    const float a = max3(v(0), v(1), v(2)), b = max3(v(3), v(4), v(5)), c = max3(v(6), v(7), v(8)), d = max3(v(9), v(10), v(11)),
+                e = max3(v(12), v(13), v(14));
+    return max3(max3(a, b, c), max3(d, e, v(15)), v(15));
+}
+__device__ __forceinline__ float sum16(const float *x) {
+    float t[16];
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) add2(t[i], t[i + 1], x[i], x[i + 1], x[i + 8], x[i + 9]);
+    add2(t[0], t[1], t[0], t[1], t[4], t[5]);
+    add2(t[2], t[3], t[2], t[3], t[6], t[7]);
+    add2(t[0], t[1], t[0], t[1], t[2], t[3]);
+    return t[0] + t[1];
 }
 
 // The CTA's work, known to every thread.
@@ -221,55 +262,67 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
         const int part_lane = lane % LPR;
         const bool vec = aligned(a.q, 8) && a.q_token_stride % 4 == 0 && a.q_head_stride % 4 == 0;
         const int most = two ? kBlockRows : kTile;
-        for (int r = warp * RPW + lane / LPR; r < most; r += (kThreads / 32) * RPW) {
-            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (r < w.rows) {
-                const int row = w.row0 + r;
-                const int64_t off = (w.t0 + static_cast<int64_t>(row / a.group)) * a.q_token_stride +
-                                    (static_cast<int64_t>(w.head) * a.group + row % a.group) * a.q_head_stride + part_lane * 4;
-                uint16_t e[4];
-                const uint16_t *p = static_cast<const uint16_t *>(a.q) + off;
-                if (vec) {
-                    const uint2 t = __ldg(reinterpret_cast<const uint2 *>(p));
-                    memcpy(e, &t, 8);
-                } else {
+        constexpr int kStride = (kThreads / 32) * RPW, kAhead = 8;  // rows whose loads are in flight together
+        uint16_t e4[kAhead][4];
+        for (int r0 = warp * RPW + lane / LPR; r0 < most; r0 += kAhead * kStride) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) e[i] = p[i];
+            for (int u = 0; u < kAhead; ++u) {
+                const int r = r0 + u * kStride;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) e4[u][i] = 0;
+                if (r < w.rows) {
+                    const int row = w.row0 + r;
+                    const int64_t off = (w.t0 + static_cast<int64_t>(row / a.group)) * a.q_token_stride +
+                                        (static_cast<int64_t>(w.head) * a.group + row % a.group) * a.q_head_stride + part_lane * 4;
+                    const uint16_t *p = static_cast<const uint16_t *>(a.q) + off;
+                    if (vec) {
+                        const uint2 t = __ldg(reinterpret_cast<const uint2 *>(p));
+                        memcpy(e4[u], &t, 8);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) e4[u][i] = p[i];
+                    }
                 }
+            }
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const int r = r0 + u * kStride;
+                if (r >= most) break;
+                float v[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    v[i] = a.bf16 ? __uint_as_float(static_cast<uint32_t>(e[i]) << 16) : __half2float(__ushort_as_half(e[i]));
-            }
-            uint32_t mx = 0;
+                    v[i] = NP == 2 ? __uint_as_float(static_cast<uint32_t>(e4[u][i]) << 16) : __half2float(__ushort_as_half(e4[u][i]));
+                uint32_t mx = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) mx = max(mx, abs_bits_nan0(v[i]));
+                for (int i = 0; i < 4; ++i) mx = max(mx, abs_bits_nan0(v[i]));
 #pragma unroll
-            for (int o = LPR / 2; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            // times 2^(7 - e): the largest element comes to [128, 256); infinities stay (and saturate)
-            int e = static_cast<int>(mx >> 23);
-            e = mx == 0 ? 127 : min(max(e, 8), 253);
-            const float up = __uint_as_float(static_cast<uint32_t>(254 - e) << 23) * 128.0f;
-            if (part_lane == 0) sh.row_factor[r] = __uint_as_float(static_cast<uint32_t>(e) << 23) * 0.0078125f;
-            bool special = false;
-            float x[4];
+                for (int o = LPR / 2; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                // times 2^(7 - e): the largest element comes to [128, 256); infinities stay (and saturate)
+                int e = static_cast<int>(mx >> 23);
+                e = mx == 0 ? 127 : min(max(e, 8), 253);
+                const float up = __uint_as_float(static_cast<uint32_t>(254 - e) << 23) * 128.0f;
+                if (part_lane == 0) sh.row_factor[r] = __uint_as_float(static_cast<uint32_t>(e) << 23) * 0.0078125f;
+                bool special = false;
+                float x[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x[i] = v[i] * up;
-                special |= !(fabsf(x[i]) < INFINITY);
-            }
-            const int t = r >> 7, tr = r & 127;
+                for (int i = 0; i < 4; ++i) {
+                    x[i] = v[i] * up;
+                    special |= !(fabsf(x[i]) < INFINITY);
+                }
+                const int t = r >> 7, tr = r & 127;
 #pragma unroll
-            for (int p = 0; p < NP; ++p) {
-                uint32_t c = cvt_e4m3x2(x[0], x[1]) | (cvt_e4m3x2(x[2], x[3]) << 16);
-                if (special) c = 0x7f7f7f7fu;  // a row with an infinity or NaN has NaN scores
-                const uint32_t at = smem + (t * NP + p) * S::kQPart + kmajor_offset<D>(tr, part_lane >> 2) + (part_lane & 3) * 4;
-                asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(c) : "memory");
-                if (p + 1 < NP) {
-                    float f[4];
-                    e4m3x2_decode(c & 0xffffu, f[0], f[1]);
-                    e4m3x2_decode(c >> 16, f[2], f[3]);
+                for (int p = 0; p < NP; ++p) {
+                    uint32_t c = cvt_e4m3x2(x[0], x[1]) | (cvt_e4m3x2(x[2], x[3]) << 16);
+                    if (special) c = 0x7f7f7f7fu;  // a row with an infinity or NaN has NaN scores
+                    const uint32_t at = smem + (t * NP + p) * S::kQPart + kmajor_offset<D>(tr, part_lane >> 2) + (part_lane & 3) * 4;
+                    asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(c) : "memory");
+                    if (p + 1 < NP) {
+                        float f[4];
+                        e4m3x2_decode(c & 0xffffu, f[0], f[1]);
+                        e4m3x2_decode(c >> 16, f[2], f[3]);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) x[i] -= f[i];
+                        for (int i = 0; i < 4; ++i) x[i] -= f[i];
+                    }
                 }
             }
         }
@@ -343,47 +396,55 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
             // no copy is in flight when the CTA ends (only a given-up wait leaves any)
             for (int j = max(0, issued - S::kKStages); j < issued; ++j)
                 mbar_wait(&sh.k_full[j % S::kKStages], (j / S::kKStages) & 1, a.err, kDevTimeoutDrain);
-        } else if (warp == 13 && lane == 0 && n > 0) {
+        } else if (warp == 13 && n > 0) {
+            // The whole warp walks the schedule (uniform operands), one
+            // elected lane issues: with a per-lane branch around the loop an
+            // MMA takes 210 clocks to issue instead of the 64 it runs.
             constexpr uint32_t kIdescS = idesc_e4m3_f32(kTile, kTile, 0), kIdescO = idesc_f16(kTile, D);
+            const bool lead = elect_one();
+            auto wait = [&](uint64_t *bar, int parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, a.err, kDevTimeoutMma)) != 0; };
             auto qk = [&](int t, int j) {
-                const uint32_t kb = smem + S::kOffK + (j % S::kKStages) * S::kK;
+                const uint32_t kb = kmajor_low<D>(smem + S::kOffK + (j % S::kKStages) * S::kK), qb = kmajor_low<D>(smem + t * NP * S::kQPart);
+                if (lead) {
 #pragma unroll
-                for (int p = 0; p < NP; ++p)
+                    for (int p = 0; p < NP; ++p)
 #pragma unroll
-                    for (int k = 0; k < D / 32; ++k)
-                        umma_f8f6f4(tmem + t * kTile, sdesc_kmajor<D>(smem + (t * NP + p) * S::kQPart + k * 32), sdesc_kmajor<D>(kb + k * 32), kIdescS,
-                                    p + k > 0);
-                umma_commit(&sh.s_full[t]);
+                        for (int k = 0; k < D / 32; ++k)
+                            umma_f8f6f4(tmem + t * kTile, desc_at(qb + ((p * S::kQPart + k * 32) >> 4), kmajor_high<D>()),
+                                        desc_at(kb + k * 2, kmajor_high<D>()), kIdescS, p + k > 0);
+                    umma_commit(&sh.s_full[t]);
+                }
             };
-            bool ok = mbar_wait(&sh.k_full[0], 0, a.err, kDevTimeoutMma);
+            bool ok = wait(&sh.k_full[0], 0);
             tc_fence_after();
             if (ok) {
                 qk(0, 0);
                 if (two) qk(1, 0);
-                umma_commit(&sh.k_empty[0]);
+                if (lead) umma_commit(&sh.k_empty[0]);
             }
             for (int j = 0; j < n && ok; ++j) {
                 const int vst = j % kVStages;
-                const uint32_t vb = smem + S::kOffV + vst * S::kV;
-                ok = mbar_wait(&sh.v_full[vst], (j / kVStages) & 1, a.err, kDevTimeoutMma);
+                const uint32_t vb = values_low(smem + S::kOffV + vst * S::kV);
+                ok = wait(&sh.v_full[vst], (j / kVStages) & 1);
                 for (int t = 0; t < (two ? 2 : 1) && ok; ++t) {
-                    ok = mbar_wait(&sh.p_full[t], j & 1, a.err, kDevTimeoutMma);
+                    ok = wait(&sh.p_full[t], j & 1);
                     if (!ok) break;
                     tc_fence_after();
-#pragma unroll
-                    for (int k = 0; k < kTile / 16; ++k)
-                        umma_f16_ts(tmem + 2 * kTile + t * D, tmem + t * kTile + k * 8, sdesc_v(vb + k * 2048), kIdescO, j > 0 || k > 0);
                     const bool last_tile = t == (two ? 1 : 0);
-                    if (last_tile) umma_commit(&sh.v_empty[vst]);
+                    if (lead) {
+#pragma unroll
+                        for (int k = 0; k < kTile / 16; ++k)
+                            umma_f16_ts(tmem + 2 * kTile + t * D, tmem + t * kTile + k * 8, desc_at(vb + k * 128, kValuesHigh), kIdescO, k > 0 ? 1u : j > 0);
+                        if (last_tile) umma_commit(&sh.v_empty[vst]);
+                        if (j + 1 == n) umma_commit(&sh.o_full[t]);
+                    }
                     if (j + 1 < n) {
                         const int kst = (j + 1) % S::kKStages;
-                        if (t == 0) ok = mbar_wait(&sh.k_full[kst], ((j + 1) / S::kKStages) & 1, a.err, kDevTimeoutMma);
+                        if (t == 0) ok = wait(&sh.k_full[kst], ((j + 1) / S::kKStages) & 1);
                         if (!ok) break;
                         tc_fence_after();
                         qk(t, j + 1);
-                        if (last_tile) umma_commit(&sh.k_empty[kst]);
-                    } else {
-                        umma_commit(&sh.o_full[t]);
+                        if (last_tile && lead) umma_commit(&sh.k_empty[kst]);
                     }
                 }
             }
@@ -487,38 +548,53 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tc_fence_after();
-                uint32_t sr[4][32];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) tmem_ld_32x32b_x32(ts + q * 32, sr[q]);
-                tmem_wait_ld();
                 const int base = (w.tile_lo + j) * kTile;
                 const bool whole = __all_sync(0xffffffffu, first <= base && last >= base + kTile - 1);
-                const bool scaled = CAP || !whole;  // scores brought to log2 units element by element
+                float gf[kGroups], gb[kGroups];  // a group's scores in log2 units: S gf + gb
+#pragma unroll
+                for (int g = 0; g < kGroups; ++g) {
+                    const float2 gi = *reinterpret_cast<const float2 *>(&sh.info[st][g]);
+                    gf[g] = gi.x * factor;
+                    gb[g] = gi.y;
+                }
+                // S is read twice, 32 columns at a time and one read ahead:
+                // for the maximum, then for the weights. Holding the row's 128
+                // scores instead takes over 190 registers and spills.
                 float top = -INFINITY;
-                if (!scaled) {
+                uint32_t sr[2][32];
+                tmem_ld_32x32b_x32(ts, sr[0]);
+                if (!CAP && whole) {
 #pragma unroll
-                    for (int g = 0; g < kGroups; ++g) {
-                        const GroupInfo gi = sh.info[st][g];
-                        float mx = __uint_as_float(sr[g >> 1][(g & 1) * 16]);
-#pragma unroll
-                        for (int e = 1; e < 16; ++e) mx = fmaxf(mx, __uint_as_float(sr[g >> 1][(g & 1) * 16 + e]));
-                        top = fmaxf(top, fmaf(mx, gi.k_scale * factor, gi.log2_v));
+                    for (int q = 0; q < 4; ++q) {
+                        tmem_wait_ld();
+                        tmem_ld_32x32b_x32(ts + ((q + 1) & 3) * 32, sr[(q + 1) & 1]);  // the last one: the next pass's first
+                        top = max3(top, fmaf(max16(sr[q & 1]), gf[2 * q], gb[2 * q]), fmaf(max16(sr[q & 1] + 16), gf[2 * q + 1], gb[2 * q + 1]));
                     }
                 } else {
+                    // masked or capped, element by element; the results (log2 units) replace S
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        tmem_wait_ld();
+                        uint32_t(&r)[32] = sr[q & 1];
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            const int g = 2 * q + (e >> 4), k = base + q * 32 + e;
+                            const float x = __uint_as_float(r[e]);
+                            float y = CAP ? cap_score(x, gf[g], a.cap) + gb[g] : fmaf(x, gf[g], gb[g]);
+                            y = k >= first && k <= last ? y : -INFINITY;
+                            r[e] = __float_as_uint(y);
+                        }
+                        top = max3(top, max16(r), max16(r + 16));
+                        tmem_st_32x32b_x32(ts + q * 32, r);
+                        if (q < 3) tmem_ld_32x32b_x32(ts + (q + 1) * 32, sr[(q + 1) & 1]);
+                    }
 #pragma unroll
                     for (int g = 0; g < kGroups; ++g) {
-                        const GroupInfo gi = sh.info[st][g];
-                        const float f = gi.k_scale * factor;
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const int k = base + g * 16 + e;
-                            const float x = __uint_as_float(sr[g >> 1][(g & 1) * 16 + e]);
-                            float y = CAP ? cap_score(x, f, a.cap) + gi.log2_v : fmaf(x, f, gi.log2_v);
-                            y = k >= first && k <= last ? y : -INFINITY;
-                            sr[g >> 1][(g & 1) * 16 + e] = __float_as_uint(y);
-                            top = fmaxf(top, y);
-                        }
+                        gf[g] = 1.0f;
+                        gb[g] = 0.0f;
                     }
+                    tmem_wait_st();
+                    tmem_ld_32x32b_x32(ts, sr[0]);
                 }
                 // The reference maximum moves only when a score passes it by
                 // 2^8: most tiles leave O alone. The S of this tile being full
@@ -543,25 +619,22 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
                 const float ref = m == -INFINITY ? 0.0f : m;
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
+                    tmem_wait_ld();
+                    if (q < 3) tmem_ld_32x32b_x32(ts + (q + 1) * 32, sr[(q + 1) & 1]);
                     uint32_t p[16];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const GroupInfo gi = sh.info[st][q * 2 + h];
-                        const float f = scaled ? 1.0f : gi.k_scale * factor;
-                        const float b = (scaled ? 0.0f : gi.log2_v) - ref;
-                        float s0 = 0.0f, s1 = 0.0f;
+                        const float f = gf[q * 2 + h], b = gb[q * 2 + h] - ref;
+                        float x[16];
 #pragma unroll
                         for (int e = 0; e < 16; e += 2) {
-                            float x0, x1;
-                            fma2(x0, x1, __uint_as_float(sr[q][h * 16 + e]), __uint_as_float(sr[q][h * 16 + e + 1]), f, f, b, b);
-                            x0 = exp2_approx(x0);
-                            x1 = exp2_approx(x1);
-                            s0 += x0;
-                            s1 += x1;
-                            const __half2 hp = __floats2half2_rn(x0, x1);
+                            fma2(x[e], x[e + 1], __uint_as_float(sr[q & 1][h * 16 + e]), __uint_as_float(sr[q & 1][h * 16 + e + 1]), f, f, b, b);
+                            x[e] = exp2_approx(x[e]);
+                            x[e + 1] = exp2_approx(x[e + 1]);
+                            const __half2 hp = __floats2half2_rn(x[e], x[e + 1]);
                             p[h * 8 + e / 2] = *reinterpret_cast<const uint32_t *>(&hp);
                         }
-                        l = fmaf(s0 + s1, gi.inv_v, l);
+                        l = fmaf(sum16(x), sh.info[st][q * 2 + h].inv_v, l);
                     }
                     tmem_st_32x32b_x16(ts + q * 16, p);
                 }
@@ -595,7 +668,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const float y0 = l != 0.0f ? __uint_as_float(o[2 * e]) * inv : 0.0f, y1 = l != 0.0f ? __uint_as_float(o[2 * e + 1]) * inv : 0.0f;
-                    if (a.bf16) {
+                    if (NP == 2) {
                         const __nv_bfloat162 b = __floats2bfloat162_rn(y0, y1);
                         pk[e] = *reinterpret_cast<const uint32_t *>(&b);
                     } else {
@@ -620,7 +693,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
         }
     }
 
-    __syncwarp();  // lane 0 of the MMA warp comes last
+    __syncwarp();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
