@@ -29,6 +29,7 @@
 
 #include <cstring>
 #include <mutex>
+#include <type_traits>
 
 #include "lcml_attention.cuh"
 
@@ -41,6 +42,7 @@ constexpr int kThreads = 512;
 constexpr int kGroups = kTile / 16;       // 16-token groups of a key tile: one pair of scales each
 constexpr int kInfoStages = 4;
 constexpr int kVStages = 2;
+constexpr int kPolyPairs = 2;             // of 8 pairs of weights, by polynomial (whole tiles)
 
 // Registers per thread by role; 256 * 192 + 128 * 80 + 128 * 48 = 512 * 128,
 // the block's allocation at launch.
@@ -65,7 +67,7 @@ struct Shape {
 
 struct Shared {
     uint64_t k_full[3], k_empty[3], v_full[kVStages], v_empty[kVStages], info_full[kInfoStages], info_empty[kInfoStages];
-    uint64_t s_full[2], p_full[2], o_full[2];
+    uint64_t q_full[2], s_full[2], p_full[2][2], o_full[2];  // P in halves of 64 keys
     uint32_t tmem;
     int nan_seen;
     GroupInfo info[kInfoStages][kGroups];
@@ -91,14 +93,6 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
         : "memory");
 }
 
-__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
-        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-        : "memory");
-}
 __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
@@ -156,6 +150,26 @@ __device__ __forceinline__ void add2(float &d0, float &d1, float a0, float a1, f
         "mov.b64 {%0, %1}, rd;\n\t}"
         : "=f"(d0), "=f"(d1)
         : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+
+// 2^x of two values on the FMA pipe, for part of a tile's weights: the special
+// function unit alone takes 8 clocks a warp and value. n = round(x) by the
+// addition of 1.5 * 2^23 (+ 127: the exponent field), 2^(x - n) by the
+// degree-4 polynomial of least relative error on [-1/2, 1/2] (Remez exchange
+// in 64 bits: 2.6e-6), far below the 2^-11 of the half it becomes. NaN stays NaN.
+__device__ __forceinline__ void exp2_poly(float &x0, float &x1) {
+    constexpr float kMagic = 12582912.0f + 127.0f;
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x0) : "f"(-126.0f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x1) : "f"(-126.0f));
+    float t0, t1, f0, f1, p0, p1;
+    add2(t0, t1, x0, x1, kMagic, kMagic);
+    add2(f0, f1, t0, t1, -kMagic, -kMagic);
+    fma2(f0, f1, f0, f1, -1.0f, -1.0f, x0, x1);
+    fma2(p0, p1, f0, f1, 0.009570102207362652f, 0.009570102207362652f, 0.05591785907745361f, 0.05591785907745361f);
+    fma2(p0, p1, p0, p1, f0, f1, 0.240247443318367f, 0.240247443318367f);
+    fma2(p0, p1, p0, p1, f0, f1, 0.6931217908859253f, 0.6931217908859253f);
+    fma2(p0, p1, p0, p1, f0, f1, 0.9999992847442627f, 0.9999992847442627f);
+    mul2(x0, x1, p0, p1, __uint_as_float(__float_as_uint(t0) << 23), __uint_as_float(__float_as_uint(t1) << 23));
 }
 
 __device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
@@ -242,7 +256,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
             }
             for (int i = 0; i < 2; ++i) {
                 mbar_init(&sh.s_full[i], 1);
-                mbar_init(&sh.p_full[i], 4);
+                mbar_init(&sh.q_full[i], 4);
+                mbar_init(&sh.p_full[i][0], 4);
+                mbar_init(&sh.p_full[i][1], 4);
                 mbar_init(&sh.o_full[i], 1);
             }
             sh.nan_seen = 0;
@@ -255,79 +271,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
         tmem_relinquish();
     }
 
-    // Q -> e4m3 parts. A lane takes 4 elements of a row: 32 lanes a row at
-    // head_dim 128, 16 at 64. Rows past the block's end are zeros.
-    {
-        constexpr int LPR = D / 4, RPW = 32 / LPR;
-        const int part_lane = lane % LPR;
-        const bool vec = aligned(a.q, 8) && a.q_token_stride % 4 == 0 && a.q_head_stride % 4 == 0;
-        const int most = two ? kBlockRows : kTile;
-        constexpr int kStride = (kThreads / 32) * RPW, kAhead = 8;  // rows whose loads are in flight together
-        uint16_t e4[kAhead][4];
-        for (int r0 = warp * RPW + lane / LPR; r0 < most; r0 += kAhead * kStride) {
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                const int r = r0 + u * kStride;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) e4[u][i] = 0;
-                if (r < w.rows) {
-                    const int row = w.row0 + r;
-                    const int64_t off = (w.t0 + static_cast<int64_t>(row / a.group)) * a.q_token_stride +
-                                        (static_cast<int64_t>(w.head) * a.group + row % a.group) * a.q_head_stride + part_lane * 4;
-                    const uint16_t *p = static_cast<const uint16_t *>(a.q) + off;
-                    if (vec) {
-                        const uint2 t = __ldg(reinterpret_cast<const uint2 *>(p));
-                        memcpy(e4[u], &t, 8);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) e4[u][i] = p[i];
-                    }
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                const int r = r0 + u * kStride;
-                if (r >= most) break;
-                float v[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    v[i] = NP == 2 ? __uint_as_float(static_cast<uint32_t>(e4[u][i]) << 16) : __half2float(__ushort_as_half(e4[u][i]));
-                uint32_t mx = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) mx = max(mx, abs_bits_nan0(v[i]));
-#pragma unroll
-                for (int o = LPR / 2; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                // times 2^(7 - e): the largest element comes to [128, 256); infinities stay (and saturate)
-                int e = static_cast<int>(mx >> 23);
-                e = mx == 0 ? 127 : min(max(e, 8), 253);
-                const float up = __uint_as_float(static_cast<uint32_t>(254 - e) << 23) * 128.0f;
-                if (part_lane == 0) sh.row_factor[r] = __uint_as_float(static_cast<uint32_t>(e) << 23) * 0.0078125f;
-                bool special = false;
-                float x[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    x[i] = v[i] * up;
-                    special |= !(fabsf(x[i]) < INFINITY);
-                }
-                const int t = r >> 7, tr = r & 127;
-#pragma unroll
-                for (int p = 0; p < NP; ++p) {
-                    uint32_t c = cvt_e4m3x2(x[0], x[1]) | (cvt_e4m3x2(x[2], x[3]) << 16);
-                    if (special) c = 0x7f7f7f7fu;  // a row with an infinity or NaN has NaN scores
-                    const uint32_t at = smem + (t * NP + p) * S::kQPart + kmajor_offset<D>(tr, part_lane >> 2) + (part_lane & 3) * 4;
-                    asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(c) : "memory");
-                    if (p + 1 < NP) {
-                        float f[4];
-                        e4m3x2_decode(c & 0xffffu, f[0], f[1]);
-                        e4m3x2_decode(c >> 16, f[2], f[3]);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) x[i] -= f[i];
-                    }
-                }
-            }
-        }
-        fence_proxy_async_smem();
-    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -415,11 +358,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
                     umma_commit(&sh.s_full[t]);
                 }
             };
-            bool ok = wait(&sh.k_full[0], 0);
-            tc_fence_after();
+            bool ok = wait(&sh.k_full[0], 0) && wait(&sh.q_full[0], 0);
             if (ok) {
                 qk(0, 0);
-                if (two) qk(1, 0);
+                if (two) {
+                    ok = wait(&sh.q_full[1], 0);
+                    if (ok) qk(1, 0);
+                }
                 if (lead) umma_commit(&sh.k_empty[0]);
             }
             for (int j = 0; j < n && ok; ++j) {
@@ -427,14 +372,20 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
                 const uint32_t vb = values_low(smem + S::kOffV + vst * S::kV);
                 ok = wait(&sh.v_full[vst], (j / kVStages) & 1);
                 for (int t = 0; t < (two ? 2 : 1) && ok; ++t) {
-                    ok = wait(&sh.p_full[t], j & 1);
-                    if (!ok) break;
-                    tc_fence_after();
                     const bool last_tile = t == (two ? 1 : 0);
-                    if (lead) {
 #pragma unroll
-                        for (int k = 0; k < kTile / 16; ++k)
-                            umma_f16_ts(tmem + 2 * kTile + t * D, tmem + t * kTile + k * 8, desc_at(vb + k * 128, kValuesHigh), kIdescO, k > 0 ? 1u : j > 0);
+                    for (int h = 0; h < 2; ++h) {  // the first half's product runs under the second half's exponentials
+                        ok = ok && wait(&sh.p_full[t][h], j & 1);
+                        tc_fence_after();
+                        if (ok && lead) {
+#pragma unroll
+                            for (int k = h * 4; k < h * 4 + 4; ++k)
+                                umma_f16_ts(tmem + 2 * kTile + t * D, tmem + t * kTile + k * 8, desc_at(vb + k * 128, kValuesHigh), kIdescO,
+                                            k > 0 ? 1u : j > 0);
+                        }
+                    }
+                    if (!ok) break;
+                    if (lead) {
                         if (last_tile) umma_commit(&sh.v_empty[vst]);
                         if (j + 1 == n) umma_commit(&sh.o_full[t]);
                     }
@@ -451,12 +402,19 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
         }
     } else if (warp >= 8) {
         reg_dec<kConvertRegs>();
-        // A thread takes 16 codes of every kRowsPer-th token: global -> two
-        // 16-byte stores of halves, the loads one tile ahead of the stores.
+        // A thread takes 16 codes of some tokens: global -> two 16-byte stores
+        // of halves, the loads one tile ahead of the stores. Eight lanes take
+        // four 16-code chunks (one 128-byte swizzled row of halves) of two
+        // neighbouring tokens: their stores meet in no bank.
         constexpr int CH = D / 16;                 // 16-code chunks of a token
         constexpr int kPer = kTile * CH / 128;     // per thread and tile
         constexpr int kRowsPer = 128 / CH;         // tokens covered by the warpgroup at once
-        const int wt = threadIdx.x - 256, ch = wt % CH, tok0 = wt / CH;
+        const int wt = threadIdx.x - 256;
+        const int ch = (wt & 3) + (D == 128 ? ((wt >> 3) & 1) * 4 : 0), tok0 = D == 128 ? ((wt >> 4) << 1) + ((wt >> 2) & 1) : wt >> 2;
+        // keys that every row of the block sees: [all_lo, all_hi]
+        const int qa = w.row0 / a.group, qz = (w.row0 + w.rows - 1) / a.group;
+        const int all_hi = a.causal ? min(w.pos0 + qa, w.len - 1) : w.len - 1;
+        const int all_lo = a.window > 0 ? max(0, w.pos0 + qz - a.window + 1) : 0;
         uint4 codes[kPer];
         auto fetch = [&](int j) -> bool {
             const int st = j % kInfoStages;
@@ -480,12 +438,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
             ok = __all_sync(0xffffffffu, mbar_wait(&sh.v_empty[vst], ((j / kVStages) & 1) ^ 1, a.err, kDevTimeoutProducer));
             if (!ok) break;
             const uint32_t vb = smem + S::kOffV + vst * S::kV;
+            const int base = (w.tile_lo + j) * kTile;
             uint32_t nan = 0;
+            if (base < all_lo || base + kTile - 1 > all_hi) {  // elsewhere a NaN reaches only rows that see it
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                const uint32_t cw[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
+                for (int i = 0; i < kPer; ++i) {
+                    const uint32_t cw[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
 #pragma unroll
-                for (int q = 0; q < 4; ++q) nan |= (cw[q] & 0x7f7f7f7fu) + 0x01010101u;
+                    for (int q = 0; q < 4; ++q) nan |= (cw[q] & 0x7f7f7f7fu) + 0x01010101u;
+                }
             }
             if (__any_sync(0xffffffffu, (nan & 0x80808080u) != 0)) {
                 // NaN codes: zeros here, so 0 * NaN reaches no row that does
@@ -509,15 +470,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
                     h[2 * q + 1] = e4m3x2_to_half2(cw[q] >> 16);
                 }
                 const uint32_t row = vb + (ch >> 2) * (kTile * 128) + tok * 128;
-                // lanes of the second 64 d store their halves in the other order: no two lanes of a
-                // quarter warp meet in a bank
-                const int flip = D == 128 ? ch >> 2 : 0;
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    const int half = s ^ flip;
+                for (int half = 0; half < 2; ++half) {
                     const uint32_t at = row + ((((ch & 3) * 2 + half) ^ (tok & 7)) << 4);
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(half ? h[4] : h[0]), "r"(half ? h[5] : h[1]),
-                                 "r"(half ? h[6] : h[2]), "r"(half ? h[7] : h[3])
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(h[4 * half]), "r"(h[4 * half + 1]), "r"(h[4 * half + 2]),
+                                 "r"(h[4 * half + 3])
                                  : "memory");
                 }
             }
@@ -530,13 +487,91 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
         reg_inc<kSoftmaxRegs>();
         const int t = warp >> 2;
         if (t == 0 || two) {
+            // Q tile -> e4m3 parts. A lane takes 8 elements of a row: 16 lanes
+            // a row at head_dim 128, 8 at 64; a warp its tile's rows
+            // warp % 4 * 32 .. + 31. Rows past the block's end are zeros.
+            {
+                constexpr int LPR = D / 8, RPW = 32 / LPR, kPasses = 32 / RPW, kAhead = 8;  // rows in flight together
+                const int part_lane = lane % LPR;
+                const bool vec = aligned(a.q, 16) && a.q_token_stride % 8 == 0 && a.q_head_stride % 8 == 0;
+#pragma unroll 1
+                for (int p0 = 0; p0 < kPasses; p0 += kAhead) {
+                    uint4 e8[kAhead];
+#pragma unroll
+                    for (int u = 0; u < kAhead; ++u) {
+                        const int r = warp * 32 + (p0 + u) * RPW + lane / LPR;
+                        e8[u] = make_uint4(0, 0, 0, 0);
+                        if (r < w.rows) {
+                            const int row = w.row0 + r;
+                            const int64_t off = (w.t0 + static_cast<int64_t>(row / a.group)) * a.q_token_stride +
+                                                (static_cast<int64_t>(w.head) * a.group + row % a.group) * a.q_head_stride + part_lane * 8;
+                            const uint16_t *p = static_cast<const uint16_t *>(a.q) + off;
+                            if (vec) {
+                                e8[u] = __ldg(reinterpret_cast<const uint4 *>(p));
+                            } else {
+                                uint32_t h[4];
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) h[i] = p[2 * i] | (static_cast<uint32_t>(p[2 * i + 1]) << 16);
+                                e8[u] = make_uint4(h[0], h[1], h[2], h[3]);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int u = 0; u < kAhead; ++u) {
+                        const int r = warp * 32 + (p0 + u) * RPW + lane / LPR;
+                        const uint32_t h[4] = {e8[u].x, e8[u].y, e8[u].z, e8[u].w};
+                        float x[8];
+                        uint32_t mx = 0;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const uint32_t bits = i & 1 ? h[i / 2] >> 16 : h[i / 2] & 0xffffu;
+                            x[i] = NP == 2 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+                            mx = max(mx, abs_bits_nan0(x[i]));
+                        }
+#pragma unroll
+                        for (int o = LPR / 2; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                        // times 2^(7 - e): the largest element comes to [128, 256)
+                        int e = static_cast<int>(mx >> 23);
+                        e = mx == 0 ? 127 : min(max(e, 8), 253);
+                        const float up = __uint_as_float(static_cast<uint32_t>(254 - e) << 23) * 128.0f;
+                        if (part_lane == 0) sh.row_factor[r] = __uint_as_float(static_cast<uint32_t>(e) << 23) * 0.0078125f;
+                        bool special = false;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            special |= !(fabsf(x[i]) < INFINITY);
+                            x[i] *= up;
+                        }
+#pragma unroll
+                        for (int p = 0; p < NP; ++p) {
+                            uint32_t c[2];
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) c[i] = cvt_e4m3x2(x[4 * i], x[4 * i + 1]) | (cvt_e4m3x2(x[4 * i + 2], x[4 * i + 3]) << 16);
+                            if (special) c[0] = 0x7f7f7f7fu;  // a row with an infinity or NaN has NaN scores
+                            const uint32_t at = smem + (t * NP + p) * S::kQPart + kmajor_offset<D>(r & 127, part_lane >> 1) + (part_lane & 1) * 8;
+                            asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(c[0]), "r"(c[1]) : "memory");
+                            if (p + 1 < NP) {
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    float f0, f1;
+                                    e4m3x2_decode((c[i / 2] >> (16 * (i & 1))) & 0xffffu, f0, f1);
+                                    x[2 * i] -= f0;
+                                    x[2 * i + 1] -= f1;
+                                }
+                            }
+                        }
+                    }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.q_full[t]);
+            }
             const int r = threadIdx.x;  // row of the block
             const int row = w.row0 + r;
             const bool live = r < w.rows;  // the others (zero queries) are computed and dropped
             const int pos = w.pos0 + row / a.group;
             const int last = a.causal ? min(pos, w.len - 1) : w.len - 1;
             const int first = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-            const float factor = sh.row_factor[r] * (CAP ? a.inv_cap : a.scale_log2);
+            const float factor = sh.row_factor[r] * (CAP ? a.inv_cap : a.scale_log2);  // this warp's own rows
             const uint32_t lane_base = static_cast<uint32_t>(warp & 3) << 21;  // TMEM lanes 32 (warp % 4) ..
             const uint32_t ts = tmem + lane_base + t * kTile, to = tmem + lane_base + 2 * kTile + t * D;
             float m = -INFINITY, l = 0.0f;
@@ -550,25 +585,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
                 tc_fence_after();
                 const int base = (w.tile_lo + j) * kTile;
                 const bool whole = __all_sync(0xffffffffu, first <= base && last >= base + kTile - 1);
-                float gf[kGroups], gb[kGroups];  // a group's scores in log2 units: S gf + gb
-#pragma unroll
-                for (int g = 0; g < kGroups; ++g) {
-                    const float2 gi = *reinterpret_cast<const float2 *>(&sh.info[st][g]);
-                    gf[g] = gi.x * factor;
-                    gb[g] = gi.y;
-                }
                 // S is read twice, 32 columns at a time and one read ahead:
                 // for the maximum, then for the weights. Holding the row's 128
-                // scores instead takes over 190 registers and spills.
+                // scores instead leaves no registers for the polynomial's
+                // constants, which then cost a move at every use.
                 float top = -INFINITY;
                 uint32_t sr[2][32];
                 tmem_ld_32x32b_x32(ts, sr[0]);
-                if (!CAP && whole) {
+                const bool plain = !CAP && whole;
+                if (plain) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
+                        const float2 g0 = *reinterpret_cast<const float2 *>(&sh.info[st][2 * q]), g1 = *reinterpret_cast<const float2 *>(&sh.info[st][2 * q + 1]);
                         tmem_wait_ld();
                         tmem_ld_32x32b_x32(ts + ((q + 1) & 3) * 32, sr[(q + 1) & 1]);  // the last one: the next pass's first
-                        top = max3(top, fmaf(max16(sr[q & 1]), gf[2 * q], gb[2 * q]), fmaf(max16(sr[q & 1] + 16), gf[2 * q + 1], gb[2 * q + 1]));
+                        top = max3(top, fmaf(max16(sr[q & 1]), g0.x * factor, g0.y), fmaf(max16(sr[q & 1] + 16), g1.x * factor, g1.y));
                     }
                 } else {
                     // masked or capped, element by element; the results (log2 units) replace S
@@ -578,20 +609,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
                         uint32_t(&r)[32] = sr[q & 1];
 #pragma unroll
                         for (int e = 0; e < 32; ++e) {
-                            const int g = 2 * q + (e >> 4), k = base + q * 32 + e;
-                            const float x = __uint_as_float(r[e]);
-                            float y = CAP ? cap_score(x, gf[g], a.cap) + gb[g] : fmaf(x, gf[g], gb[g]);
+                            const float2 gi = *reinterpret_cast<const float2 *>(&sh.info[st][2 * q + (e >> 4)]);
+                            const int k = base + q * 32 + e;
+                            const float x = __uint_as_float(r[e]), f = gi.x * factor;
+                            float y = CAP ? cap_score(x, f, a.cap) + gi.y : fmaf(x, f, gi.y);
                             y = k >= first && k <= last ? y : -INFINITY;
                             r[e] = __float_as_uint(y);
                         }
                         top = max3(top, max16(r), max16(r + 16));
                         tmem_st_32x32b_x32(ts + q * 32, r);
                         if (q < 3) tmem_ld_32x32b_x32(ts + (q + 1) * 32, sr[(q + 1) & 1]);
-                    }
-#pragma unroll
-                    for (int g = 0; g < kGroups; ++g) {
-                        gf[g] = 1.0f;
-                        gb[g] = 0.0f;
                     }
                     tmem_wait_st();
                     tmem_ld_32x32b_x32(ts, sr[0]);
@@ -617,43 +644,57 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
                     }
                 }
                 const float ref = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    tmem_wait_ld();
-                    if (q < 3) tmem_ld_32x32b_x32(ts + (q + 1) * 32, sr[(q + 1) & 1]);
-                    uint32_t p[16];
+                // One branch for the whole tile: one per pair of weights would
+                // serialise them.
+                auto weights = [&](auto plain_tile) {
+                    constexpr bool kPlain = decltype(plain_tile)::value;
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const float f = gf[q * 2 + h], b = gb[q * 2 + h] - ref;
-                        float x[16];
+                        uint32_t p[32];
 #pragma unroll
-                        for (int e = 0; e < 16; e += 2) {
-                            fma2(x[e], x[e + 1], __uint_as_float(sr[q & 1][h * 16 + e]), __uint_as_float(sr[q & 1][h * 16 + e + 1]), f, f, b, b);
-                            x[e] = exp2_approx(x[e]);
-                            x[e + 1] = exp2_approx(x[e + 1]);
-                            const __half2 hp = __floats2half2_rn(x[e], x[e + 1]);
-                            p[h * 8 + e / 2] = *reinterpret_cast<const uint32_t *>(&hp);
+                        for (int g = 0; g < 4; ++g) {
+                            const int q = h * 2 + g / 2;  // 32 columns: two groups
+                            if (g % 2 == 0) {
+                                tmem_wait_ld();
+                                if (q < 3) tmem_ld_32x32b_x32(ts + (q + 1) * 32, sr[(q + 1) & 1]);
+                            }
+                            const float4 gi = *reinterpret_cast<const float4 *>(&sh.info[st][h * 4 + g]);
+                            const float f = kPlain ? gi.x * factor : 1.0f, b = (kPlain ? gi.y : 0.0f) - ref;
+                            float x[16];
+#pragma unroll
+                            for (int e = 0; e < 16; e += 2) {
+                                const int i = g % 2 * 16 + e;
+                                fma2(x[e], x[e + 1], __uint_as_float(sr[q & 1][i]), __uint_as_float(sr[q & 1][i + 1]), f, f, b, b);
+                                if (kPlain && e / 2 < kPolyPairs) {
+                                    exp2_poly(x[e], x[e + 1]);
+                                } else {
+                                    x[e] = exp2_approx(x[e]);
+                                    x[e + 1] = exp2_approx(x[e + 1]);
+                                }
+                                const __half2 hp = __floats2half2_rn(x[e], x[e + 1]);
+                                p[g * 8 + e / 2] = *reinterpret_cast<const uint32_t *>(&hp);
+                            }
+                            l = fmaf(sum16(x), gi.z, l);
                         }
-                        l = fmaf(sum16(x), sh.info[st][q * 2 + h].inv_v, l);
+                        tmem_st_32x32b_x32(ts + h * 32, p);
+                        tmem_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sh.p_full[t][h]);
                     }
-                    tmem_st_32x32b_x16(ts + q * 16, p);
-                }
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&sh.p_full[t]);
-                    mbar_arrive(&sh.info_empty[st]);
-                }
+                };
+                if (plain) weights(std::true_type{});
+                else weights(std::false_type{});
+                if (lane == 0) mbar_arrive(&sh.info_empty[st]);
             }
             if (ok && n > 0) ok = mbar_wait(&sh.o_full[t], 0, a.err, kDevTimeoutEpilogue);
             ok = __all_sync(0xffffffffu, ok);
             tc_fence_after();
-            // one row per thread: D halves, 16 bytes at a time where aligned
+            // one row per thread, in whole 32-byte sectors where aligned
             const int64_t token = w.t0 + static_cast<int64_t>(row / a.group);
             const int qh = w.head * a.group + row % a.group;
             uint16_t *out = static_cast<uint16_t *>(a.out) + token * a.out_token_stride + qh * a.out_head_stride;
-            const bool vec = aligned(a.out, 16) && a.out_token_stride % 8 == 0 && a.out_head_stride % 8 == 0;
+            const bool vec = aligned(a.out, 32) && a.out_token_stride % 16 == 0 && a.out_head_stride % 16 == 0;
             const float inv = l != 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
             for (int q = 0; q < D / 32; ++q) {
@@ -678,7 +719,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
                 }
                 if (vec && live && ok) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) reinterpret_cast<uint4 *>(out + q * 32)[e] = make_uint4(pk[4 * e], pk[4 * e + 1], pk[4 * e + 2], pk[4 * e + 3]);
+                    for (int e = 0; e < 2; ++e)
+                        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out + q * 32 + e * 16), "r"(pk[8 * e]),
+                                     "r"(pk[8 * e + 1]), "r"(pk[8 * e + 2]), "r"(pk[8 * e + 3]), "r"(pk[8 * e + 4]), "r"(pk[8 * e + 5]),
+                                     "r"(pk[8 * e + 6]), "r"(pk[8 * e + 7])
+                                     : "memory");
                 } else if (live && ok) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
