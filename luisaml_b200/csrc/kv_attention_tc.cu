@@ -67,7 +67,7 @@ struct Shape {
 
 struct Shared {
     uint64_t k_full[3], k_empty[3], v_full[kVStages], v_empty[kVStages], info_full[kInfoStages], info_empty[kInfoStages];
-    uint64_t q_full[2], s_full[2], p_full[2][2], o_full[2];  // P in halves of 64 keys
+    uint64_t q_full[2], s_full[2], p_full[2], o_full[2];
     uint32_t tmem;
     int nan_seen;
     GroupInfo info[kInfoStages][kGroups];
@@ -257,8 +257,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
             for (int i = 0; i < 2; ++i) {
                 mbar_init(&sh.s_full[i], 1);
                 mbar_init(&sh.q_full[i], 4);
-                mbar_init(&sh.p_full[i][0], 4);
-                mbar_init(&sh.p_full[i][1], 4);
+                mbar_init(&sh.p_full[i], 4);
                 mbar_init(&sh.o_full[i], 1);
             }
             sh.nan_seen = 0;
@@ -373,19 +372,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
                 ok = wait(&sh.v_full[vst], (j / kVStages) & 1);
                 for (int t = 0; t < (two ? 2 : 1) && ok; ++t) {
                     const bool last_tile = t == (two ? 1 : 0);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {  // the first half's product runs under the second half's exponentials
-                        ok = ok && wait(&sh.p_full[t][h], j & 1);
-                        tc_fence_after();
-                        if (ok && lead) {
-#pragma unroll
-                            for (int k = h * 4; k < h * 4 + 4; ++k)
-                                umma_f16_ts(tmem + 2 * kTile + t * D, tmem + t * kTile + k * 8, desc_at(vb + k * 128, kValuesHigh), kIdescO,
-                                            k > 0 ? 1u : j > 0);
-                        }
-                    }
+                    ok = wait(&sh.p_full[t], j & 1);
                     if (!ok) break;
+                    tc_fence_after();
                     if (lead) {
+#pragma unroll
+                        for (int k = 0; k < kTile / 16; ++k)
+                            umma_f16_ts(tmem + 2 * kTile + t * D, tmem + t * kTile + k * 8, desc_at(vb + k * 128, kValuesHigh), kIdescO, k > 0 ? 1u : j > 0);
                         if (last_tile) umma_commit(&sh.v_empty[vst]);
                         if (j + 1 == n) umma_commit(&sh.o_full[t]);
                     }
@@ -584,108 +577,107 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
                 if (!ok) break;
                 tc_fence_after();
                 const int base = (w.tile_lo + j) * kTile;
-                const bool whole = __all_sync(0xffffffffu, first <= base && last >= base + kTile - 1);
-                // S is read twice, 32 columns at a time and one read ahead:
-                // for the maximum, then for the weights. Holding the row's 128
-                // scores instead leaves no registers for the polynomial's
-                // constants, which then cost a move at every use.
-                float top = -INFINITY;
-                uint32_t sr[2][32];
-                tmem_ld_32x32b_x32(ts, sr[0]);
-                const bool plain = !CAP && whole;
-                if (plain) {
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const float2 g0 = *reinterpret_cast<const float2 *>(&sh.info[st][2 * q]), g1 = *reinterpret_cast<const float2 *>(&sh.info[st][2 * q + 1]);
-                        tmem_wait_ld();
-                        tmem_ld_32x32b_x32(ts + ((q + 1) & 3) * 32, sr[(q + 1) & 1]);  // the last one: the next pass's first
-                        top = max3(top, fmaf(max16(sr[q & 1]), g0.x * factor, g0.y), fmaf(max16(sr[q & 1] + 16), g1.x * factor, g1.y));
-                    }
-                } else {
-                    // masked or capped, element by element; the results (log2 units) replace S
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        tmem_wait_ld();
-                        uint32_t(&r)[32] = sr[q & 1];
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) {
-                            const float2 gi = *reinterpret_cast<const float2 *>(&sh.info[st][2 * q + (e >> 4)]);
-                            const int k = base + q * 32 + e;
-                            const float x = __uint_as_float(r[e]), f = gi.x * factor;
-                            float y = CAP ? cap_score(x, f, a.cap) + gi.y : fmaf(x, f, gi.y);
-                            y = k >= first && k <= last ? y : -INFINITY;
-                            r[e] = __float_as_uint(y);
-                        }
-                        top = max3(top, max16(r), max16(r + 16));
-                        tmem_st_32x32b_x32(ts + q * 32, r);
-                        if (q < 3) tmem_ld_32x32b_x32(ts + (q + 1) * 32, sr[(q + 1) & 1]);
-                    }
-                    tmem_wait_st();
+                const bool plain = !CAP && __all_sync(0xffffffffu, first <= base && last >= base + kTile - 1);
+                const GroupInfo *info = sh.info[st];
+                uint32_t sr[2][32], p[64];
+                // Weights of the tile against the reference maximum, 32 scores
+                // at a time and the next 32 on their way. Returns the largest
+                // exponent. kRaw: S as the MMA left it, else in log2 units.
+                auto weights = [&](auto raw, float ref, float &sum) {
+                    constexpr bool kRaw = decltype(raw)::value;
+                    float top = -INFINITY;
                     tmem_ld_32x32b_x32(ts, sr[0]);
-                }
-                // The reference maximum moves only when a score passes it by
-                // 2^8: most tiles leave O alone. The S of this tile being full
-                // means that the previous P V is done.
-                if (__any_sync(0xffffffffu, top > m + 8.0f)) {
-                    const float nm = fmaxf(m, top);
-                    const float f = nm == m ? 1.0f : exp2_approx(m - nm);
-                    m = nm;
-                    l *= f;
-                    if (j > 0) {
 #pragma unroll
-                        for (int q = 0; q < D / 32; ++q) {
-                            uint32_t o[32];
-                            tmem_ld_32x32b_x32(to + q * 32, o);
-                            tmem_wait_ld();
+                    for (int q = 0; q < 4; ++q) {
+                        const float4 g0 = *reinterpret_cast<const float4 *>(info + 2 * q), g1 = *reinterpret_cast<const float4 *>(info + 2 * q + 1);
+                        tmem_wait_ld();
+                        if (q < 3) tmem_ld_32x32b_x32(ts + (q + 1) * 32, sr[(q + 1) & 1]);
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                            tmem_st_32x32b_x32(to + q * 32, o);
-                        }
-                    }
-                }
-                const float ref = m == -INFINITY ? 0.0f : m;
-                // One branch for the whole tile: one per pair of weights would
-                // serialise them.
-                auto weights = [&](auto plain_tile) {
-                    constexpr bool kPlain = decltype(plain_tile)::value;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        uint32_t p[32];
-#pragma unroll
-                        for (int g = 0; g < 4; ++g) {
-                            const int q = h * 2 + g / 2;  // 32 columns: two groups
-                            if (g % 2 == 0) {
-                                tmem_wait_ld();
-                                if (q < 3) tmem_ld_32x32b_x32(ts + (q + 1) * 32, sr[(q + 1) & 1]);
-                            }
-                            const float4 gi = *reinterpret_cast<const float4 *>(&sh.info[st][h * 4 + g]);
-                            const float f = kPlain ? gi.x * factor : 1.0f, b = (kPlain ? gi.y : 0.0f) - ref;
+                        for (int g = 0; g < 2; ++g) {
+                            const float f = kRaw ? (g ? g1.x : g0.x) * factor : 1.0f, b = (kRaw ? (g ? g1.y : g0.y) : 0.0f) - ref;
                             float x[16];
 #pragma unroll
+                            for (int e = 0; e < 16; e += 2)
+                                fma2(x[e], x[e + 1], __uint_as_float(sr[q & 1][g * 16 + e]), __uint_as_float(sr[q & 1][g * 16 + e + 1]), f, f, b, b);
+                            top = fmaxf(top, max16(reinterpret_cast<const uint32_t *>(x)));
+#pragma unroll
                             for (int e = 0; e < 16; e += 2) {
-                                const int i = g % 2 * 16 + e;
-                                fma2(x[e], x[e + 1], __uint_as_float(sr[q & 1][i]), __uint_as_float(sr[q & 1][i + 1]), f, f, b, b);
-                                if (kPlain && e / 2 < kPolyPairs) {
+                                if (kRaw && e / 2 < kPolyPairs) {
                                     exp2_poly(x[e], x[e + 1]);
                                 } else {
                                     x[e] = exp2_approx(x[e]);
                                     x[e + 1] = exp2_approx(x[e + 1]);
                                 }
                                 const __half2 hp = __floats2half2_rn(x[e], x[e + 1]);
-                                p[g * 8 + e / 2] = *reinterpret_cast<const uint32_t *>(&hp);
+                                p[q * 16 + g * 8 + e / 2] = *reinterpret_cast<const uint32_t *>(&hp);
                             }
-                            l = fmaf(sum16(x), gi.z, l);
+                            sum = fmaf(sum16(x), g ? g1.z : g0.z, sum);
                         }
-                        tmem_st_32x32b_x32(ts + h * 32, p);
-                        tmem_wait_st();
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&sh.p_full[t][h]);
                     }
+                    return top;
                 };
-                if (plain) weights(std::true_type{});
-                else weights(std::false_type{});
-                if (lane == 0) mbar_arrive(&sh.info_empty[st]);
+                // The reference maximum moves only when a score passes it by
+                // 2^8 (a weight as a half has room for that), so after the
+                // first tile the weights are taken against the old one at
+                // once, without a pass for the maximum; a tile that passes it
+                // (any row of the warp) is done again below. S stays until P
+                // is known to be good.
+                bool done = false;
+                if (plain && __all_sync(0xffffffffu, m > -INFINITY)) {
+                    float sum = l;
+                    const float top = weights(std::true_type{}, m, sum);
+                    done = !__any_sync(0xffffffffu, top > 8.0f);
+                    if (done) l = sum;
+                }
+                if (!done) {
+                    // scores in log2 units, masked, in place of S; their maximum
+                    float top = -INFINITY;
+#pragma unroll 1
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t(&r)[32] = sr[0];
+                        tmem_ld_32x32b_x32(ts + q * 32, r);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            const float2 gi = *reinterpret_cast<const float2 *>(info + 2 * q + (e >> 4));
+                            const int k = base + q * 32 + e;
+                            const float x = __uint_as_float(r[e]), f = gi.x * factor;
+                            const float y = CAP ? cap_score(x, f, a.cap) + gi.y : fmaf(x, f, gi.y);
+                            r[e] = __float_as_uint(k >= first && k <= last ? y : -INFINITY);
+                        }
+                        top = max3(top, max16(r), max16(r + 16));
+                        tmem_st_32x32b_x32(ts + q * 32, r);
+                    }
+                    tmem_wait_st();
+                    // The S of this tile being full means that the previous P V is done.
+                    if (__any_sync(0xffffffffu, top > m + 8.0f)) {
+                        const float nm = fmaxf(m, top);
+                        const float f = nm == m ? 1.0f : exp2_approx(m - nm);
+                        m = nm;
+                        l *= f;
+                        if (j > 0) {
+#pragma unroll 1
+                            for (int q = 0; q < D / 32; ++q) {
+                                uint32_t(&o)[32] = sr[0];
+                                tmem_ld_32x32b_x32(to + q * 32, o);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                                tmem_st_32x32b_x32(to + q * 32, o);
+                            }
+                        }
+                    }
+                    weights(std::false_type{}, m == -INFINITY ? 0.0f : m, l);
+                }
+                tmem_st_32x32b_x32(ts, reinterpret_cast<uint32_t(&)[32]>(p[0]));
+                tmem_st_32x32b_x32(ts + 32, reinterpret_cast<uint32_t(&)[32]>(p[32]));
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&sh.p_full[t]);
+                    mbar_arrive(&sh.info_empty[st]);
+                }
             }
             if (ok && n > 0) ok = mbar_wait(&sh.o_full[t], 0, a.err, kDevTimeoutEpilogue);
             ok = __all_sync(0xffffffffu, ok);
