@@ -484,72 +484,74 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
             // a row at head_dim 128, 8 at 64; a warp its tile's rows
             // warp % 4 * 32 .. + 31. Rows past the block's end are zeros.
             {
-                constexpr int LPR = D / 8, RPW = 32 / LPR, kPasses = 32 / RPW, kAhead = 8;  // rows in flight together
-                const int part_lane = lane % LPR;
+                constexpr int LPR = D / 8, RPW = 32 / LPR, kPasses = 32 / RPW;
+                const int part_lane = lane % LPR, r0 = warp * 32 + lane / LPR;
                 const bool vec = aligned(a.q, 16) && a.q_token_stride % 8 == 0 && a.q_head_stride % 8 == 0;
-#pragma unroll 1
-                for (int p0 = 0; p0 < kPasses; p0 += kAhead) {
-                    uint4 e8[kAhead];
+                uint4 e8[kPasses];  // all loads at once: one latency
+                uint32_t mx[kPasses];
 #pragma unroll
-                    for (int u = 0; u < kAhead; ++u) {
-                        const int r = warp * 32 + (p0 + u) * RPW + lane / LPR;
-                        e8[u] = make_uint4(0, 0, 0, 0);
-                        if (r < w.rows) {
-                            const int row = w.row0 + r;
-                            const int64_t off = (w.t0 + static_cast<int64_t>(row / a.group)) * a.q_token_stride +
-                                                (static_cast<int64_t>(w.head) * a.group + row % a.group) * a.q_head_stride + part_lane * 8;
-                            const uint16_t *p = static_cast<const uint16_t *>(a.q) + off;
-                            if (vec) {
-                                e8[u] = __ldg(reinterpret_cast<const uint4 *>(p));
-                            } else {
-                                uint32_t h[4];
+                for (int u = 0; u < kPasses; ++u) {
+                    const int r = r0 + u * RPW;
+                    e8[u] = make_uint4(0, 0, 0, 0);
+                    if (r < w.rows) {
+                        const int row = w.row0 + r;
+                        const int64_t off = (w.t0 + static_cast<int64_t>(row / a.group)) * a.q_token_stride +
+                                            (static_cast<int64_t>(w.head) * a.group + row % a.group) * a.q_head_stride + part_lane * 8;
+                        const uint16_t *p = static_cast<const uint16_t *>(a.q) + off;
+                        if (vec) {
+                            e8[u] = __ldg(reinterpret_cast<const uint4 *>(p));
+                        } else {
+                            uint32_t h[4];
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) h[i] = p[2 * i] | (static_cast<uint32_t>(p[2 * i + 1]) << 16);
-                                e8[u] = make_uint4(h[0], h[1], h[2], h[3]);
-                            }
+                            for (int i = 0; i < 4; ++i) h[i] = p[2 * i] | (static_cast<uint32_t>(p[2 * i + 1]) << 16);
+                            e8[u] = make_uint4(h[0], h[1], h[2], h[3]);
                         }
                     }
+                }
+                // a row's largest magnitude: 16-bit floats order like their bits (NaN above infinity)
 #pragma unroll
-                    for (int u = 0; u < kAhead; ++u) {
-                        const int r = warp * 32 + (p0 + u) * RPW + lane / LPR;
-                        const uint32_t h[4] = {e8[u].x, e8[u].y, e8[u].z, e8[u].w};
-                        float x[8];
-                        uint32_t mx = 0;
+                for (int u = 0; u < kPasses; ++u) {
+                    const uint32_t h[4] = {e8[u].x & 0x7fff7fffu, e8[u].y & 0x7fff7fffu, e8[u].z & 0x7fff7fffu, e8[u].w & 0x7fff7fffu};
+                    const uint32_t m2 = __vmaxu2(__vmaxu2(h[0], h[1]), __vmaxu2(h[2], h[3]));
+                    mx[u] = max(m2 & 0xffffu, m2 >> 16);
+                }
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const uint32_t bits = i & 1 ? h[i / 2] >> 16 : h[i / 2] & 0xffffu;
-                            x[i] = NP == 2 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
-                            mx = max(mx, abs_bits_nan0(x[i]));
-                        }
+                for (int o = LPR / 2; o > 0; o >>= 1)
 #pragma unroll
-                        for (int o = LPR / 2; o > 0; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                        // times 2^(7 - e): the largest element comes to [128, 256)
-                        int e = static_cast<int>(mx >> 23);
-                        e = mx == 0 ? 127 : min(max(e, 8), 253);
-                        const float up = __uint_as_float(static_cast<uint32_t>(254 - e) << 23) * 128.0f;
-                        if (part_lane == 0) sh.row_factor[r] = __uint_as_float(static_cast<uint32_t>(e) << 23) * 0.0078125f;
-                        bool special = false;
+                    for (int u = 0; u < kPasses; ++u) mx[u] = max(mx[u], __shfl_xor_sync(0xffffffffu, mx[u], o));
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            special |= !(fabsf(x[i]) < INFINITY);
-                            x[i] *= up;
-                        }
+                for (int u = 0; u < kPasses; ++u) {
+                    const int r = r0 + u * RPW;
+                    const uint32_t h[4] = {e8[u].x, e8[u].y, e8[u].z, e8[u].w};
+                    // times 2^(7 - e): the largest element comes to [128, 256);
+                    // a row with an infinity or NaN has NaN scores
+                    const uint32_t top = NP == 2 ? mx[u] << 16 : __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(mx[u]))));
+                    const bool special = top >= 0x7f800000u;
+                    int e = static_cast<int>(top >> 23);
+                    e = top == 0 ? 127 : min(max(e, 8), 253);
+                    const float up = __uint_as_float(static_cast<uint32_t>(254 - e) << 23) * 128.0f;
+                    if (part_lane == 0) sh.row_factor[r] = __uint_as_float(static_cast<uint32_t>(e) << 23) * 0.0078125f;
+                    float x[8];
 #pragma unroll
-                        for (int p = 0; p < NP; ++p) {
-                            uint32_t c[2];
+                    for (int i = 0; i < 8; ++i) {
+                        const uint32_t bits = i & 1 ? h[i / 2] >> 16 : h[i / 2] & 0xffffu;
+                        x[i] = up * (NP == 2 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(bits))));
+                    }
 #pragma unroll
-                            for (int i = 0; i < 2; ++i) c[i] = cvt_e4m3x2(x[4 * i], x[4 * i + 1]) | (cvt_e4m3x2(x[4 * i + 2], x[4 * i + 3]) << 16);
-                            if (special) c[0] = 0x7f7f7f7fu;  // a row with an infinity or NaN has NaN scores
-                            const uint32_t at = smem + (t * NP + p) * S::kQPart + kmajor_offset<D>(r & 127, part_lane >> 1) + (part_lane & 1) * 8;
-                            asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(c[0]), "r"(c[1]) : "memory");
-                            if (p + 1 < NP) {
+                    for (int p = 0; p < NP; ++p) {
+                        uint32_t c[2];
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    float f0, f1;
-                                    e4m3x2_decode((c[i / 2] >> (16 * (i & 1))) & 0xffffu, f0, f1);
-                                    x[2 * i] -= f0;
-                                    x[2 * i + 1] -= f1;
-                                }
+                        for (int i = 0; i < 2; ++i) c[i] = cvt_e4m3x2(x[4 * i], x[4 * i + 1]) | (cvt_e4m3x2(x[4 * i + 2], x[4 * i + 3]) << 16);
+                        if (special) c[0] = 0x7f7f7f7fu;
+                        const uint32_t at = smem + (t * NP + p) * S::kQPart + kmajor_offset<D>(r & 127, part_lane >> 1) + (part_lane & 1) * 8;
+                        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(c[0]), "r"(c[1]) : "memory");
+                        if (p + 1 < NP) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                float f0, f1;
+                                e4m3x2_decode((c[i / 2] >> (16 * (i & 1))) & 0xffffu, f0, f1);
+                                x[2 * i] -= f0;
+                                x[2 * i + 1] -= f1;
                             }
                         }
                     }
@@ -582,10 +584,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
                 uint32_t sr[2][32], p[64];
                 // Weights of the tile against the reference maximum, 32 scores
                 // at a time and the next 32 on their way. Returns the largest
-                // exponent. kRaw: S as the MMA left it, else in log2 units.
+                // sum of 16 weights, a bound of each. kRaw: S as the MMA left
+                // it, else in log2 units.
                 auto weights = [&](auto raw, float ref, float &sum) {
                     constexpr bool kRaw = decltype(raw)::value;
-                    float top = -INFINITY;
+                    float most = 0.0f;
                     tmem_ld_32x32b_x32(ts, sr[0]);
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
@@ -597,11 +600,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
                             const float f = kRaw ? (g ? g1.x : g0.x) * factor : 1.0f, b = (kRaw ? (g ? g1.y : g0.y) : 0.0f) - ref;
                             float x[16];
 #pragma unroll
-                            for (int e = 0; e < 16; e += 2)
-                                fma2(x[e], x[e + 1], __uint_as_float(sr[q & 1][g * 16 + e]), __uint_as_float(sr[q & 1][g * 16 + e + 1]), f, f, b, b);
-                            top = fmaxf(top, max16(reinterpret_cast<const uint32_t *>(x)));
-#pragma unroll
                             for (int e = 0; e < 16; e += 2) {
+                                fma2(x[e], x[e + 1], __uint_as_float(sr[q & 1][g * 16 + e]), __uint_as_float(sr[q & 1][g * 16 + e + 1]), f, f, b, b);
                                 if (kRaw && e / 2 < kPolyPairs) {
                                     exp2_poly(x[e], x[e + 1]);
                                 } else {
@@ -611,22 +611,24 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
                                 const __half2 hp = __floats2half2_rn(x[e], x[e + 1]);
                                 p[q * 16 + g * 8 + e / 2] = *reinterpret_cast<const uint32_t *>(&hp);
                             }
-                            sum = fmaf(sum16(x), g ? g1.z : g0.z, sum);
+                            const float of16 = sum16(x);
+                            most = fmaxf(most, of16);
+                            sum = fmaf(of16, g ? g1.z : g0.z, sum);
                         }
                     }
-                    return top;
+                    return most;
                 };
-                // The reference maximum moves only when a score passes it by
-                // 2^8 (a weight as a half has room for that), so after the
-                // first tile the weights are taken against the old one at
-                // once, without a pass for the maximum; a tile that passes it
-                // (any row of the warp) is done again below. S stays until P
-                // is known to be good.
+                // The reference maximum moves only when a weight passes 2^8 (a
+                // half has room for that), so after the first tile the weights
+                // are taken against the old one at once, without a pass for
+                // the maximum; a tile with 16 weights of a larger sum (in any
+                // row of the warp) is done again below. S stays until P is
+                // known to be good.
                 bool done = false;
                 if (plain && __all_sync(0xffffffffu, m > -INFINITY)) {
                     float sum = l;
-                    const float top = weights(std::true_type{}, m, sum);
-                    done = !__any_sync(0xffffffffu, top > 8.0f);
+                    const float most = weights(std::true_type{}, m, sum);
+                    done = !__any_sync(0xffffffffu, most > 256.0f);
                     if (done) l = sum;
                 }
                 if (!done) {
@@ -650,7 +652,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
                     }
                     tmem_wait_st();
                     // The S of this tile being full means that the previous P V is done.
-                    if (__any_sync(0xffffffffu, top > m + 8.0f)) {
+                    if (__any_sync(0xffffffffu, top > m + (plain ? 0.0f : 8.0f))) {
                         const float nm = fmaxf(m, top);
                         const float f = nm == m ? 1.0f : exp2_approx(m - nm);
                         m = nm;
