@@ -164,6 +164,12 @@ __device__ __forceinline__ void cp_async_zfill(uint32_t dst, const void *src, ui
     else asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(bytes) : "memory");
 }
 
+template <int BYTES>
+__device__ __forceinline__ void cp_async(uint32_t dst, const void *src) {
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+}
+
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
@@ -204,7 +210,7 @@ __device__ __forceinline__ uint32_t nan_cleared(uint32_t w) {
     return w & ~((m >> 7) * 0xffu);
 }
 
-template <int D>
+template <int D, bool CAP>
 __global__ void __launch_bounds__(kThreads, 1) k_kv_attention(AttnArgs a, int target, int max_rows, JoinItem *join_items, int *join_count,
                                                               float *part_ml, float *part_o) {
     using S = Shape<D>;
@@ -300,9 +306,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention(AttnArgs a, int ta
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int r = g + 8 * i;
-        fac[i] = q_factor[r] * (a.cap != 0.0f ? a.inv_cap : a.scale_log2);
-        const int pos = pos0 + (it.tile * kRows + r) / a.group;
-        last[i] = r < rows ? (a.causal ? min(pos, sp.len - 1) : sp.len - 1) : -1;
+        fac[i] = q_factor[r] * (CAP ? a.inv_cap : a.scale_log2);
+        // rows past the tile's end (zero queries) see what its last row sees; they are not written
+        const int pos = pos0 + (it.tile * kRows + min(r, rows - 1)) / a.group;
+        last[i] = a.causal ? min(pos, sp.len - 1) : sp.len - 1;
         first[i] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
     }
     // Over the tile: keys outside [tile_lo, tile_hi] are seen by no row, keys in [all_lo, all_hi] by every one.
@@ -322,11 +329,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention(AttnArgs a, int ta
 
     const int32_t *table = a.b.block_table + it.seq * a.b.table_stride;
     const int page_size = a.c.page_size, blk = a.c.scale_block;
-    const int64_t page_bytes = static_cast<int64_t>(page_size) * D;
-
     // Look-ups of 32 steps at a time, one step per lane: row of the cache
     // (-1: none), key scale, value scale.
-    int64_t look_row = -1;
+    int look_row = -1;
     float look_k = 0.0f, look_v = 1.0f;
     auto look_up = [&](int i0) {
         look_row = -1;
@@ -338,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention(AttnArgs a, int ta
             const int col = key / page_size, slot = key - col * page_size;
             const int64_t page = col < a.b.table_cols ? __ldg(table + col) : -1;
             if (page >= 0 && page < a.c.num_pages) {
-                const int64_t row = (page * a.c.kv_heads + head) * page_size + slot;
+                const int row = static_cast<int>((page * a.c.kv_heads + head) * page_size + slot);
                 look_row = row;
                 look_k = __ldg(a.c.k_scale + row / blk);
                 look_v = value_scale(__ldg(a.c.v_scale + row / blk));
@@ -350,27 +355,39 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention(AttnArgs a, int ta
 
     const uint32_t ring = smem_u32(smem) + warp * (kStages * S::kStageBytes) + lane * 16;
     const uint32_t ring_v = smem_u32(smem) + warp * (kStages * S::kStageBytes) + kStep * D + lane * VP;
+    const uint8_t *lane_k = a.c.k + g * D + c * 16, *lane_v = a.c.v + 2 * c * D + g * VB;
+    uint32_t put = 0;  // byte offset of the ring stage the next issue fills
     auto issue = [&](int i) {
         if (i < mine) {
-            const int64_t row = __shfl_sync(0xffffffffu, look_row, i & 31);
-            const int key = key0 + i * (kWarps * kStep);
-            const int held = row >= 0 ? sp.len - key : 0;  // slots of the step that hold a token (> 0)
-            const uint32_t st = (i % kStages) * S::kStageBytes;
-            const uint8_t *kp = a.c.k + max(row, static_cast<int64_t>(0)) * D;
-            const uint8_t *vp = a.c.v + max(row, static_cast<int64_t>(0)) * D;
+            const int row = __shfl_sync(0xffffffffu, look_row, i & 31);
+            const int held = row >= 0 ? sp.len - (key0 + i * (kWarps * kStep)) : 0;  // slots of the step that hold a token
+            const int64_t off = static_cast<int64_t>(max(row, 0)) * D;
+            const uint8_t *kp = lane_k + off, *vp = lane_v + off;
+            if (held >= kStep) {
 #pragma unroll
-            for (int nt = 0; nt < 2; ++nt)
+                for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-                for (int j = 0; j < KC; ++j)
-                    cp_async_zfill<16>(ring + st + (nt * KC + j) * 512, kp + (g + 8 * nt) * D + j * 64 + c * 16, g + 8 * nt < held ? 16u : 0u);
+                    for (int j = 0; j < KC; ++j) cp_async<16>(ring + put + (nt * KC + j) * 512, kp + nt * 8 * D + j * 64);
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const int tok = 2 * c + (t & 1) + (t >> 1) * 8;
+                for (int t = 0; t < 4; ++t)
 #pragma unroll
-                for (int j = 0; j < VC; ++j)
-                    cp_async_zfill<VP>(ring_v + st + (t * VC + j) * (32 * VP), vp + tok * D + g * VB + j * VP, tok < held ? VP : 0u);
+                    for (int j = 0; j < VC; ++j)
+                        cp_async<VP>(ring_v + put + (t * VC + j) * (32 * VP), vp + ((t & 1) + (t >> 1) * 8) * D + j * VP);
+            } else {  // the sequence's last step: zeros for the slots that hold nothing
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                    for (int j = 0; j < KC; ++j)
+                        cp_async_zfill<16>(ring + put + (nt * KC + j) * 512, kp + nt * 8 * D + j * 64, g + 8 * nt < held ? 16u : 0u);
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int j = 0; j < VC; ++j)
+                        cp_async_zfill<VP>(ring_v + put + (t * VC + j) * (32 * VP), vp + ((t & 1) + (t >> 1) * 8) * D + j * VP,
+                                           2 * c + (t & 1) + (t >> 1) * 8 < held ? VP : 0u);
             }
         }
+        put = put == (kStages - 1) * S::kStageBytes ? 0 : put + S::kStageBytes;
         cp_async_commit();
     };
 
@@ -378,12 +395,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention(AttnArgs a, int ta
 #pragma unroll
     for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.0f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    bool first_step = true;  // some row has seen no key yet
 
     look_up(0);
     float use_k = look_k, use_v = look_v;  // the batch of look-ups being consumed (the ring runs ahead by less than 32)
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) issue(i);
 
+    uint32_t st = 0;  // the ring stage being consumed
     for (int i = 0; i < mine; ++i) {
         if ((i & 31) == 0 && i > 0) {
             use_k = look_k;
@@ -394,7 +413,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention(AttnArgs a, int ta
         issue(ahead);
         cp_async_wait<kStages - 1>();
         const float ks = __shfl_sync(0xffffffffu, use_k, i & 31), vs = __shfl_sync(0xffffffffu, use_v, i & 31);
-        const uint32_t st = (i % kStages) * S::kStageBytes;
 
         // scores: 16 rows x 16 keys; this lane: rows g, g + 8, keys 2c, 2c + 1 (+ 8)
         float x[2][4];
@@ -407,7 +425,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention(AttnArgs a, int ta
                 const uint32_t w[4] = {kv.x, kv.y, kv.z, kv.w};
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const uint32_t b0 = e4m3x2_to_half2(w[q] & 0xffffu), b1 = e4m3x2_to_half2(w[q] >> 16);
+                    uint32_t b0, b1;
+                    e4m3x4_to_half2(w[q], b0, b1);
                     if constexpr (kQRegs) {
                         mma_f16(x[nt], qf[j * 4 + q], b0, b1);
                     } else {
@@ -419,52 +438,69 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention(AttnArgs a, int ta
             }
         }
         const int key = key0 + i * (kWarps * kStep);
-        const float lvs = __log2f(vs);
+        const float lvs = __log2f(vs), inv_vs = __fdividef(1.0f, vs);
+        const float f0 = fac[0] * ks, f1 = fac[1] * ks;
         const bool edge = key < all_lo || key + kStep - 1 > all_hi;
-        float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const float f = fac[r] * ks;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float &y = x[e >> 1][2 * r + (e & 1)];
-                y = (a.cap != 0.0f ? cap_score(y, f, a.cap) : y * f) + lvs;
-                if (edge) {
-                    const int k = key + (e >> 1) * 8 + 2 * c + (e & 1);
-                    if (k > last[r] || k < first[r]) y = -INFINITY;
-                }
-                top[r] = fmaxf(top[r], y);
-            }
-        }
-        // The maximum moves only when a score passes it by 2^8 (weights stay
-        // far inside fp16's range), so most steps need no exchange.
-        if (__any_sync(0xffffffffu, top[0] > m[0] + 8.0f || top[1] > m[1] + 8.0f)) {
+        float e[2][4], rows_sum[2];
+        // Weights against the running reference maximum, which moves only when
+        // a weight passes 2^8 (halves have room for that): no exchange between
+        // lanes in most steps. The sum of a lane's weights bounds each.
+        bool again = CAP || edge || first_step;
+        if (!again) {
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
+                const float f = r ? f1 : f0, b = lvs - m[r];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) e[r][k] = exp2_approx(fmaf(x[k >> 1][2 * r + (k & 1)], f, b));
+                rows_sum[r] = (e[r][0] + e[r][1]) + (e[r][2] + e[r][3]);
+            }
+            again = __any_sync(0xffffffffu, rows_sum[0] > 256.0f || rows_sum[1] > 256.0f);
+        }
+        if (again) {
+            float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const float f = r ? f1 : f0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    float y = x[k >> 1][2 * r + (k & 1)];
+                    y = CAP ? cap_score(y, f, a.cap) + lvs : fmaf(y, f, lvs);
+                    const int at = key + (k >> 1) * 8 + 2 * c + (k & 1);
+                    e[r][k] = at <= last[r] && at >= first[r] ? y : -INFINITY;
+                    top[r] = fmaxf(top[r], e[r][k]);
+                }
                 top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
                 top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-                const float to = fmaxf(m[r], top[r]);
-                const float f = to == m[r] ? 1.0f : exp2_approx(m[r] - to);  // 0 for the first keys
-                m[r] = to;
-                l[r] *= f;
+            }
+            if (__any_sync(0xffffffffu, top[0] > m[0] + (CAP || edge ? 8.0f : 0.0f) || top[1] > m[1] + (CAP || edge ? 8.0f : 0.0f))) {
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    o[t][2 * r] *= f;
-                    o[t][2 * r + 1] *= f;
+                for (int r = 0; r < 2; ++r) {
+                    const float to = fmaxf(m[r], top[r]);
+                    const float f = to == m[r] ? 1.0f : exp2_approx(m[r] - to);  // 0 for the first keys
+                    m[r] = to;
+                    l[r] *= f;
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        o[t][2 * r] *= f;
+                        o[t][2 * r + 1] *= f;
+                    }
                 }
+                first_step = !__all_sync(0xffffffffu, m[0] > -INFINITY && m[1] > -INFINITY);
+            }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const float base = m[r] == -INFINITY ? 0.0f : m[r];  // nothing seen yet: 2^(-inf - 0) = 0
+#pragma unroll
+                for (int k = 0; k < 4; ++k) e[r][k] = exp2_approx(e[r][k] - base);
+                rows_sum[r] = (e[r][0] + e[r][1]) + (e[r][2] + e[r][3]);
             }
         }
-        const float inv_vs = __fdividef(1.0f, vs);
         uint32_t p[4];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            const float base = m[r] == -INFINITY ? 0.0f : m[r];  // nothing seen yet: 2^(-inf - 0) = 0
-            float e[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) e[k] = exp2_approx(x[k >> 1][2 * r + (k & 1)] - base);
-            l[r] = fmaf((e[0] + e[1]) + (e[2] + e[3]), inv_vs, l[r]);
-            p[r] = half2_bits(e[0], e[1]);
-            p[2 + r] = half2_bits(e[2], e[3]);
+            l[r] = fmaf(rows_sum[r], inv_vs, l[r]);
+            p[r] = half2_bits(e[r][0], e[r][1]);
+            p[2 + r] = half2_bits(e[r][2], e[r][3]);
         }
         // values: words of the lane's four keys, paired per output column
         uint32_t v[4][VW];
@@ -529,11 +565,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention(AttnArgs a, int ta
         for (int w = 0; w < VW; ++w) {
             const uint32_t a0 = __byte_perm(v[0][w], v[1][w], 0x5140), a1 = __byte_perm(v[0][w], v[1][w], 0x7362);
             const uint32_t b0 = __byte_perm(v[2][w], v[3][w], 0x5140), b1 = __byte_perm(v[2][w], v[3][w], 0x7362);
-            mma_f16(o[w * 4], p, e4m3x2_to_half2(a0 & 0xffffu), e4m3x2_to_half2(b0 & 0xffffu));
-            mma_f16(o[w * 4 + 1], p, e4m3x2_to_half2(a0 >> 16), e4m3x2_to_half2(b0 >> 16));
-            mma_f16(o[w * 4 + 2], p, e4m3x2_to_half2(a1 & 0xffffu), e4m3x2_to_half2(b1 & 0xffffu));
-            mma_f16(o[w * 4 + 3], p, e4m3x2_to_half2(a1 >> 16), e4m3x2_to_half2(b1 >> 16));
+            uint32_t ha[4], hb[4];
+            e4m3x4_to_half2(a0, ha[0], ha[1]);
+            e4m3x4_to_half2(a1, ha[2], ha[3]);
+            e4m3x4_to_half2(b0, hb[0], hb[1]);
+            e4m3x4_to_half2(b1, hb[2], hb[3]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mma_f16(o[w * 4 + k], p, ha[k], hb[k]);
         }
+        st = st == (kStages - 1) * S::kStageBytes ? 0 : st + S::kStageBytes;
     }
     cp_async_wait<0>();
 
@@ -709,9 +749,10 @@ int launch_stream(const lcml_kv_attention_desc *d, const AttnArgs &a, int max_ro
     float *ml = p.max_slots ? reinterpret_cast<float *>(ws + w.ml) : nullptr;
     float *o = p.max_slots ? reinterpret_cast<float *>(ws + w.o) : nullptr;
     LCML_CHECK_ARG(p.max_items * d->cache->kv_heads <= 0x7fffffff, "lcml_kv_attention: too much work for one call");
-    int rc = ensure_max_smem(reinterpret_cast<const void *>(k_kv_attention<D>), Shape<D>::kSmem, "kv_attention");
+    auto kern = a.cap != 0.0f ? k_kv_attention<D, true> : k_kv_attention<D, false>;
+    int rc = ensure_max_smem(reinterpret_cast<const void *>(kern), Shape<D>::kSmem, "kv_attention");
     if (rc != LCML_OK) return rc;
-    rc = launch_dependent(k_kv_attention<D>, dim3(static_cast<unsigned>(p.max_items * d->cache->kv_heads)), kThreads, Shape<D>::kSmem, st,
+    rc = launch_dependent(kern, dim3(static_cast<unsigned>(p.max_items * d->cache->kv_heads)), kThreads, Shape<D>::kSmem, st,
                           "kv_attention", a, p.target, max_rows, items, count, ml, o);
     if (rc != LCML_OK || p.max_slots == 0) return rc;
     return launch_dependent(k_kv_attention_join<D>, dim3(static_cast<unsigned>(p.max_joins), d->cache->kv_heads, kRows), 128, 0, st,

@@ -458,10 +458,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
                 const uint32_t cw[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
                 uint32_t h[8];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    h[2 * q] = e4m3x2_to_half2(cw[q] & 0xffffu);
-                    h[2 * q + 1] = e4m3x2_to_half2(cw[q] >> 16);
-                }
+                for (int q = 0; q < 4; ++q) e4m3x4_to_half2(cw[q], h[2 * q], h[2 * q + 1]);
                 const uint32_t row = vb + (ch >> 2) * (kTile * 128) + tok * 128;
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {

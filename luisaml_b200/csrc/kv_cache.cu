@@ -23,7 +23,8 @@ int check_cache(const lcml_kv_cache *c, const char *what) {
     LCML_CHECK_ARG(c->scale_block > 0 && c->scale_block % 16 == 0 && c->page_size % c->scale_block == 0,
                    "%s: scale_block %d is not a multiple of 16 that divides page_size %d", what, c->scale_block, c->page_size);
     LCML_CHECK_ARG(static_cast<int64_t>(c->scale_block) * c->head_dim <= 32768, "%s: scale_block * head_dim exceeds 32768", what);
-    LCML_CHECK_ARG(c->kv_heads <= 4096 && c->page_size <= 65536 && c->num_pages <= 0x7fffffff, "%s: cache extent too large", what);
+    LCML_CHECK_ARG(c->kv_heads <= 4096 && c->page_size <= 65536 && c->num_pages <= 0x7fffffff / (c->kv_heads * static_cast<int64_t>(c->page_size)),
+                   "%s: num_pages * kv_heads * page_size exceeds 2^31 - 1", what);
     if (c->num_pages > 0) {
         LCML_CHECK_ARG(c->k && c->v && c->k_scale && c->v_scale, "%s: null cache pointer", what);
         LCML_CHECK_ARG(aligned(c->k, 16) && aligned(c->v, 16) && aligned(c->k_scale, 4) && aligned(c->v_scale, 4),

@@ -53,6 +53,13 @@ __device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t b) {
     return h;
 }
 
+// The four codes of a word -> two pairs of halves.
+__device__ __forceinline__ void e4m3x4_to_half2(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
+}
+
 // The tensor-core path for long runs of queries (kv_attention_tc.cu).
 bool kv_attention_tc_fits(const lcml_kv_attention_desc *d);
 int kv_attention_tc(const lcml_kv_attention_desc *d, const AttnArgs &a, int min_rows, cudaStream_t st);
