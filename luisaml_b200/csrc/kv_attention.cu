@@ -2,26 +2,34 @@
 // short runs of queries) and the entry points.
 //
 // Rows of a sequence and cache head are its n queries x group heads, r = query
-// * group + head, in tiles of 16 (the M of mma.m16n8k16). A segment is one row
-// tile of one cache head over all the keys it sees, in steps of 16 keys. The
-// batch's segments lie end to end in one list of steps, and every CTA of a
-// grid that fits the machine once takes an equal stretch of it, whatever the
-// lengths: no CTA is idle and none is late. Within a CTA warp w takes steps w,
-// w + kWarps, ...; its ring of copies runs on over segment ends.
+// * group + head, in tiles of 8 or 16. A segment is one row tile of one cache
+// head over all the keys it sees, in steps of 16 keys. The batch's segments
+// lie end to end in one list of steps, and every CTA of a grid that fits the
+// machine once takes an equal stretch of it, whatever the lengths: no CTA is
+// idle and none is late. Within a CTA warp w takes steps w, w + kWarps, ...;
+// its ring of copies runs on over segment ends.
 //
-// Keys and values go from global memory through the per-lane cp.async ring
-// straight into the fragment layout: the dot product's order of d is free, so
-// a lane's key fragments are 16 consecutive bytes of one key row, and a
-// value's output column is free too, so a lane reads consecutive bytes of four
-// value rows and pairs them by byte permutes. Every lane reads back only what
-// it copied itself: no barriers, no bank conflicts. Codes become halves by one
-// exact conversion per pair; the block scales multiply the scores (keys) and
-// join the exponent (values, value_scale()).
+// Both products are computed transposed, S^T = K Q^T and O^T = V^T P^T, with
+// keys and d on the 16-row side of mma.m16n8k16 and 8 query rows on the other:
+// a decode step's 8 rows fill the tile (as the 16-row side they would leave
+// half of it, and half of the accumulators, empty). Keys and values go from
+// global memory through the per-lane cp.async ring straight into the fragment
+// layout: the dot product's order of d is free, so a lane's key fragments are
+// 16 consecutive bytes of two key rows, and O^T's row is free too, so a lane
+// reads consecutive bytes of four value rows and pairs them by byte permutes.
+// Every lane reads back only what it copied itself: no barriers, no bank
+// conflicts. Codes become halves by one exact conversion per pair (mma.sync
+// takes e4m3 operands too, but converts them itself for every use: measured
+// slower); the block scales multiply the scores (keys) and join the exponent
+// (values, value_scale()). P^T reaches its operand layout by one movmatrix per
+// 8 keys.
 //
-// At a segment's end the warps join through shared memory. A segment that lies
-// in several CTAs leaves (m, l, O) per CTA, which k_kv_attention_join merges
-// in list order (deterministic). Where no sequence can be longer than
-// kWholeSteps, a CTA takes whole segments and there is nothing to join.
+// At a segment's end each warp leaves its (m, l, O) in shared memory and goes
+// on; the last of them joins and writes. A segment that lies in several CTAs
+// leaves (m, l, O) per CTA, which k_kv_attention_join merges in list order
+// (deterministic: the warps' shares are joined in warp order by whichever comes
+// last). Where no sequence can be longer than kWholeSteps, a CTA takes whole
+// segments and there is nothing to join.
 //
 // Bound: HBM, 2 head_dim bytes per key and cache head.
 #include "lcml_attention.cuh"
@@ -29,26 +37,40 @@
 namespace lcml {
 namespace {
 
-constexpr int kRows = 16;          // rows per tile
 constexpr int kStep = 16;          // keys per warp step
 constexpr int kMinRange = 32;      // steps a CTA takes at least
 constexpr int kWholeSteps = 64;    // up to here splitting a segment costs more than it gains
 constexpr int kMaxBatch = 1024;    // sequences per launch (the plan's table in shared memory)
 constexpr int kTcRows = 128;       // rows of a sequence from which the tensor-core kernel takes it
 
-template <int D>
+// RG: groups of 8 rows per tile. Two CTAs of 128-register threads per SM where
+// the accumulators leave room for that: the steps' dependent chains want more
+// warps, not more registers.
+template <int D, int RG>
 struct Shape {
-    static constexpr int kWarps = D == 256 ? 4 : 8;
+    static constexpr int kWarps = 8;
     static constexpr int kThreads = kWarps * 32;
-    static constexpr int kCtasPerSm = D == 64 ? 2 : 1;
-    static constexpr int kStages = D == 64 ? 4 : 3;
+    static constexpr int kRows = 8 * RG;                           // rows per tile
+    static constexpr int kCtasPerSm = D * RG <= 128 ? 2 : 1;
+    static constexpr int kStages = D == 64 ? 4 : (D == 128 && RG == 2 ? 4 : 2);
     static constexpr int kStageBytes = 2 * kStep * D;              // per warp
     static constexpr int kRing = kWarps * kStages * kStageBytes;
-    static constexpr int kJoin = kWarps * kRows * D * 4;           // the warps' O
-    static constexpr int kQ = D == 256 ? kRows * D * 2 : 0;        // Q as halves, fragment order (in registers below 256)
+    static constexpr int kShare = kRows * D;                       // floats of one warp's O
+    static constexpr int kJoin = kWarps * kShare * 4;
     static constexpr int kPlan = kMaxBatch * 12 + 16;              // first step and steps per segment of each sequence
-    static constexpr int kSmem = kRing + kJoin + kQ + kPlan;
+    static constexpr int kSmem = kRing + kJoin + kPlan;
 };
+
+// Where 16-byte chunk q of row r of a warp's share lies: rows of D floats, the
+// chunks of each 128 bytes permuted so that neither the fragment-order stores
+// (8 lanes: four rows 2c + e, two runs of d) nor the row-order loads (8
+// consecutive chunks) meet in a bank.
+template <int D>
+__device__ __forceinline__ int share_chunk(int r, int q) {
+    const int line = q >> 3, c = (r >> 1) & 3;
+    const int turn = D == 64 ? (c & 1) | (c >> 1) << 2 : (D == 128 ? c : c | (line & 1) << 2);
+    return r * (D / 4) + line * 8 + ((q & 7) ^ turn);
+}
 
 // A segment cut by CTA boundaries: CTAs first .. first + pieces - 1 hold its pieces.
 struct JoinItem {
@@ -64,6 +86,7 @@ struct Span {
 
 // Sequence s; steps counts from lo over all the keys any of its queries sees
 // (at least one step, so that a row without keys still gets its zeros).
+template <int ROWS>
 __device__ __forceinline__ Span span_of(const AttnArgs &a, int s) {
     Span r;
     r.t0 = __ldg(a.b.cu_tokens + s);
@@ -76,7 +99,7 @@ __device__ __forceinline__ Span span_of(const AttnArgs &a, int s) {
     const int64_t first = static_cast<int64_t>(r.pos0) - a.window + 1;  // the first query's oldest key
     r.lo = a.window > 0 && first > 0 ? static_cast<int>(first) & ~(kStep - 1) : 0;
     r.steps = max(1, (r.len - r.lo + kStep - 1) / kStep);
-    r.tiles = static_cast<int>((static_cast<int64_t>(r.n) * a.group + kRows - 1) / kRows);
+    r.tiles = static_cast<int>((static_cast<int64_t>(r.n) * a.group + ROWS - 1) / ROWS);
     return r;
 }
 
@@ -117,9 +140,30 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// Transpose of an 8x8 matrix of halves held as fragments (lane: row g, columns 2c, 2c + 1).
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
 __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Bounded wait of a warp until another has set *flag (shared memory) to `value`.
+__device__ __forceinline__ bool wait_for(const int *flag, int value, int *err) {
+    const volatile int *f = flag;
+    bool ok = true;
+    if (*f != value) {
+        const long long t0 = clock64();
+        while (*f != value && ok) ok = clock64() - t0 <= kWaitLimitCycles;
+        if (!ok) record_device_error(err, kDevTimeoutEpilogue);
+    }
+    ok = __all_sync(0xffffffffu, ok);
+    __threadfence_block();
+    return ok;
 }
 
 // Bytes of w that hold a NaN code (0x7f or 0xff), as the e4m3 code of 1.0 there and 0 elsewhere.
@@ -132,22 +176,23 @@ __device__ __forceinline__ uint32_t nan_cleared(uint32_t w) {
     return w & ~((m >> 7) * 0xffu);
 }
 
-template <int D, bool CAP>
-__global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtasPerSm) k_kv_attention(AttnArgs a, int max_rows, bool whole, int part_rows,
+template <int D, int RG, bool BF16, bool CAP>
+__global__ void __launch_bounds__(Shape<D, RG>::kThreads, Shape<D, RG>::kCtasPerSm) k_kv_attention(AttnArgs a, int max_rows, bool whole, int part_rows,
                                                                                           JoinItem *join_items, float *part_ml, float *part_o) {
-    using S = Shape<D>;
-    constexpr int kWarps = S::kWarps, kThreads = S::kThreads, kStages = S::kStages;
+    using S = Shape<D, RG>;
+    constexpr int kWarps = S::kWarps, kThreads = S::kThreads, kStages = S::kStages, kRows = S::kRows;
     constexpr int KC = D / 64;        // 16-byte pieces of a key row per lane
     constexpr int VB = D / 8;         // bytes of a value row per lane
     constexpr int VP = VB >= 16 ? 16 : 8;
     constexpr int VC = VB / VP;       // pieces of a value row per lane
     constexpr int VW = VB / 4;        // words of a value row per lane
-    constexpr int NT = D / 8;         // output tiles of 8 columns
+    constexpr int MT = D / 16;        // tiles of 16 d of O^T
     constexpr int KK = D / 16;        // k-steps of the dot product
-    constexpr bool kQRegs = S::kQ == 0;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float join_m[kWarps][kRows], join_l[kWarps][kRows];
+    __shared__ int join_count, join_done;  // shares left of the segment, and segments joined
     __shared__ int64_t scan[kWarps];
+    if (threadIdx.x == 0) join_count = join_done = 0;  // ordered by the plan's barriers
 
     griddep_wait();
     griddep_launch_dependents();  // the join waits for this grid's end; its CTAs only become resident early
@@ -159,7 +204,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtasPerSm) k_kv
     // The plan: where each sequence's steps begin in the list, and the steps
     // of its segments. Sequences of more than max_rows rows are left to the
     // other kernel (no segments).
-    int64_t *plan_first = reinterpret_cast<int64_t *>(smem + S::kRing + S::kJoin + S::kQ);  // [batch + 1]
+    int64_t *plan_first = reinterpret_cast<int64_t *>(smem + S::kRing + S::kJoin);  // [batch + 1]
     int *plan_steps = reinterpret_cast<int *>(plan_first + kMaxBatch + 1);                     // [batch]
     {
         int64_t total = 0;
@@ -167,7 +212,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtasPerSm) k_kv
             const int s = s0 + threadIdx.x;
             int64_t mine = 0;
             if (s < batch) {
-                const Span p = span_of(a, s);
+                const Span p = span_of<kRows>(a, s);
                 if (p.cut && blockIdx.x == 0) record_device_error(a.err, kDevBadBatch);
                 if (static_cast<int64_t>(p.n) * a.group <= max_rows) mine = static_cast<int64_t>(p.tiles) * heads * p.steps;
                 plan_steps[s] = p.steps;
@@ -226,13 +271,14 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtasPerSm) k_kv
     // (-1: nothing to load), slots that hold a token, key scale, value scale
     // (0: no row sees the step).
     const int page_size = a.c.page_size, blk = a.c.scale_block;
-    const int count = to - from > warp ? static_cast<int>((to - from - warp + kWarps - 1) / kWarps) : 0;  // this warp's steps
-    int look_row = -1, look_held = 0;
-    float look_k = 0.0f, look_v = 0.0f;
+    const int span = static_cast<int>(to - from);  // positions below are relative to `from`
+    const int count = span > warp ? (span - warp + kWarps - 1) / kWarps : 0;  // this warp's steps
+    struct Look {
+        int row, held;
+        float k, v;
+    };
     auto look_up = [&](int i0) {
-        look_row = -1;
-        look_held = 0;
-        look_k = look_v = 0.0f;
+        Look r{-1, 0, 0.0f, 0.0f};
         const int i = i0 + lane;
         if (i < count) {
             const int64_t p = from + warp + static_cast<int64_t>(i) * kWarps;
@@ -241,7 +287,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtasPerSm) k_kv
             const int64_t in = p - plan_first[s];
             const int th = static_cast<int>(in / steps), st = static_cast<int>(in - static_cast<int64_t>(th) * steps);
             const int tile = th / heads, head = th - tile * heads;
-            const Span sp = span_of(a, s);
+            const Span sp = span_of<kRows>(a, s);
             const int key = sp.lo + st * kStep;
             const int row_a = tile * kRows / a.group, row_z = (min(tile * kRows + kRows, sp.n * a.group) - 1) / a.group;
             const int hi = a.causal ? min(sp.pos0 + row_z, sp.len - 1) : sp.len - 1, lo = a.window > 0 ? sp.pos0 + row_a - a.window + 1 : 0;
@@ -249,23 +295,26 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtasPerSm) k_kv
                 const int col = key / page_size, slot = key - col * page_size;
                 const int64_t page = __ldg(a.b.block_table + s * a.b.table_stride + col);  // key < len <= the table's reach
                 if (page >= 0 && page < a.c.num_pages) {
-                    look_row = static_cast<int>((page * heads + head) * page_size + slot);
-                    look_held = sp.len - key;
-                    look_k = __ldg(a.c.k_scale + look_row / blk);
-                    look_v = value_scale(__ldg(a.c.v_scale + look_row / blk));
+                    r.row = static_cast<int>((page * heads + head) * page_size + slot);
+                    r.held = sp.len - key;
+                    r.k = __ldg(a.c.k_scale + r.row / blk);
+                    r.v = value_scale(__ldg(a.c.v_scale + r.row / blk));
                 } else {
                     record_device_error(a.err, kDevBadPage);
                 }
             }
         }
+        return r;
     };
 
     const uint32_t ring = smem_u32(smem) + warp * (kStages * S::kStageBytes) + lane * 16;
     const uint32_t ring_v = smem_u32(smem) + warp * (kStages * S::kStageBytes) + kStep * D + lane * VP;
     const uint8_t *lane_k = a.c.k + g * D + c * 16, *lane_v = a.c.v + 2 * c * D + g * VB;
     uint32_t put = 0;  // byte offset of the ring stage the next issue fills
+    Look cur, next = look_up(0);  // the batch being consumed, and the one being issued (the ring runs ahead by less than 32)
+    cur = next;
     auto issue = [&](int i) {
-        const int row = __shfl_sync(0xffffffffu, look_row, i & 31), held = __shfl_sync(0xffffffffu, look_held, i & 31);
+        const int row = __shfl_sync(0xffffffffu, next.row, i & 31), held = __shfl_sync(0xffffffffu, next.held, i & 31);
         if (row >= 0) {
             const int64_t off = static_cast<int64_t>(row) * D;
             const uint8_t *kp = lane_k + off, *vp = lane_v + off;
@@ -297,8 +346,6 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtasPerSm) k_kv
         cp_async_commit();
     };
 
-    look_up(0);
-    float use_k = look_k, use_v = look_v;  // the batch of look-ups being consumed (the ring runs ahead by less than 32)
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) issue(i);
     uint32_t st = 0;  // the ring stage being consumed
@@ -306,30 +353,31 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtasPerSm) k_kv
 
     int seq = sequence_at(from);
     int th = static_cast<int>((from - plan_first[seq]) / plan_steps[seq]);  // segment of the sequence: tile * heads + head
-    for (int64_t at = from; at < to;) {
-        while (plan_first[seq + 1] <= at) {
+    int segment = 0;  // how many segments this CTA has left behind
+    bool give_up = false;
+    for (int at = 0; at < span;) {
+        while (plan_first[seq + 1] <= from + at) {
             ++seq;
             th = 0;
         }
-        const Span sp = span_of(a, seq);
+        const Span sp = span_of<kRows>(a, seq);
         const int tile = th / heads, head = th - tile * heads;
-        const int64_t seg = plan_first[seq] + static_cast<int64_t>(th) * sp.steps;  // the segment's first step
-        const int64_t end = min(seg + sp.steps, to);
+        const int seg = static_cast<int>(plan_first[seq] + static_cast<int64_t>(th) * sp.steps - from);  // the segment's first step
+        const int end = min(seg + sp.steps, span);
         const int rows = min(kRows, sp.n * a.group - tile * kRows);
 
-        // Q fragments: a0: row g, first pair; a1: row g + 8, first pair; a2:
-        // row g, second pair; a3. A lane's elements of a row are 16
-        // consecutive ones of every 64. A bf16 row is multiplied by a power
-        // of two first (exact), so its largest element is in [1, 2) and
-        // fp16's range covers it.
-        uint32_t qf[KK][4];
-        float fac[2];
-        int last[2], first[2];
+        // Q^T fragments: row g (+ 8), b0 and b1 the d of a key word's two pairs.
+        // A lane's elements of a row are 16 consecutive ones of every 64. A
+        // bf16 row is multiplied by a power of two first (exact), so its
+        // largest element is in [1, 2) and fp16's range covers it.
+        uint32_t qf[RG][KK][2];
+        float fac[RG][2];  // of rows 2c, 2c + 1 (+ 8), as the scores lie
+        int last[RG][2], first[RG][2];
         {
             const bool vec = aligned(a.q, 16) && a.q_token_stride % 8 == 0 && a.q_head_stride % 8 == 0;
 #pragma unroll
-            for (int r2 = 0; r2 < 2; ++r2) {
-                const int r = g + 8 * r2, row = tile * kRows + r;
+            for (int rg = 0; rg < RG; ++rg) {
+                const int r = g + 8 * rg, row = tile * kRows + r;
                 uint32_t raw[KC][8];
 #pragma unroll
                 for (int j = 0; j < KC; ++j)
@@ -351,7 +399,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtasPerSm) k_kv
                     }
                 }
                 float f = 1.0f;
-                if (a.bf16) {
+                if (BF16) {
                     uint32_t mx = 0;
 #pragma unroll
                     for (int j = 0; j < KC; ++j)
@@ -370,141 +418,145 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtasPerSm) k_kv
                         for (int w = 0; w < 8; ++w)
                             raw[j][w] = half2_bits(__uint_as_float(raw[j][w] << 16) * inv, __uint_as_float(raw[j][w] & 0xffff0000u) * inv);
                 }
+                f *= CAP ? a.inv_cap : a.scale_log2;
 #pragma unroll
                 for (int j = 0; j < KC; ++j)
 #pragma unroll
-                    for (int w = 0; w < 8; ++w) qf[j * 4 + w / 2][(w & 1) * 2 + r2] = raw[j][w];
-                fac[r2] = f * (CAP ? a.inv_cap : a.scale_log2);
-                // rows past the tile's end (zero queries) see what its last row sees; they are not written
-                const int pos = sp.pos0 + (tile * kRows + min(r, rows - 1)) / a.group;
-                last[r2] = a.causal ? min(pos, sp.len - 1) : sp.len - 1;
-                first[r2] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-            }
-        }
-        const uint32_t qs = smem_u32(smem) + S::kRing + S::kJoin;
-        if constexpr (!kQRegs) {  // every warp has the same fragments: one copy for all
+                    for (int w = 0; w < 8; ++w) qf[rg][j * 4 + w / 2][w & 1] = raw[j][w];
 #pragma unroll
-            for (int kk = 0; kk < KK; ++kk)
-                if (kk % kWarps == warp)
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(qs + (kk * 32 + lane) * 16), "r"(qf[kk][0]), "r"(qf[kk][1]),
-                                 "r"(qf[kk][2]), "r"(qf[kk][3])
-                                 : "memory");
-            __syncthreads();
+                for (int e = 0; e < 2; ++e) {
+                    fac[rg][e] = __shfl_sync(0xffffffffu, f, (2 * c + e) * 4);
+                    // rows past the tile's end (zero queries) see what its last row sees; they are not written
+                    const int pos = sp.pos0 + (tile * kRows + min(8 * rg + 2 * c + e, rows - 1)) / a.group;
+                    last[rg][e] = a.causal ? min(pos, sp.len - 1) : sp.len - 1;
+                    first[rg][e] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+                }
+            }
         }
         // keys in [all_lo, all_hi] are seen by every row of the tile
         const int row_a = tile * kRows / a.group, row_z = (tile * kRows + rows - 1) / a.group;
         const int all_hi = a.causal ? min(sp.pos0 + row_a, sp.len - 1) : sp.len - 1;
         const int all_lo = a.window > 0 ? max(0, sp.pos0 + row_z - a.window + 1) : 0;
 
-        float o[NT][4];
+        float o[RG][MT][4];  // O^T: d = g VB + 2 tile (+ 1 in 2, 3), rows 2c, 2c + 1
+        float m[RG][2], l[RG][2];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.0f;
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+        for (int rg = 0; rg < RG; ++rg) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t) o[rg][t][0] = o[rg][t][1] = o[rg][t][2] = o[rg][t][3] = 0.0f;
+            m[rg][0] = m[rg][1] = -INFINITY;
+            l[rg][0] = l[rg][1] = 0.0f;
+        }
         bool first_step = true;  // some row has seen no key yet
 
-        const int stop = end - from > warp ? static_cast<int>((end - from - warp + kWarps - 1) / kWarps) : 0;
+        const int stop = end > warp ? (end - warp + kWarps - 1) / kWarps : 0;
         for (; i < stop; ++i) {
-            if ((i & 31) == 0 && i > 0) {
-                use_k = look_k;
-                use_v = look_v;
-            }
+            if ((i & 31) == 0 && i > 0) cur = next;
             const int ahead = i + kStages - 1;
-            if ((ahead & 31) == 0) look_up(ahead);
+            if ((ahead & 31) == 0) next = look_up(ahead);
             issue(ahead);
             cp_async_wait<kStages - 1>();
             const uint32_t now = st;
             st = st == (kStages - 1) * S::kStageBytes ? 0 : st + S::kStageBytes;
-            const float ks = __shfl_sync(0xffffffffu, use_k, i & 31), vs = __shfl_sync(0xffffffffu, use_v, i & 31);
+            const float ks = __shfl_sync(0xffffffffu, cur.k, i & 31), vs = __shfl_sync(0xffffffffu, cur.v, i & 31);
             if (vs == 0.0f) continue;
-            const int key = sp.lo + static_cast<int>(from + warp + static_cast<int64_t>(i) * kWarps - seg) * kStep;
-            // scores: 16 rows x 16 keys; this lane: rows g, g + 8, keys 2c, 2c + 1 (+ 8)
-            float x[2][4];
+            const int key = sp.lo + (warp + i * kWarps - seg) * kStep;
+            // scores: keys g, g + 8 x rows 2c, 2c + 1 (+ 8)
+            float x[RG][4];
 #pragma unroll
-            for (int nt = 0; nt < 2; ++nt) {
-                x[nt][0] = x[nt][1] = x[nt][2] = x[nt][3] = 0.0f;
+            for (int rg = 0; rg < RG; ++rg) x[rg][0] = x[rg][1] = x[rg][2] = x[rg][3] = 0.0f;
 #pragma unroll
-                for (int j = 0; j < KC; ++j) {
-                    const uint4 kv = lds128(ring + now + (nt * KC + j) * 512);
-                    const uint32_t w[4] = {kv.x, kv.y, kv.z, kv.w};
+            for (int j = 0; j < KC; ++j) {
+                const uint4 k0 = lds128(ring + now + j * 512), k8 = lds128(ring + now + (KC + j) * 512);
+                const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w8[4] = {k8.x, k8.y, k8.z, k8.w};
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        uint32_t b0, b1;
-                        e4m3x4_to_half2(w[q], b0, b1);
-                        if constexpr (kQRegs) {
-                            mma_f16(x[nt], qf[j * 4 + q], b0, b1);
-                        } else {
-                            const uint4 t = lds128(qs + ((j * 4 + q) * 32 + lane) * 16);
-                            const uint32_t af[4] = {t.x, t.y, t.z, t.w};
-                            mma_f16(x[nt], af, b0, b1);
-                        }
-                    }
+                for (int q = 0; q < 4; ++q) {
+                    const uint32_t af[4] = {e4m3x2_to_half2(w0[q]), e4m3x2_to_half2(w8[q]), e4m3x2_to_half2(w0[q] >> 16), e4m3x2_to_half2(w8[q] >> 16)};
+#pragma unroll
+                    for (int rg = 0; rg < RG; ++rg) mma_f16(x[rg], af, qf[rg][j * 4 + q][0], qf[rg][j * 4 + q][1]);
                 }
             }
             const float lvs = __log2f(vs), inv_vs = __fdividef(1.0f, vs);
-            const float f0 = fac[0] * ks, f1 = fac[1] * ks;
             const bool edge = key < all_lo || key + kStep - 1 > all_hi;
-            float e[2][4], rows_sum[2];
-            // Weights against the running reference maximum, which moves only when
-            // a weight passes 2^8 (halves have room for that): no exchange between
-            // lanes in most steps. The sum of a lane's weights bounds each.
+            float e[RG][2][2], rows_sum[RG][2];  // weights [row][key g, g + 8]
+            // Weights against the running reference maximum, which moves only
+            // when a weight passes 2^8 (halves have room for that): no exchange
+            // between lanes in most steps. The sum of a lane's weights bounds
+            // each.
             bool again = CAP || edge || first_step;
             if (!again) {
+                bool over = false;
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const float f = r ? f1 : f0, b = lvs - m[r];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) e[r][k] = exp2_approx(fmaf(x[k >> 1][2 * r + (k & 1)], f, b));
-                    rows_sum[r] = (e[r][0] + e[r][1]) + (e[r][2] + e[r][3]);
-                }
-                again = __any_sync(0xffffffffu, rows_sum[0] > 256.0f || rows_sum[1] > 256.0f);
-            }
-            if (again) {
-                float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const float f = r ? f1 : f0;
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        float y = x[k >> 1][2 * r + (k & 1)];
-                        y = CAP ? cap_score(y, f, a.cap) + lvs : fmaf(y, f, lvs);
-                        const int at = key + (k >> 1) * 8 + 2 * c + (k & 1);
-                        e[r][k] = at <= last[r] && at >= first[r] ? y : -INFINITY;
-                        top[r] = fmaxf(top[r], e[r][k]);
-                    }
-                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-                }
-                if (__any_sync(0xffffffffu, top[0] > m[0] + (CAP || edge ? 8.0f : 0.0f) || top[1] > m[1] + (CAP || edge ? 8.0f : 0.0f))) {
+                for (int rg = 0; rg < RG; ++rg)
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
-                        const float to = fmaxf(m[r], top[r]);
-                        const float f = to == m[r] ? 1.0f : exp2_approx(m[r] - to);  // 0 for the first keys
-                        m[r] = to;
-                        l[r] *= f;
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            o[t][2 * r] *= f;
-                            o[t][2 * r + 1] *= f;
-                        }
+                        const float f = fac[rg][r] * ks, b = lvs - m[rg][r];
+                        e[rg][r][0] = exp2_approx(fmaf(x[rg][r], f, b));
+                        e[rg][r][1] = exp2_approx(fmaf(x[rg][2 + r], f, b));
+                        rows_sum[rg][r] = e[rg][r][0] + e[rg][r][1];
+                        over |= rows_sum[rg][r] > 256.0f;
                     }
-                    first_step = !__all_sync(0xffffffffu, m[0] > -INFINITY && m[1] > -INFINITY);
+                again = __any_sync(0xffffffffu, over);
+            }
+            if (again) {
+                bool over = false;
+                float top[RG][2];
+#pragma unroll
+                for (int rg = 0; rg < RG; ++rg)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const float f = fac[rg][r] * ks;
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const float y = CAP ? cap_score(x[rg][2 * k + r], f, a.cap) + lvs : fmaf(x[rg][2 * k + r], f, lvs);
+                            const int at_key = key + g + 8 * k;
+                            e[rg][r][k] = at_key <= last[rg][r] && at_key >= first[rg][r] ? y : -INFINITY;
+                        }
+                        float t = fmaxf(e[rg][r][0], e[rg][r][1]);
+                        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
+                        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
+                        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
+                        top[rg][r] = t;
+                        over |= t > m[rg][r] + (CAP || edge ? 8.0f : 0.0f);
+                    }
+                if (__any_sync(0xffffffffu, over)) {
+                    bool seen = true;
+#pragma unroll
+                    for (int rg = 0; rg < RG; ++rg)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            const float to_m = fmaxf(m[rg][r], top[rg][r]);
+                            const float f = to_m == m[rg][r] ? 1.0f : exp2_approx(m[rg][r] - to_m);  // 0 for the first keys
+                            m[rg][r] = to_m;
+                            l[rg][r] *= f;
+#pragma unroll
+                            for (int t = 0; t < MT; ++t) {
+                                o[rg][t][r] *= f;
+                                o[rg][t][2 + r] *= f;
+                            }
+                            seen &= to_m > -INFINITY;
+                        }
+                    first_step = !__all_sync(0xffffffffu, seen);
                 }
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const float base = m[r] == -INFINITY ? 0.0f : m[r];  // nothing seen yet: 2^(-inf - 0) = 0
+                for (int rg = 0; rg < RG; ++rg)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) e[r][k] = exp2_approx(e[r][k] - base);
-                    rows_sum[r] = (e[r][0] + e[r][1]) + (e[r][2] + e[r][3]);
-                }
-            }
-            uint32_t p[4];
+                    for (int r = 0; r < 2; ++r) {
+                        const float base = m[rg][r] == -INFINITY ? 0.0f : m[rg][r];  // nothing seen yet: 2^(-inf - 0) = 0
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                l[r] = fmaf(rows_sum[r], inv_vs, l[r]);
-                p[r] = half2_bits(e[r][0], e[r][1]);
-                p[2 + r] = half2_bits(e[r][2], e[r][3]);
+                        for (int k = 0; k < 2; ++k) e[rg][r][k] = exp2_approx(e[rg][r][k] - base);
+                        rows_sum[rg][r] = e[rg][r][0] + e[rg][r][1];
+                    }
             }
-            // values: words of the lane's four keys, paired per output column
+            uint32_t pf[RG][2];  // P^T fragments: row g, keys 2c, 2c + 1 (+ 8)
+#pragma unroll
+            for (int rg = 0; rg < RG; ++rg) {
+#pragma unroll
+                for (int r = 0; r < 2; ++r) l[rg][r] = fmaf(rows_sum[rg][r], inv_vs, l[rg][r]);
+                pf[rg][0] = transpose8x8(half2_bits(e[rg][0][0], e[rg][1][0]));
+                pf[rg][1] = transpose8x8(half2_bits(e[rg][0][1], e[rg][1][1]));
+            }
+            // values: words of keys 2c, 2c + 1, 2c + 8, 2c + 9, paired per d
             uint32_t v[4][VW];
 #pragma unroll
             for (int t = 0; t < 4; ++t)
@@ -522,159 +574,178 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, Shape<D>::kCtasPerSm) k_kv
                         v[t][1] = u.y;
                     }
                 }
+            // bytes 2h, 2h + 1 of word w: d of tile 2w + h
+            auto value_tile = [&](const uint32_t(&from_v)[4][VW], int w, int h, uint32_t(&af)[4]) {
+                const uint32_t lo = h ? 0x0062u : 0x0040u, hi = h ? 0x0073u : 0x0051u;
+                af[0] = e4m3x2_to_half2(__byte_perm(from_v[0][w], from_v[1][w], lo));
+                af[1] = e4m3x2_to_half2(__byte_perm(from_v[0][w], from_v[1][w], hi));
+                af[2] = e4m3x2_to_half2(__byte_perm(from_v[2][w], from_v[3][w], lo));
+                af[3] = e4m3x2_to_half2(__byte_perm(from_v[2][w], from_v[3][w], hi));
+            };
             if (edge) {
-                // A NaN among the values of a key that some row does not see must
-                // not reach that row through 0 * NaN: count, per row and column,
-                // the seen keys with a NaN there, and clear the codes.
+                // A NaN among the values of a key that some row does not see
+                // must not reach that row through 0 * NaN: count, per row and
+                // d, the seen keys with a NaN there, and clear the codes.
                 uint32_t any = 0;
 #pragma unroll
                 for (int t = 0; t < 4; ++t)
 #pragma unroll
                     for (int w = 0; w < VW; ++w) any |= nan_ones(v[t][w]);
                 if (__any_sync(0xffffffffu, any != 0)) {
-                    uint32_t see[4];
+                    uint32_t ones[4][VW];
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        float f[4];
+                    for (int t = 0; t < 4; ++t)
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const int j = key + (k >> 1) * 8 + 2 * c + (k & 1);
-                            f[k] = j <= last[r] && j >= first[r] ? 1.0f : 0.0f;
-                        }
-                        see[r] = half2_bits(f[0], f[1]);
-                        see[2 + r] = half2_bits(f[2], f[3]);
-                    }
-#pragma unroll
-                    for (int w = 0; w < VW; ++w) {
-                        const uint32_t n0 = nan_ones(v[0][w]), n1 = nan_ones(v[1][w]), n2 = nan_ones(v[2][w]), n3 = nan_ones(v[3][w]);
-                        const uint32_t a0 = __byte_perm(n0, n1, 0x5140), a1 = __byte_perm(n0, n1, 0x7362);
-                        const uint32_t b0 = __byte_perm(n2, n3, 0x5140), b1 = __byte_perm(n2, n3, 0x7362);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            float cnt[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                            const uint32_t wa = k < 2 ? a0 : a1, wb = k < 2 ? b0 : b1;
-                            mma_f16(cnt, see, e4m3x2_to_half2((wa >> ((k & 1) * 16)) & 0xffffu), e4m3x2_to_half2((wb >> ((k & 1) * 16)) & 0xffffu));
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                if (cnt[e] > 0.0f) o[w * 4 + k][e] = NAN;
+                        for (int w = 0; w < VW; ++w) {
+                            ones[t][w] = nan_ones(v[t][w]);
+                            v[t][w] = nan_cleared(v[t][w]);
                         }
 #pragma unroll
-                        for (int t = 0; t < 4; ++t) v[t][w] = nan_cleared(v[t][w]);
+                    for (int rg = 0; rg < RG; ++rg) {
+                        const int pos = sp.pos0 + (tile * kRows + min(8 * rg + g, rows - 1)) / a.group;
+                        const int hi = a.causal ? min(pos, sp.len - 1) : sp.len - 1, lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+                        float see[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const int at_key = key + 2 * c + (k & 1) + (k >> 1) * 8;
+                            see[k] = at_key <= hi && at_key >= lo ? 1.0f : 0.0f;
+                        }
+                        const uint32_t s0 = half2_bits(see[0], see[1]), s1 = half2_bits(see[2], see[3]);
+#pragma unroll
+                        for (int t = 0; t < MT; ++t) {
+                            uint32_t af[4];
+                            float count_nan[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            value_tile(ones, t / 2, t % 2, af);
+                            mma_f16(count_nan, af, s0, s1);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                if (count_nan[k] > 0.0f) o[rg][t][k] = NAN;
+                        }
                     }
                 }
             }
 #pragma unroll
-            for (int w = 0; w < VW; ++w) {
-                const uint32_t a0 = __byte_perm(v[0][w], v[1][w], 0x5140), a1 = __byte_perm(v[0][w], v[1][w], 0x7362);
-                const uint32_t b0 = __byte_perm(v[2][w], v[3][w], 0x5140), b1 = __byte_perm(v[2][w], v[3][w], 0x7362);
-                uint32_t ha[4], hb[4];
-                e4m3x4_to_half2(a0, ha[0], ha[1]);
-                e4m3x4_to_half2(a1, ha[2], ha[3]);
-                e4m3x4_to_half2(b0, hb[0], hb[1]);
-                e4m3x4_to_half2(b1, hb[2], hb[3]);
+            for (int t = 0; t < MT; ++t) {
+                uint32_t af[4];
+                value_tile(v, t / 2, t % 2, af);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) mma_f16(o[w * 4 + k], p, ha[k], hb[k]);
+                for (int rg = 0; rg < RG; ++rg) mma_f16(o[rg][t], af, pf[rg][0], pf[rg][1]);
             }
         }
 
-        // Join the warps: O in fragment order [warp][tile * 4 + reg][lane], the valid rows' lanes.
+        // Leave this warp's share, m, l and the valid rows of O, once the last
+        // segment's have been joined (after a wait that was given up nothing
+        // more is left or written).
+        give_up = give_up || !wait_for(&join_done, segment, a.err);
+        float4 *share = reinterpret_cast<float4 *>(smem + S::kRing) + warp * (S::kShare / 4);
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-            if (c == 0) {
-                join_m[warp][g + 8 * r] = m[r];
-                join_l[warp][g + 8 * r] = l[r];
-            }
-        }
-        float *all_o = reinterpret_cast<float *>(smem + S::kRing);
-        {
-            float *os = all_o + warp * (kRows * D) + lane;
-            if (g < rows) {
+        for (int rg = 0; rg < RG; ++rg)
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    os[t * 128] = o[t][0];
-                    os[t * 128 + 32] = o[t][1];
+            for (int e = 0; e < 2; ++e) {
+                float sum = l[rg][e];
+                sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+                const int r = 8 * rg + 2 * c + e;
+                if (r < rows && !give_up) {
+                    if (g == 0) {
+                        join_m[warp][r] = m[rg][e];
+                        join_l[warp][r] = sum;
+                    }
+#pragma unroll
+                    for (int k = 0; k < MT / 2; ++k)
+                        share[share_chunk<D>(r, g * (MT / 2) + k)] =
+                            make_float4(o[rg][2 * k][e], o[rg][2 * k][2 + e], o[rg][2 * k + 1][e], o[rg][2 * k + 1][2 + e]);
                 }
             }
-            if (g + 8 < rows) {
+        __threadfence_block();
+        __syncwarp();
+        int before = 0;
+        if (lane == 0 && !give_up) before = atomicAdd(&join_count, 1);
+        before = __shfl_sync(0xffffffffu, before, 0);
+        if (before == kWarps - 1) {  // the last: join the shares in warp order and write
+            __threadfence_block();
+            const bool cut = seg < 0 || seg + sp.steps > span;
+            const float4 *all = reinterpret_cast<const float4 *>(smem + S::kRing);
+            constexpr int LPR = D / 4 < 32 ? D / 4 : 32, RPW = 32 / LPR, CPL = D / 4 / LPR;  // lanes per row, rows at once, chunks per lane
+            for (int r0 = 0; r0 < rows; r0 += RPW) {
+                const int r = r0 + lane / LPR;
+                if (r < rows) {
+                    float top = -INFINITY;
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    os[t * 128 + 64] = o[t][2];
-                    os[t * 128 + 96] = o[t][3];
-                }
-            }
-        }
-        __syncthreads();
-        // A thread takes runs of consecutive columns of one row: lane and reg e
-        // give the row and VB columns, cut into kParts runs over the warps.
-        constexpr int kParts = kWarps / 4, kRun = NT / kParts;
-        const int part = warp / 4, e = warp & 3;
-        const int r = g + 8 * (e >> 1);
-        if (r < rows) {
-            float top = -INFINITY;
+                    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, join_m[w][r]);
+                    float sum = 0.0f;
+                    float4 acc[CPL];
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, join_m[w][r]);
-            float wt[kWarps], sum = 0.0f;
+                    for (int k = 0; k < CPL; ++k) acc[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                wt[w] = join_m[w][r] == -INFINITY ? 0.0f : exp2_approx(join_m[w][r] - top);
-                sum = fmaf(wt[w], join_l[w][r], sum);
-            }
-            const bool cut = seg < from || seg + sp.steps > to;
-            const int d0 = (2 * c + (e & 1)) * VB + part * kRun;
-            const float inv = 1.0f / sum;
-            const int row = tile * kRows + r;
-            const int64_t token = sp.t0 + row / a.group;
-            const int qh = head * a.group + row % a.group;
-            const int64_t off = token * a.out_token_stride + qh * a.out_head_stride + d0;
-            const int64_t slot = (2 * static_cast<int64_t>(blockIdx.x) + (seg < from ? 0 : 1)) * part_rows + r;
+                    for (int w = 0; w < kWarps; ++w) {
+                        const float wt = join_m[w][r] == -INFINITY ? 0.0f : exp2_approx(join_m[w][r] - top);
+                        sum = fmaf(wt, join_l[w][r], sum);
 #pragma unroll
-            for (int t0 = 0; t0 < kRun; t0 += 4) {
-                float acc[4];
+                        for (int k = 0; k < CPL; ++k) {
+                            const float4 v = all[w * (S::kShare / 4) + share_chunk<D>(r, k * LPR + lane % LPR)];
+                            acc[k].x = fmaf(wt, v.x, acc[k].x);
+                            acc[k].y = fmaf(wt, v.y, acc[k].y);
+                            acc[k].z = fmaf(wt, v.z, acc[k].z);
+                            acc[k].w = fmaf(wt, v.w, acc[k].w);
+                        }
+                    }
+                    const int row = tile * kRows + r;
+                    const int64_t token = sp.t0 + row / a.group;
+                    const int qh = head * a.group + row % a.group;
+                    const int64_t slot = (2 * static_cast<int64_t>(blockIdx.x) + (seg < 0 ? 0 : 1)) * part_rows + r;
+                    const float inv = 1.0f / sum;
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    acc[t] = 0.0f;
+                    for (int k = 0; k < CPL; ++k) {
+                        const int d0 = (k * LPR + lane % LPR) * 4;
+                        if (cut) {
+                            *reinterpret_cast<float4 *>(part_o + slot * D + d0) = acc[k];
+                        } else {
+                            const float y[4] = {acc[k].x, acc[k].y, acc[k].z, acc[k].w};
+                            const int64_t off = token * a.out_token_stride + qh * a.out_head_stride + d0;
 #pragma unroll
-                    for (int w = 0; w < kWarps; ++w)
-                        acc[t] = fmaf(wt[w], all_o[w * (kRows * D) + ((part * kRun + t0 + t) * 4 + e) * 32 + lane], acc[t]);
-                }
-                if (cut) {
-                    *reinterpret_cast<float4 *>(part_o + slot * D + d0 + t0) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-                } else {
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        const float y = sum != 0.0f ? acc[t] * inv : 0.0f;  // NaN sums stay NaN
-                        if (a.bf16) static_cast<__nv_bfloat16 *>(a.out)[off + t0 + t] = __float2bfloat16_rn(y);
-                        else static_cast<__half *>(a.out)[off + t0 + t] = __float2half_rn(y);
+                            for (int t = 0; t < 4; ++t) {
+                                const float z = sum != 0.0f ? y[t] * inv : 0.0f;  // NaN sums stay NaN
+                                if (BF16) static_cast<__nv_bfloat16 *>(a.out)[off + t] = __float2bfloat16_rn(z);
+                                else static_cast<__half *>(a.out)[off + t] = __float2half_rn(z);
+                            }
+                        }
+                    }
+                    if (lane % LPR == 0) {
+                        if (cut) {
+                            part_ml[slot * 2] = top;
+                            part_ml[slot * 2 + 1] = sum;
+                        } else if (a.lse != nullptr) {
+                            a.lse[token * (static_cast<int64_t>(heads) * a.group) + qh] = sum == 0.0f ? -INFINITY : kLn2 * (top + log2f(sum));
+                        }
                     }
                 }
             }
-            if (part == 0 && (e & 1) == 0 && c == 0) {
-                if (cut) {
-                    part_ml[slot * 2] = top;
-                    part_ml[slot * 2 + 1] = sum;
-                } else if (a.lse != nullptr) {
-                    a.lse[token * (static_cast<int64_t>(heads) * a.group) + qh] = sum == 0.0f ? -INFINITY : kLn2 * (top + log2f(sum));
-                }
+            __threadfence_block();
+            __syncwarp();
+            if (lane == 0) {
+                join_count = 0;
+                __threadfence_block();
+                *const_cast<volatile int *>(&join_done) = segment + 1;
             }
         }
         // The CTA in which a cut segment begins names it to the join.
-        if (join_items != nullptr && threadIdx.x == 0 && end == to) {
+        if (join_items != nullptr && threadIdx.x == 0 && end == span) {
             JoinItem it{seq, tile, head, 0};
-            if (seg >= from && seg + sp.steps > to) it.pieces = static_cast<int>((seg + sp.steps - 1) / range) - static_cast<int>(blockIdx.x) + 1;
+            if (seg >= 0 && seg + sp.steps > span) it.pieces = static_cast<int>((from + seg + sp.steps - 1) / range) - static_cast<int>(blockIdx.x) + 1;
             join_items[blockIdx.x] = it;
         }
-        __syncthreads();  // the next segment's O goes where this one's was
         at = end;
         ++th;
+        ++segment;
     }
     cp_async_wait<0>();
 }
 
 // Merges the pieces of one row of a cut segment: grid (CTAs of the streaming
 // kernel) x rows, 128 threads = 4 groups of pieces x 32 runs of columns.
-template <int D>
+template <int D, int RG>
 __global__ void __launch_bounds__(128) k_kv_attention_join(AttnArgs a, int part_rows, const JoinItem *items, const float *part_ml,
                                                            const float *part_o) {
     griddep_launch_dependents();
@@ -682,7 +753,8 @@ __global__ void __launch_bounds__(128) k_kv_attention_join(AttnArgs a, int part_
     const JoinItem it = items[blockIdx.x];
     const int r = blockIdx.y;
     if (it.pieces == 0) return;
-    const Span sp = span_of(a, it.seq);
+    constexpr int kRows = Shape<D, RG>::kRows;
+    const Span sp = span_of<kRows>(a, it.seq);
     const int row = it.tile * kRows + r;
     if (row >= sp.n * a.group) return;
     constexpr int E = D / 32;
@@ -729,6 +801,7 @@ __global__ void __launch_bounds__(128) k_kv_attention_join(AttnArgs a, int part_
 
 // What the host knows without the lengths.
 struct Plan {
+    int groups;     // of 8 rows per tile
     int grid;       // CTAs
     bool whole;     // no sequence reaches kWholeSteps: whole segments, no join
     int part_rows;  // rows of a piece in the workspace
@@ -737,16 +810,17 @@ struct Plan {
 
 Plan make_plan(const lcml_kv_attention_desc *d, int max_rows) {
     const lcml_kv_cache *c = d->cache;
-    const int group = d->q_heads / c->kv_heads;
     int64_t most = d->max_tokens < d->batch->total_tokens ? d->max_tokens : d->batch->total_tokens;
-    most *= group;
+    most *= d->q_heads / c->kv_heads;
     if (most > max_rows) most = max_rows;
+    if (most < 1) most = 1;
     Plan p{};
-    p.grid = sm_count() * (c->head_dim == 64 ? Shape<64>::kCtasPerSm : (c->head_dim == 128 ? Shape<128>::kCtasPerSm : Shape<256>::kCtasPerSm));
+    p.groups = most <= 8 || c->head_dim == 256 ? 1 : 2;
+    p.grid = sm_count() * (c->head_dim * p.groups <= 128 ? 2 : 1);
     const int64_t reach = static_cast<int64_t>(d->batch->table_cols) * c->page_size;  // no sequence is longer
     p.whole = (reach + kStep - 1) / kStep <= kWholeSteps;
     if (p.whole) return p;
-    p.part_rows = static_cast<int>(most < kRows ? (most > 0 ? most : 1) : kRows);
+    p.part_rows = static_cast<int>(most < 8 * p.groups ? most : 8 * p.groups);
     const int64_t rows = 2 * static_cast<int64_t>(p.grid) * p.part_rows;
     p.items = 0;
     p.ml = (p.grid * static_cast<int64_t>(sizeof(JoinItem)) + 15) / 16 * 16;
@@ -755,15 +829,16 @@ Plan make_plan(const lcml_kv_attention_desc *d, int max_rows) {
     return p;
 }
 
-template <int D>
-int launch_stream(const lcml_kv_attention_desc *d, const AttnArgs &args, int max_rows, cudaStream_t st) {
-    const Plan p = make_plan(d, max_rows);
+template <int D, int RG>
+int launch_stream(const lcml_kv_attention_desc *d, const AttnArgs &args, const Plan &p, int max_rows, cudaStream_t st) {
+    using S = Shape<D, RG>;
     uint8_t *ws = static_cast<uint8_t *>(d->workspace);
     JoinItem *items = p.whole ? nullptr : reinterpret_cast<JoinItem *>(ws + p.items);
     float *ml = p.whole ? nullptr : reinterpret_cast<float *>(ws + p.ml);
     float *o = p.whole ? nullptr : reinterpret_cast<float *>(ws + p.o);
-    auto kern = args.cap != 0.0f ? k_kv_attention<D, true> : k_kv_attention<D, false>;
-    int rc = ensure_max_smem(reinterpret_cast<const void *>(kern), Shape<D>::kSmem, "kv_attention");
+    auto kern = args.bf16 ? (args.cap != 0.0f ? k_kv_attention<D, RG, true, true> : k_kv_attention<D, RG, true, false>)
+                          : (args.cap != 0.0f ? k_kv_attention<D, RG, false, true> : k_kv_attention<D, RG, false, false>);
+    int rc = ensure_max_smem(reinterpret_cast<const void *>(kern), S::kSmem, "kv_attention");
     for (int64_t b0 = 0; rc == LCML_OK && b0 < d->batch->batch; b0 += kMaxBatch) {
         AttnArgs a = args;
         const int64_t n = d->batch->batch - b0;
@@ -771,10 +846,10 @@ int launch_stream(const lcml_kv_attention_desc *d, const AttnArgs &args, int max
         a.b.cu_tokens += b0;
         a.b.lengths += b0;
         a.b.block_table += b0 * a.b.table_stride;
-        rc = launch_dependent(kern, dim3(static_cast<unsigned>(p.grid)), Shape<D>::kThreads, Shape<D>::kSmem, st, "kv_attention", a, max_rows, p.whole,
-                              p.part_rows, items, ml, o);
+        rc = launch_dependent(kern, dim3(static_cast<unsigned>(p.grid)), S::kThreads, S::kSmem, st, "kv_attention", a, max_rows, p.whole, p.part_rows,
+                              items, ml, o);
         if (rc == LCML_OK && !p.whole)
-            rc = launch_dependent(k_kv_attention_join<D>, dim3(static_cast<unsigned>(p.grid), static_cast<unsigned>(p.part_rows)), 128, 0, st,
+            rc = launch_dependent(k_kv_attention_join<D, RG>, dim3(static_cast<unsigned>(p.grid), static_cast<unsigned>(p.part_rows)), 128, 0, st,
                                   "kv_attention_join", a, p.part_rows, items, ml, o);
     }
     return rc;
@@ -840,10 +915,11 @@ int lcml_kv_attention(const lcml_kv_attention_desc *d, lcml_stream_t stream) {
         if (rc2 != LCML_OK || min_rows == 0 || d->batch->batch == 1) return rc2;
     }
     const int max_rows = min_rows == 0x7fffffff ? min_rows : min_rows - 1;
+    const Plan p = make_plan(d, max_rows);
     switch (d->cache->head_dim) {
-        case 64: return launch_stream<64>(d, a, max_rows, st);
-        case 128: return launch_stream<128>(d, a, max_rows, st);
-        default: return launch_stream<256>(d, a, max_rows, st);
+        case 64: return p.groups == 1 ? launch_stream<64, 1>(d, a, p, max_rows, st) : launch_stream<64, 2>(d, a, p, max_rows, st);
+        case 128: return p.groups == 1 ? launch_stream<128, 1>(d, a, p, max_rows, st) : launch_stream<128, 2>(d, a, p, max_rows, st);
+        default: return launch_stream<256, 1>(d, a, p, max_rows, st);
     }
 }
 

@@ -7,11 +7,9 @@
 //   S_t = sum over parts p of Q_t,p K_j^T    tcgen05 kind::f8f6f4, fp32 in TMEM
 //   P_t = 2^(S_t scale + log2 s_v - m)       one thread per row, halves in TMEM over S_t
 //   O_t += P_t V_j                           tcgen05 kind::f16, A from TMEM
-// Keys go from global memory to the MMA as they are: a row of q, times a power
-// of two, is split into e4m3 parts hi + lo (+ lo2) whose sum is q exactly (a
-// bf16 has 8 significant bits, two e4m3 parts with 4 each and a sign carry
-// them; an fp16 takes three), down to 2^-17 of the row's largest element. Two
-// e4m3 products cost what one 16-bit product does, and no key is converted.
+// Keys go from global memory to the MMA as they are, against q's e4m3 parts
+// (QScale, split_q). Two e4m3 products cost what one 16-bit product does, and
+// no key is converted.
 // Values are converted to halves (exact) by one warpgroup, from global memory
 // into the MN-major 128-byte-swizzled layout of the B operand: the weights
 // need more range than e4m3 has.
@@ -520,37 +518,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
                 for (int u = 0; u < kPasses; ++u) {
                     const int r = r0 + u * RPW;
                     const uint32_t h[4] = {e8[u].x, e8[u].y, e8[u].z, e8[u].w};
-                    // times 2^(7 - e): the largest element comes to [128, 256);
-                    // a row with an infinity or NaN has NaN scores
-                    const uint32_t top = NP == 2 ? mx[u] << 16 : __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(mx[u]))));
-                    const bool special = top >= 0x7f800000u;
-                    int e = static_cast<int>(top >> 23);
-                    e = top == 0 ? 127 : min(max(e, 8), 253);
-                    const float up = __uint_as_float(static_cast<uint32_t>(254 - e) << 23) * 128.0f;
-                    if (part_lane == 0) sh.row_factor[r] = __uint_as_float(static_cast<uint32_t>(e) << 23) * 0.0078125f;
-                    float x[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const uint32_t bits = i & 1 ? h[i / 2] >> 16 : h[i / 2] & 0xffffu;
-                        x[i] = up * (NP == 2 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(bits))));
-                    }
+                    const QScale<NP> qs(mx[u]);
+                    if (part_lane == 0) sh.row_factor[r] = qs.factor;
+                    uint32_t lo[NP], hi[NP];
+                    split_q<NP>(h[0], h[1], qs, lo);
+                    split_q<NP>(h[2], h[3], qs, hi);
 #pragma unroll
                     for (int p = 0; p < NP; ++p) {
-                        uint32_t c[2];
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) c[i] = cvt_e4m3x2(x[4 * i], x[4 * i + 1]) | (cvt_e4m3x2(x[4 * i + 2], x[4 * i + 3]) << 16);
-                        if (special) c[0] = 0x7f7f7f7fu;
                         const uint32_t at = smem + (t * NP + p) * S::kQPart + kmajor_offset<D>(r & 127, part_lane >> 1) + (part_lane & 1) * 8;
-                        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(c[0]), "r"(c[1]) : "memory");
-                        if (p + 1 < NP) {
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                float f0, f1;
-                                e4m3x2_decode((c[i / 2] >> (16 * (i & 1))) & 0xffffu, f0, f1);
-                                x[2 * i] -= f0;
-                                x[2 * i + 1] -= f1;
-                            }
-                        }
+                        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(lo[p]), "r"(hi[p]) : "memory");
                     }
                 }
                 fence_proxy_async_smem();

@@ -60,6 +60,52 @@ __device__ __forceinline__ void e4m3x4_to_half2(uint32_t w, uint32_t &lo, uint32
         : "r"(w));
 }
 
+// A row of q as e4m3 parts. Times 2^(7 - e) its largest element (exponent e)
+// comes to [128, 256); part 1 is the nearest e4m3 value of that, part 2 the
+// nearest of what is left, and so on. e4m3 has 4 significant bits and the rest
+// has a sign, so two parts are a bf16 (8 bits) exactly and three an fp16 (11),
+// but for elements so small that e4m3's least step (2^-9) rounds them: an
+// error of 2^-10, 2^-17 of the row's largest element. A row with an infinity
+// or NaN becomes NaN.
+template <int NP>
+struct QScale {
+    float up, factor;  // 2^(7 - e) and 2^(e - 7)
+    bool special;
+    // mx: the row's largest magnitude as bits of its type (16-bit floats order
+    // like their bits, NaN above infinity)
+    __device__ __forceinline__ explicit QScale(uint32_t mx) {
+        const uint32_t top = NP == 2 ? mx << 16 : __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(mx))));
+        special = top >= 0x7f800000u;
+        int e = static_cast<int>(top >> 23);
+        e = top == 0 ? 127 : min(max(e, 8), 253);
+        up = __uint_as_float(static_cast<uint32_t>(254 - e) << 23) * 128.0f;
+        factor = __uint_as_float(static_cast<uint32_t>(e) << 23) * 0.0078125f;
+    }
+};
+
+// Four elements (two words of 16-bit floats) -> one word of each part.
+template <int NP>
+__device__ __forceinline__ void split_q(uint32_t w0, uint32_t w1, const QScale<NP> &s, uint32_t (&parts)[NP]) {
+    float x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t w = i < 2 ? w0 : w1, bits = i & 1 ? w >> 16 : w & 0xffffu;
+        x[i] = s.up * (NP == 2 ? __uint_as_float(bits << 16) : __half2float(__ushort_as_half(static_cast<unsigned short>(bits))));
+    }
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+        const uint32_t c = cvt_e4m3x2(x[0], x[1]) | (cvt_e4m3x2(x[2], x[3]) << 16);
+        parts[p] = s.special ? 0x7f7f7f7fu : c;
+        if (p + 1 < NP) {
+            float f[4];
+            e4m3x2_decode(c & 0xffffu, f[0], f[1]);
+            e4m3x2_decode(c >> 16, f[2], f[3]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] -= f[i];
+        }
+    }
+}
+
 // The tensor-core path for long runs of queries (kv_attention_tc.cu).
 bool kv_attention_tc_fits(const lcml_kv_attention_desc *d);
 int kv_attention_tc(const lcml_kv_attention_desc *d, const AttnArgs &a, int min_rows, cudaStream_t st);
