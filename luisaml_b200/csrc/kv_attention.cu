@@ -285,7 +285,8 @@ __global__ void __launch_bounds__(Shape<D, RG>::kThreads, Shape<D, RG>::kCtasPer
             const int s = sequence_at(p);
             const int steps = plan_steps[s];
             const int64_t in = p - plan_first[s];
-            const int th = static_cast<int>(in / steps), st = static_cast<int>(in - static_cast<int64_t>(th) * steps);
+            const int th = in <= 0x7fffffff ? static_cast<int>(in) / steps : static_cast<int>(in / steps);  // 64-bit division is slow
+            const int st = static_cast<int>(in - static_cast<int64_t>(th) * steps);
             const int tile = th / heads, head = th - tile * heads;
             const Span sp = span_of<kRows>(a, s);
             const int key = sp.lo + st * kStep;
@@ -471,7 +472,9 @@ __global__ void __launch_bounds__(Shape<D, RG>::kThreads, Shape<D, RG>::kCtasPer
                 const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w8[4] = {k8.x, k8.y, k8.z, k8.w};
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const uint32_t af[4] = {e4m3x2_to_half2(w0[q]), e4m3x2_to_half2(w8[q]), e4m3x2_to_half2(w0[q] >> 16), e4m3x2_to_half2(w8[q] >> 16)};
+                    uint32_t af[4];
+                    e4m3x4_to_half2(w0[q], af[0], af[2]);
+                    e4m3x4_to_half2(w8[q], af[1], af[3]);
 #pragma unroll
                     for (int rg = 0; rg < RG; ++rg) mma_f16(x[rg], af, qf[rg][j * 4 + q][0], qf[rg][j * 4 + q][1]);
                 }
@@ -576,11 +579,8 @@ __global__ void __launch_bounds__(Shape<D, RG>::kThreads, Shape<D, RG>::kCtasPer
                 }
             // bytes 2h, 2h + 1 of word w: d of tile 2w + h
             auto value_tile = [&](const uint32_t(&from_v)[4][VW], int w, int h, uint32_t(&af)[4]) {
-                const uint32_t lo = h ? 0x0062u : 0x0040u, hi = h ? 0x0073u : 0x0051u;
-                af[0] = e4m3x2_to_half2(__byte_perm(from_v[0][w], from_v[1][w], lo));
-                af[1] = e4m3x2_to_half2(__byte_perm(from_v[0][w], from_v[1][w], hi));
-                af[2] = e4m3x2_to_half2(__byte_perm(from_v[2][w], from_v[3][w], lo));
-                af[3] = e4m3x2_to_half2(__byte_perm(from_v[2][w], from_v[3][w], hi));
+                e4m3x4_to_half2(__byte_perm(from_v[0][w], from_v[1][w], h ? 0x7362u : 0x5140u), af[0], af[1]);
+                e4m3x4_to_half2(__byte_perm(from_v[2][w], from_v[3][w], h ? 0x7362u : 0x5140u), af[2], af[3]);
             };
             if (edge) {
                 // A NaN among the values of a key that some row does not see
