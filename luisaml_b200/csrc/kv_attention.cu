@@ -43,16 +43,16 @@ constexpr int kWholeSteps = 64;    // up to here splitting a segment costs more 
 constexpr int kMaxBatch = 1024;    // sequences per launch (the plan's table in shared memory)
 constexpr int kTcRows = 128;       // rows of a sequence from which the tensor-core kernel takes it
 
-// RG: groups of 8 rows per tile. Two CTAs of 128-register threads per SM where
-// the accumulators leave room for that: the steps' dependent chains want more
-// warps, not more registers.
+// RG: groups of 8 rows per tile. One CTA per SM with a deep ring, two at
+// head_dim 64 (two CTAs of 128-register threads at 128 leave the ring two
+// stages: 66 -> 70 us for 131072 tokens of 8 cache heads).
 template <int D, int RG>
 struct Shape {
     static constexpr int kWarps = 8;
     static constexpr int kThreads = kWarps * 32;
     static constexpr int kRows = 8 * RG;                           // rows per tile
-    static constexpr int kCtasPerSm = D * RG <= 128 ? 2 : 1;
-    static constexpr int kStages = D == 64 ? 4 : (D == 128 && RG == 2 ? 4 : 2);
+    static constexpr int kCtasPerSm = D == 64 ? 2 : 1;
+    static constexpr int kStages = D == 256 ? 2 : 4;
     static constexpr int kStageBytes = 2 * kStep * D;              // per warp
     static constexpr int kRing = kWarps * kStages * kStageBytes;
     static constexpr int kShare = kRows * D;                       // floats of one warp's O
@@ -74,7 +74,10 @@ __device__ __forceinline__ int share_chunk(int r, int q) {
 
 // A segment cut by CTA boundaries: CTAs first .. first + pieces - 1 hold its pieces.
 struct JoinItem {
-    int seq, tile, head, pieces;
+    int pieces, rows;
+    int row0, t0;  // the tile's first row within the sequence, the sequence's first packed token
+    int head;
+    int pad[3];
 };
 
 struct Span {
@@ -313,7 +316,6 @@ __global__ void __launch_bounds__(Shape<D, RG>::kThreads, Shape<D, RG>::kCtasPer
     const uint8_t *lane_k = a.c.k + g * D + c * 16, *lane_v = a.c.v + 2 * c * D + g * VB;
     uint32_t put = 0;  // byte offset of the ring stage the next issue fills
     Look cur, next = look_up(0);  // the batch being consumed, and the one being issued (the ring runs ahead by less than 32)
-    cur = next;
     auto issue = [&](int i) {
         const int row = __shfl_sync(0xffffffffu, next.row, i & 31), held = __shfl_sync(0xffffffffu, next.held, i & 31);
         if (row >= 0) {
@@ -349,6 +351,7 @@ __global__ void __launch_bounds__(Shape<D, RG>::kThreads, Shape<D, RG>::kCtasPer
 
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) issue(i);
+    cur = next;  // not before: this waits for the scales
     uint32_t st = 0;  // the ring stage being consumed
     int i = 0;        // this warp's step
 
@@ -486,7 +489,7 @@ __global__ void __launch_bounds__(Shape<D, RG>::kThreads, Shape<D, RG>::kCtasPer
             // when a weight passes 2^8 (halves have room for that): no exchange
             // between lanes in most steps. The sum of a lane's weights bounds
             // each.
-            bool again = CAP || edge || first_step;
+            bool again = edge || first_step;
             if (!again) {
                 bool over = false;
 #pragma unroll
@@ -494,8 +497,8 @@ __global__ void __launch_bounds__(Shape<D, RG>::kThreads, Shape<D, RG>::kCtasPer
 #pragma unroll
                     for (int r = 0; r < 2; ++r) {
                         const float f = fac[rg][r] * ks, b = lvs - m[rg][r];
-                        e[rg][r][0] = exp2_approx(fmaf(x[rg][r], f, b));
-                        e[rg][r][1] = exp2_approx(fmaf(x[rg][2 + r], f, b));
+                        e[rg][r][0] = exp2_approx(CAP ? cap_score(x[rg][r], f, a.cap) + b : fmaf(x[rg][r], f, b));
+                        e[rg][r][1] = exp2_approx(CAP ? cap_score(x[rg][2 + r], f, a.cap) + b : fmaf(x[rg][2 + r], f, b));
                         rows_sum[rg][r] = e[rg][r][0] + e[rg][r][1];
                         over |= rows_sum[rg][r] > 256.0f;
                     }
@@ -520,7 +523,7 @@ __global__ void __launch_bounds__(Shape<D, RG>::kThreads, Shape<D, RG>::kCtasPer
                         t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 8));
                         t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 16));
                         top[rg][r] = t;
-                        over |= t > m[rg][r] + (CAP || edge ? 8.0f : 0.0f);
+                        over |= t > m[rg][r] + (edge ? 8.0f : 0.0f);
                     }
                 if (__any_sync(0xffffffffu, over)) {
                     bool seen = true;
@@ -732,7 +735,7 @@ __global__ void __launch_bounds__(Shape<D, RG>::kThreads, Shape<D, RG>::kCtasPer
         }
         // The CTA in which a cut segment begins names it to the join.
         if (join_items != nullptr && threadIdx.x == 0 && end == span) {
-            JoinItem it{seq, tile, head, 0};
+            JoinItem it{0, rows, tile * kRows, sp.t0, head, {0, 0, 0}};
             if (seg >= 0 && seg + sp.steps > span) it.pieces = static_cast<int>((from + seg + sp.steps - 1) / range) - static_cast<int>(blockIdx.x) + 1;
             join_items[blockIdx.x] = it;
         }
@@ -752,44 +755,69 @@ __global__ void __launch_bounds__(128) k_kv_attention_join(AttnArgs a, int part_
     griddep_wait();
     const JoinItem it = items[blockIdx.x];
     const int r = blockIdx.y;
-    if (it.pieces == 0) return;
-    constexpr int kRows = Shape<D, RG>::kRows;
-    const Span sp = span_of<kRows>(a, it.seq);
-    const int row = it.tile * kRows + r;
-    if (row >= sp.n * a.group) return;
-    constexpr int E = D / 32;
+    if (it.pieces == 0 || r >= it.rows) return;
+    constexpr int E = D / 32, kAhead = 8;
     __shared__ float red[4][D];
-    __shared__ float red_l[4];
+    __shared__ float red_m[4], red_l[4];
     const int part = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // the first CTA's piece began with the segment (slot 1), the others' before their stretch (slot 0)
     auto at = [&](int k) { return (2 * (static_cast<int64_t>(blockIdx.x) + k) + (k == 0 ? 1 : 0)) * part_rows + r; };
-    float top = -INFINITY;
-    for (int k = lane; k < it.pieces; k += 32) top = fmaxf(top, part_ml[at(k) * 2]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float acc[E], sum = 0.0f;
+    // warp `part` takes pieces part, part + 4, ..., several loads in flight, with a running maximum
+    float top = -INFINITY, acc[E], sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < E; ++j) acc[j] = 0.0f;
-#pragma unroll 4
-    for (int k = part; k < it.pieces; k += 4) {
-        const float mc = part_ml[at(k) * 2], lc = part_ml[at(k) * 2 + 1];
-        const float w = mc == -INFINITY ? 0.0f : exp2_approx(mc - top);
-        sum = fmaf(w, lc, sum);
-        float t[E];
-        load_vec<float, E>(part_o + at(k) * D + lane * E, t);
+    for (int k0 = part; k0 < it.pieces; k0 += 4 * kAhead) {
+        float2 ml[kAhead];
+        float t[kAhead][E];
 #pragma unroll
-        for (int j = 0; j < E; ++j) acc[j] = fmaf(w, t[j], acc[j]);
+        for (int u = 0; u < kAhead; ++u) {
+            const int k = k0 + 4 * u;
+            ml[u] = make_float2(-INFINITY, 0.0f);
+            if (k < it.pieces) {
+                ml[u] = *reinterpret_cast<const float2 *>(part_ml + at(k) * 2);
+                load_vec<float, E>(part_o + at(k) * D + lane * E, t[u]);
+            }
+        }
+        float next = top;
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) next = fmaxf(next, ml[u].x);
+        const float f = next == top ? 1.0f : exp2_approx(top - next);
+        top = next;
+        sum *= f;
+#pragma unroll
+        for (int j = 0; j < E; ++j) acc[j] *= f;
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            if (k0 + 4 * u >= it.pieces) break;
+            const float w = ml[u].x == -INFINITY ? 0.0f : exp2_approx(ml[u].x - top);
+            sum = fmaf(w, ml[u].y, sum);
+#pragma unroll
+            for (int j = 0; j < E; ++j) acc[j] = fmaf(w, t[u][j], acc[j]);
+        }
     }
 #pragma unroll
     for (int j = 0; j < E; ++j) red[part][lane * E + j] = acc[j];
-    if (lane == 0) red_l[part] = sum;
+    if (lane == 0) {
+        red_m[part] = top;
+        red_l[part] = sum;
+    }
     __syncthreads();
-    sum = (red_l[0] + red_l[1]) + (red_l[2] + red_l[3]);
-    const int64_t token = sp.t0 + row / a.group;
+    top = fmaxf(fmaxf(red_m[0], red_m[1]), fmaxf(red_m[2], red_m[3]));
+    float wt[4];
+    sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        wt[k] = red_m[k] == -INFINITY ? 0.0f : exp2_approx(red_m[k] - top);
+        sum = fmaf(wt[k], red_l[k], sum);
+    }
+    const int row = it.row0 + r;
+    const int64_t token = it.t0 + row / a.group;
     const int qh = it.head * a.group + row % a.group;
     const float inv = 1.0f / sum;
     for (int d = threadIdx.x; d < D; d += 128) {
-        const float v = (red[0][d] + red[1][d]) + (red[2][d] + red[3][d]);
+        float v = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v = fmaf(wt[k], red[k][d], v);
         const float y = sum != 0.0f ? v * inv : 0.0f;
         const int64_t off = token * a.out_token_stride + qh * a.out_head_stride + d;
         if (a.bf16) static_cast<__nv_bfloat16 *>(a.out)[off] = __float2bfloat16_rn(y);
@@ -816,7 +844,7 @@ Plan make_plan(const lcml_kv_attention_desc *d, int max_rows) {
     if (most < 1) most = 1;
     Plan p{};
     p.groups = most <= 8 || c->head_dim == 256 ? 1 : 2;
-    p.grid = sm_count() * (c->head_dim * p.groups <= 128 ? 2 : 1);
+    p.grid = sm_count() * (c->head_dim == 64 ? 2 : 1);
     const int64_t reach = static_cast<int64_t>(d->batch->table_cols) * c->page_size;  // no sequence is longer
     p.whole = (reach + kStep - 1) / kStep <= kWholeSteps;
     if (p.whole) return p;
