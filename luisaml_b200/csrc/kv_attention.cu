@@ -40,6 +40,7 @@ namespace {
 constexpr int kStep = 16;          // keys per warp step
 constexpr int kMinRange = 32;      // steps a CTA takes at least
 constexpr int kWholeSteps = 64;    // up to here splitting a segment costs more than it gains
+constexpr int kPad = 16;           // what a segment's set-up and join cost, in steps
 constexpr int kMaxBatch = 1024;    // sequences per launch (the plan's table in shared memory)
 constexpr int kTcRows = 128;       // rows of a sequence from which the tensor-core kernel takes it
 
@@ -87,8 +88,9 @@ struct Span {
     bool cut;  // longer than the call's bounds
 };
 
-// Sequence s; steps counts from lo over all the keys any of its queries sees
-// (at least one step, so that a row without keys still gets its zeros).
+// Sequence s; steps counts from lo over all the keys any of its queries sees,
+// and kPad empty ones: CTAs with many short segments would be late otherwise
+// (and a row without keys still gets its zeros).
 template <int ROWS>
 __device__ __forceinline__ Span span_of(const AttnArgs &a, int s) {
     Span r;
@@ -101,7 +103,7 @@ __device__ __forceinline__ Span span_of(const AttnArgs &a, int s) {
     r.pos0 = r.len - n;
     const int64_t first = static_cast<int64_t>(r.pos0) - a.window + 1;  // the first query's oldest key
     r.lo = a.window > 0 && first > 0 ? static_cast<int>(first) & ~(kStep - 1) : 0;
-    r.steps = max(1, (r.len - r.lo + kStep - 1) / kStep);
+    r.steps = (r.len - r.lo + kStep - 1) / kStep + kPad;
     r.tiles = static_cast<int>((static_cast<int64_t>(r.n) * a.group + ROWS - 1) / ROWS);
     return r;
 }
@@ -639,7 +641,7 @@ __global__ void __launch_bounds__(Shape<D, RG>::kThreads, Shape<D, RG>::kCtasPer
         // Leave this warp's share, m, l and the valid rows of O, once the last
         // segment's have been joined (after a wait that was given up nothing
         // more is left or written).
-        give_up = give_up || !wait_for(&join_done, segment, a.err);
+        if constexpr (RG == 1) give_up = give_up || !wait_for(&join_done, segment, a.err);
         float4 *share = reinterpret_cast<float4 *>(smem + S::kRing) + warp * (S::kShare / 4);
 #pragma unroll
         for (int rg = 0; rg < RG; ++rg)
@@ -663,15 +665,22 @@ __global__ void __launch_bounds__(Shape<D, RG>::kThreads, Shape<D, RG>::kCtasPer
             }
         __threadfence_block();
         __syncwarp();
+        // 8 rows: the last warp to come joins the shares, in warp order, while
+        // the others go on. 16 rows would keep it too long: all warps join two
+        // rows each.
         int before = 0;
-        if (lane == 0 && !give_up) before = atomicAdd(&join_count, 1);
-        before = __shfl_sync(0xffffffffu, before, 0);
-        if (before == kWarps - 1) {  // the last: join the shares in warp order and write
+        if constexpr (RG == 1) {
+            if (lane == 0 && !give_up) before = atomicAdd(&join_count, 1);
+            before = __shfl_sync(0xffffffffu, before, 0);
+        } else {
+            __syncthreads();
+        }
+        if (RG == 2 || before == kWarps - 1) {
             __threadfence_block();
             const bool cut = seg < 0 || seg + sp.steps > span;
             const float4 *all = reinterpret_cast<const float4 *>(smem + S::kRing);
             constexpr int LPR = D / 4 < 32 ? D / 4 : 32, RPW = 32 / LPR, CPL = D / 4 / LPR;  // lanes per row, rows at once, chunks per lane
-            for (int r0 = 0; r0 < rows; r0 += RPW) {
+            for (int r0 = RG == 1 ? 0 : warp * RPW; r0 < rows; r0 += RG == 1 ? RPW : kWarps * RPW) {
                 const int r = r0 + lane / LPR;
                 if (r < rows) {
                     float top = -INFINITY;
@@ -725,12 +734,16 @@ __global__ void __launch_bounds__(Shape<D, RG>::kThreads, Shape<D, RG>::kCtasPer
                     }
                 }
             }
-            __threadfence_block();
-            __syncwarp();
-            if (lane == 0) {
-                join_count = 0;
+            if constexpr (RG == 1) {
                 __threadfence_block();
-                *const_cast<volatile int *>(&join_done) = segment + 1;
+                __syncwarp();
+                if (lane == 0) {
+                    join_count = 0;
+                    __threadfence_block();
+                    *const_cast<volatile int *>(&join_done) = segment + 1;
+                }
+            } else {
+                __syncthreads();
             }
         }
         // The CTA in which a cut segment begins names it to the join.
