@@ -40,7 +40,7 @@ namespace {
 constexpr int kStep = 16;          // keys per warp step
 constexpr int kMinRange = 32;      // steps a CTA takes at least
 constexpr int kWholeSteps = 64;    // up to here splitting a segment costs more than it gains
-constexpr int kPad = 16;           // what a segment's set-up and join cost, in steps
+constexpr int kPad = 24;           // what a segment's set-up and join cost, in steps
 constexpr int kMaxBatch = 1024;    // sequences per launch (the plan's table in shared memory)
 constexpr int kTcRows = 128;       // rows of a sequence from which the tensor-core kernel takes it
 
