@@ -23,7 +23,8 @@ extern "C" {
  *   y = h * w * 1 / sqrt(mean(h^2) + eps)
  *   s = max|y| / 448 per row (1 for an all-zero row; NaN ignored), written to
  *       scale_out [rows]; or, with `scale` (device, one float), s = *scale
- *   q = e4m3(y / s)             (QuantizeLinear, as lcml_fp8_quantize)
+ *   q = e4m3(y / s)             (QuantizeLinear; y / s computed as h * w *
+ *       (1 / sqrt(..) / s), the codec by the rule of the GEMM's epilogues)
  * q and scale_out are the A operand and scale_a (LCML_SCALE_ROW, or TENSOR
  * for a given scale) of lcml_fp8_gemm. The norm is taken of the fp32 sum;
  * h_out receives it rounded to x's type (may alias x or residual; NULL: not

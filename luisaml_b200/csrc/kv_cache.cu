@@ -48,7 +48,9 @@ int check_batch(const lcml_kv_batch *b, const char *what) {
 
 namespace {
 
-constexpr int kUnitThreads = 1024;  // at most: scale_block * head_dim / 32 threads handle a unit
+// scale_block * head_dim / 32 threads handle a unit: at most 1024, mostly 256
+// or fewer (a second set of kernels with four times the registers)
+constexpr int kSmallUnit = 256, kLargeUnit = 1024;
 
 // One unit as a CTA sees it.
 struct Unit {
@@ -94,20 +96,59 @@ struct WriteArgs {
     int *err;
 };
 
-// |x| as ordered bits, non-finite values as 0.
-__device__ __forceinline__ uint32_t abs_bits_finite(float x) {
-    const uint32_t a = __float_as_uint(x) & 0x7fffffffu;
-    return a >= 0x7f800000u ? 0u : a;
-}
-
 constexpr float kMinScale = 7.888609052210118e-31f;  // 2^-100
 
+// quantize_block_fast() of 8 values with packed products and one test of the
+// four bytes of a word: the codes of v * r_lo and v * r_hi agree and none is
+// 0x80 or NaN, or the block takes the exact divide.
+__device__ __forceinline__ void quantize8(const float *v, float s, float r, bool s_ok, uint32_t *w) {
+    const float r_lo = r * 0.99999952316284180f;  // 1 - 2^-21
+    const float r_hi = r * 1.00000047683715820f;  // 1 + 2^-21
+    uint32_t odd = 0;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        float lo[4], hi[4];
+#pragma unroll
+        for (int k = 0; k < 4; k += 2) {
+            fma2(lo[k], lo[k + 1], v[4 * j + k], v[4 * j + k + 1], r_lo, r_lo, 0.0f, 0.0f);
+            fma2(hi[k], hi[k + 1], v[4 * j + k], v[4 * j + k + 1], r_hi, r_hi, 0.0f, 0.0f);
+        }
+        w[j] = cvt_e4m3x2(lo[0], lo[1]) | (cvt_e4m3x2(lo[2], lo[3]) << 16);
+        const uint32_t other = cvt_e4m3x2(hi[0], hi[1]) | (cvt_e4m3x2(hi[2], hi[3]) << 16);
+        // 0x7f + 1 and 0xff + 1 set bit 7 of the low seven bits' sum; a zero magnitude plus 0x7f does not
+        const uint32_t m = w[j] & 0x7f7f7f7fu;
+        odd |= (w[j] ^ other) | ((m + 0x01010101u) & 0x80808080u) | (~(m + 0x7f7f7f7fu) & w[j] & 0x80808080u);
+    }
+    if (odd != 0 || !s_ok) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            w[j] = quantize1(v[4 * j], s) | (quantize1(v[4 * j + 1], s) << 8) | (quantize1(v[4 * j + 2], s) << 16) | (quantize1(v[4 * j + 3], s) << 24);
+    }
+}
+
 // The unit's new values stay in registers (kVpt vectors of 8 per thread)
-// between the maximum and the encoding, so they are read once.
+// between the maximum and the encoding, so they are read once; the next item's
+// are on their way meanwhile.
 constexpr int kVpt = 4;
 
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kUnitThreads) k_kv_cache_write(WriteArgs a) {
+struct Row8 {
+    T e[8];
+    __device__ __forceinline__ void load(const T *p) {
+        if constexpr (VEC && sizeof(T) == 2) {
+            *reinterpret_cast<uint4 *>(e) = __ldcs(reinterpret_cast<const uint4 *>(p));
+        } else if constexpr (VEC) {
+            reinterpret_cast<uint4 *>(e)[0] = __ldcs(reinterpret_cast<const uint4 *>(p));
+            reinterpret_cast<uint4 *>(e)[1] = __ldcs(reinterpret_cast<const uint4 *>(p) + 1);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e[i] = p[i];
+        }
+    }
+};
+
+template <typename T, bool VEC, int THREADS>
+__global__ void __launch_bounds__(THREADS) k_kv_cache_write(WriteArgs a) {
     griddep_launch_dependents();
     griddep_wait();
     __shared__ uint32_t red[2][32];
@@ -117,42 +158,62 @@ __global__ void __launch_bounds__(kUnitThreads) k_kv_cache_write(WriteArgs a) {
     const int shift = d == 64 ? 3 : (d == 128 ? 4 : 5);  // per_row = 1 << shift
     const int nv = (un.hi - un.lo) * per_row;            // vectors of new values
     const int w = threadIdx.x >> 5, l = threadIdx.x & 31, nw = blockDim.x >> 5;
-    int turn = 0;
-    for (int item = blockIdx.y; item < 2 * hk; item += gridDim.y, turn ^= 1) {
+    const int64_t base0 = un.page * hk * a.c.page_size + un.slot;
+    alignas(16) Row8<T, VEC> raw[kVpt];
+    float s_old;
+    auto fetch = [&](int item) {
         const int kv = item >= hk ? 1 : 0, head = item - kv * hk;
-        const T *x = static_cast<const T *>(a.x[kv]);
-        x += un.token * a.token_stride[kv] + head * a.head_stride[kv];
-        const int64_t base = (un.page * hk + head) * a.c.page_size + un.slot;
+        const T *x = static_cast<const T *>(a.x[kv]) + un.token * a.token_stride[kv] + head * a.head_stride[kv];
+#pragma unroll
+        for (int j = 0; j < kVpt; ++j) {
+            const int i = threadIdx.x + j * blockDim.x;
+            if (i < nv) raw[j].load(x + (i >> shift) * a.token_stride[kv] + ((i & (per_row - 1)) << 3));
+        }
+        s_old = un.old > 0 ? (kv ? a.c.v_scale : a.c.k_scale)[(base0 + static_cast<int64_t>(head) * a.c.page_size) / blk] : 0.0f;
+    };
+    int item = blockIdx.y;
+    fetch(item);
+    for (int turn = 0; item < 2 * hk; item += gridDim.y, turn ^= 1) {
+        const int kv = item >= hk ? 1 : 0, head = item - kv * hk;
+        const int64_t base = base0 + static_cast<int64_t>(head) * a.c.page_size;
         uint8_t *codes = (kv ? a.c.v : a.c.k) + base * d;
         float *scale = (kv ? a.c.v_scale : a.c.k_scale) + base / blk;
-        const float s_old = un.old > 0 ? *scale : 0.0f;
         float v[kVpt][8];
-        uint32_t mx = 0;
+        const float had = s_old;
+        float mx = 0.0f;  // fmaxf ignores NaN
 #pragma unroll
         for (int j = 0; j < kVpt; ++j) {
             const int i = threadIdx.x + j * blockDim.x;
             if (i < nv) {
-                const T *p = x + (i >> shift) * a.token_stride[kv] + ((i & (per_row - 1)) << 3);
-                if constexpr (VEC) {
-                    load_vec<T, 8>(p, v[j]);
-                } else {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) v[j][e] = Elem<T>::load(p + e);
+                for (int e = 0; e < 8; e += 2) {
+                    v[j][e] = Elem<T>::load(raw[j].e + e);
+                    v[j][e + 1] = Elem<T>::load(raw[j].e + e + 1);
+                    mx = fmaxf(fmaxf(mx, fabsf(v[j][e])), fabsf(v[j][e + 1]));
                 }
-#pragma unroll
-                for (int e = 0; e < 8; ++e) mx = max(mx, abs_bits_finite(v[j][e]));
             }
         }
-        mx = __reduce_max_sync(0xffffffffu, mx);
-        if (nw > 1) {  // two buffers in turn: one barrier per item
-            if (l == 0) red[turn][w] = mx;
-            __syncthreads();
-            mx = __reduce_max_sync(0xffffffffu, l < nw ? red[turn][l] : 0u);
+        if (mx == INFINITY) {  // an infinity does not count
+            mx = 0.0f;
+#pragma unroll
+            for (int j = 0; j < kVpt; ++j)
+                if (static_cast<int>(threadIdx.x + j * blockDim.x) < nv) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (fabsf(v[j][e]) < INFINITY) mx = fmaxf(mx, fabsf(v[j][e]));
+                }
         }
-        const float amax = __uint_as_float(mx);
+        if (item + gridDim.y < 2 * hk) fetch(item + gridDim.y);
+        uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(mx));  // floats >= 0 order like their bits
+        if (nw > 1) {  // two buffers in turn: one barrier per item
+            if (l == 0) red[turn][w] = bits;
+            __syncthreads();
+            bits = __reduce_max_sync(0xffffffffu, l < nw ? red[turn][l] : 0u);
+        }
+        const float amax = __uint_as_float(bits);
         float s = amax > 0.0f ? fmaxf(__fdiv_rn(amax, 448.0f), kMinScale) : 0.0f;
-        const bool grew = un.old > 0 && s > s_old;
-        s = fmaxf(s, s_old);
+        const bool grew = un.old > 0 && s > had;
+        s = fmaxf(s, had);
         const float div = s > 0.0f ? s : 1.0f;
         const float r = __frcp_rn(div);
         const bool ok = scale_fast_ok(div, r);
@@ -161,7 +222,7 @@ __global__ void __launch_bounds__(kUnitThreads) k_kv_cache_write(WriteArgs a) {
             const int i = threadIdx.x + j * blockDim.x;
             if (i < nv) {
                 uint32_t q[2];
-                quantize_block_fast<8>(v[j], div, r, ok, q);
+                quantize8(v[j], div, r, ok, q);
                 *reinterpret_cast<uint2 *>(codes + (un.lo + (i >> shift)) * d + ((i & (per_row - 1)) << 3)) = make_uint2(q[0], q[1]);
             }
         }
@@ -175,13 +236,13 @@ __global__ void __launch_bounds__(kUnitThreads) k_kv_cache_write(WriteArgs a) {
                 e4m3x2_decode(c.y & 0xffffu, f[4], f[5]);
                 e4m3x2_decode(c.y >> 16, f[6], f[7]);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] *= s_old;
+                for (int e = 0; e < 8; ++e) f[e] *= had;
                 uint32_t q[2];
-                quantize_block_fast<8>(f, div, r, ok, q);
+                quantize8(f, div, r, ok, q);
                 *p = make_uint2(q[0], q[1]);
             }
         }
-        // every thread has its s_old before the barrier above (nw > 1) or in lockstep (one warp)
+        // every thread has read the old scale before the barrier above (nw > 1) or in lockstep (one warp)
         if (nw == 1) __syncwarp();
         if (threadIdx.x == 0) *scale = s;
     }
@@ -194,64 +255,90 @@ struct ReadArgs {
     int *err;
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kUnitThreads) k_kv_cache_read(ReadArgs a) {
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS) k_kv_cache_read(ReadArgs a) {
     griddep_launch_dependents();
     griddep_wait();
     const Unit un = find_unit(a.c, a.b, blockIdx.x, a.err);
     if (un.page < 0) return;
     const int hk = a.c.kv_heads, d = a.c.head_dim, blk = a.c.scale_block;
-    const int shift = d == 64 ? 3 : (d == 128 ? 4 : 5), per_row = 1 << shift;
-    const int nv = (un.hi - un.lo) * per_row;
-    for (int item = blockIdx.y; item < 2 * hk; item += gridDim.y) {
+    const int shift = d == 64 ? 3 : (d == 128 ? 4 : 5);
+    const int nv = (un.hi - un.lo) << shift;
+    // a thread's codes of one item: 16 at a time, twice (blockDim.x * 32 codes cover a unit)
+    constexpr int kPer = kVpt / 2;
+    const int shift16 = shift - 1, per16 = 1 << shift16, n16 = nv >> 1;
+    const int64_t base0 = un.page * hk * a.c.page_size + un.slot;
+    uint4 c[kPer];
+    float s;
+    auto fetch = [&](int item) {
         const int kv = item >= hk ? 1 : 0, head = item - kv * hk;
+        const int64_t base = base0 + static_cast<int64_t>(head) * a.c.page_size;
+        const uint4 *codes = reinterpret_cast<const uint4 *>((kv ? a.c.v : a.c.k) + (base + un.lo) * d);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            const int i = threadIdx.x + j * blockDim.x;
+            if (i < n16) c[j] = __ldg(codes + i);
+        }
+        s = __ldg((kv ? a.c.v_scale : a.c.k_scale) + base / blk);
+    };
+    int item = blockIdx.y;
+    fetch(item);
+    for (; item < 2 * hk; item += gridDim.y) {
+        const int kv = item >= hk ? 1 : 0, head = item - kv * hk;
+        uint4 now[kPer];
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) now[j] = c[j];
+        const float scale = s;
+        if (item + gridDim.y < 2 * hk) fetch(item + gridDim.y);
         if (a.y[kv] == nullptr) continue;
         T *y = static_cast<T *>(a.y[kv]) + (un.token * hk + head) * d;
-        const int64_t base = (un.page * hk + head) * a.c.page_size + un.slot;
-        const uint8_t *codes = (kv ? a.c.v : a.c.k) + (base + un.lo) * d;
-        const float s = __ldg((kv ? a.c.v_scale : a.c.k_scale) + base / blk);
-        for (int i0 = threadIdx.x; i0 < nv; i0 += 4 * blockDim.x) {
-            uint2 c[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int i = i0 + j * blockDim.x;
-                if (i < nv) c[j] = __ldg(reinterpret_cast<const uint2 *>(codes) + i);
-            }
+        for (int j = 0; j < kPer; ++j) {
+            const int i = threadIdx.x + j * blockDim.x;
+            if (i < n16) {
+                const uint32_t cw[4] = {now[j].x, now[j].y, now[j].z, now[j].w};
+                float f[16];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int i = i0 + j * blockDim.x;
-                if (i < nv) {
-                    float f[8];
-                    e4m3x2_decode(c[j].x & 0xffffu, f[0], f[1]);
-                    e4m3x2_decode(c[j].x >> 16, f[2], f[3]);
-                    e4m3x2_decode(c[j].y & 0xffffu, f[4], f[5]);
-                    e4m3x2_decode(c[j].y >> 16, f[6], f[7]);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) f[e] *= s;
-                    store_vec<T, 8>(y + static_cast<int64_t>(i >> shift) * hk * d + ((i & (per_row - 1)) << 3), f);
+                for (int q = 0; q < 4; ++q) {
+                    e4m3x2_decode(cw[q] & 0xffffu, f[4 * q], f[4 * q + 1]);
+                    e4m3x2_decode(cw[q] >> 16, f[4 * q + 2], f[4 * q + 3]);
                 }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) f[e] *= scale;
+                store_vec<T, 16>(y + static_cast<int64_t>(i >> shift16) * hk * d + ((i & (per16 - 1)) << 4), f);
             }
         }
     }
 }
 
+unsigned unit_threads(const lcml_kv_cache *c) { return static_cast<unsigned>(c->scale_block * c->head_dim / (8 * kVpt)); }
+
 // grid.x: units; grid.y: how many CTAs share a unit's 2 * kv_heads items.
-// Enough CTAs to fill the machine a few times over when the units alone do
-// not; otherwise one CTA per unit, which pays the look-ups once.
+// Enough CTAs that the last wave is a small part of all (a CTA's look-ups
+// take longer than an item), otherwise one CTA per unit.
 dim3 unit_grid(const lcml_kv_cache *c, const lcml_kv_batch *b) {
     const int64_t units = b->total_tokens / c->scale_block + 2 * static_cast<int64_t>(b->batch);
-    const int64_t want = 8 * static_cast<int64_t>(sm_count());
-    int64_t y = (want + units - 1) / units;
+    const int64_t per_sm = 2048 / unit_threads(c) < 32 ? 2048 / unit_threads(c) : 32;
+    const int64_t want = 2 * per_sm * static_cast<int64_t>(sm_count());
+    // units that hold tokens: a decode step's second units are empty
+    const int64_t busy = b->total_tokens / c->scale_block + (b->total_tokens < b->batch ? b->total_tokens : b->batch);
+    int64_t y = (want + busy - 1) / busy;
     if (y > 2 * c->kv_heads) y = 2 * c->kv_heads;
     return dim3(static_cast<unsigned>(units), static_cast<unsigned>(y < 1 ? 1 : y));
 }
 
-unsigned unit_threads(const lcml_kv_cache *c) { return static_cast<unsigned>(c->scale_block * c->head_dim / (8 * kVpt)); }
 
 template <typename T>
 int launch_write(const lcml_kv_cache *c, const lcml_kv_batch *b, const WriteArgs &a, bool vec, cudaStream_t st) {
-    return launch_dependent(vec ? k_kv_cache_write<T, true> : k_kv_cache_write<T, false>, unit_grid(c, b), unit_threads(c), 0, st,
-                            "kv_cache_write", a);
+    auto kern = unit_threads(c) <= kSmallUnit ? (vec ? k_kv_cache_write<T, true, kSmallUnit> : k_kv_cache_write<T, false, kSmallUnit>)
+                                              : (vec ? k_kv_cache_write<T, true, kLargeUnit> : k_kv_cache_write<T, false, kLargeUnit>);
+    return launch_dependent(kern, unit_grid(c, b), unit_threads(c), 0, st, "kv_cache_write", a);
+}
+
+template <typename T>
+int launch_read(const lcml_kv_cache *c, const lcml_kv_batch *b, const ReadArgs &a, cudaStream_t st) {
+    auto kern = unit_threads(c) <= kSmallUnit ? k_kv_cache_read<T, kSmallUnit> : k_kv_cache_read<T, kLargeUnit>;
+    return launch_dependent(kern, unit_grid(c, b), unit_threads(c), 0, st, "kv_cache_read", a);
 }
 
 }// namespace
@@ -297,11 +384,9 @@ int lcml_kv_cache_read(const lcml_kv_cache *cache, const lcml_kv_batch *batch, v
     LCML_CHECK_ARG(aligned(k, 16) && aligned(v, 16), "lcml_kv_cache_read: k and v must be 16-byte aligned");
     const ReadArgs a{*cache, *batch, {k, v}, device_error_word()};
     cudaStream_t st = to_cuda(stream);
-    const dim3 grid = unit_grid(cache, batch);
-    const unsigned threads = unit_threads(cache);
-    if (dtype == LCML_DTYPE_FLOAT) return launch_dependent(k_kv_cache_read<float>, grid, threads, 0, st, "kv_cache_read", a);
-    if (dtype == LCML_DTYPE_FLOAT16) return launch_dependent(k_kv_cache_read<__half>, grid, threads, 0, st, "kv_cache_read", a);
-    return launch_dependent(k_kv_cache_read<__nv_bfloat16>, grid, threads, 0, st, "kv_cache_read", a);
+    if (dtype == LCML_DTYPE_FLOAT) return launch_read<float>(cache, batch, a, st);
+    if (dtype == LCML_DTYPE_FLOAT16) return launch_read<__half>(cache, batch, a, st);
+    return launch_read<__nv_bfloat16>(cache, batch, a, st);
 }
 
 }// extern "C"

@@ -26,13 +26,12 @@ struct NormArgs {
 };
 
 // Block-wide (sum, max): every thread gets both.
-__device__ __forceinline__ void block_sum_max(float &sum, uint32_t &mx) {
-    __shared__ float red_s[32];
-    __shared__ uint32_t red_m[32];
+__device__ __forceinline__ void block_sum_max(float &sum, float &mx) {
+    __shared__ float red_s[32], red_m[32];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     }
     const int w = threadIdx.x >> 5, l = threadIdx.x & 31, nw = blockDim.x >> 5;
     if (nw == 1) return;
@@ -42,11 +41,11 @@ __device__ __forceinline__ void block_sum_max(float &sum, uint32_t &mx) {
     }
     __syncthreads();
     sum = l < nw ? red_s[l] : 0.0f;
-    mx = l < nw ? red_m[l] : 0u;
+    mx = l < nw ? red_m[l] : 0.0f;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     }
 }
 
@@ -78,8 +77,7 @@ __global__ void __launch_bounds__(1024) k_rmsnorm_quantize(NormArgs a) {
             }
         }
     }
-    float sum = 0.0f;
-    uint32_t mx = 0;
+    float sum = 0.0f, mx = 0.0f;  // fmaxf ignores NaN
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
         const int i = threadIdx.x + j * blockDim.x;
@@ -88,34 +86,52 @@ __global__ void __launch_bounds__(1024) k_rmsnorm_quantize(NormArgs a) {
                 store_vec<T, E>(static_cast<T *>(a.h_out) + row * a.ldh + static_cast<int64_t>(i) * E, v + j * E);
             float w[E];
             load_vec<W, E>(static_cast<const W *>(a.weight) + static_cast<int64_t>(i) * E, w);
+            if constexpr (E == 1) {
+                sum = fmaf(v[j], v[j], sum);
+                v[j] *= w[0];
+                mx = fmaxf(mx, fabsf(v[j]));
+            } else {
+                float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int k = j * E + e;
-                sum = fmaf(v[k], v[k], sum);
-                v[k] *= w[e];
-                mx = max(mx, abs_bits_nan0(v[k]));
+                for (int e = 0; e < E; e += 2) {
+                    float &v0 = v[j * E + e], &v1 = v[j * E + e + 1];
+                    fma2(s0, s1, v0, v1, v0, v1, s0, s1);
+                    mul2(v0, v1, v0, v1, w[e], w[e + 1]);
+                    mx = fmaxf(fmaxf(mx, fabsf(v0)), fabsf(v1));
+                }
+                sum += s0 + s1;
             }
         }
     }
     block_sum_max(sum, mx);
     const float r = rsqrtf(sum / static_cast<float>(a.cols) + a.eps);
-    const float s = a.scale != nullptr ? __ldg(a.scale) : scale_from_amax(__uint_as_float(mx) * r);
+    const float s = a.scale != nullptr ? __ldg(a.scale) : scale_from_amax(mx * r);
     if (a.scale_out != nullptr && threadIdx.x == 0) a.scale_out[row] = s;
-    const float rs = __frcp_rn(s);
-    const bool ok = scale_fast_ok(s, rs);
+    // y / s as h w (r / s): one product per element, and the codec by the rule
+    // of the fused GEMM epilogues (quantize_block_rcp). It differs from a
+    // division only where y / s lies within a few fp32 ulps of an e4m3
+    // boundary, as y itself is uncertain by the order of its sum.
+    const float f = r * __frcp_rn(s);
+    const bool ok = scale_fast_ok(s, f);
     uint8_t *q = a.q + row * a.cols;
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
         const int i = threadIdx.x + j * blockDim.x;
         if (i < nv) {
-            float y[E];
-#pragma unroll
-            for (int e = 0; e < E; ++e) y[e] = v[j * E + e] * r;
             if constexpr (E == 1) {
-                q[i] = static_cast<uint8_t>(quantize2_fast(y[0], y[0], s, rs, ok));
+                q[i] = static_cast<uint8_t>(ok ? quantize_rcp1(v[j], f) : quantize1(v[j] * r, s));
             } else {
                 uint32_t c[E / 4];
-                quantize_block_fast<E>(y, s, rs, ok, c);
+                if (ok) {
+                    quantize_block_rcp<E>(v + j * E, f, c);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < E / 4; ++k) {
+                        c[k] = 0;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) c[k] |= quantize1(v[j * E + k * 4 + e] * r, s) << (8 * e);
+                    }
+                }
                 if constexpr (E == 8) *reinterpret_cast<uint2 *>(q + static_cast<int64_t>(i) * 8) = make_uint2(c[0], c[1]);
                 else *reinterpret_cast<uint32_t *>(q + static_cast<int64_t>(i) * 4) = c[0];
             }
@@ -135,16 +151,15 @@ __global__ void __launch_bounds__(1024) k_rmsnorm_quantize_long(NormArgs a) {
     const T *rp = a.residual != nullptr ? static_cast<const T *>(a.residual) + row * a.ldr : nullptr;
     const W *w = static_cast<const W *>(a.weight);
     auto h = [&](int64_t c) { return Elem<T>::load(x + c) + (rp != nullptr ? Elem<T>::load(rp + c) : 0.0f); };
-    float sum = 0.0f;
-    uint32_t mx = 0;
+    float sum = 0.0f, mx = 0.0f;
     for (int64_t c = threadIdx.x; c < a.cols; c += blockDim.x) {
         const float v = h(c);
         sum = fmaf(v, v, sum);
-        mx = max(mx, abs_bits_nan0(v * Elem<W>::load(w + c)));
+        mx = fmaxf(mx, fabsf(v * Elem<W>::load(w + c)));
     }
     block_sum_max(sum, mx);
     const float r = rsqrtf(sum / static_cast<float>(a.cols) + a.eps);
-    const float s = a.scale != nullptr ? __ldg(a.scale) : scale_from_amax(__uint_as_float(mx) * r);
+    const float s = a.scale != nullptr ? __ldg(a.scale) : scale_from_amax(mx * r);
     if (a.scale_out != nullptr && threadIdx.x == 0) a.scale_out[row] = s;
     for (int64_t c = threadIdx.x; c < a.cols; c += blockDim.x) {
         const float v = h(c);
