@@ -98,13 +98,37 @@ struct WriteArgs {
 
 constexpr float kMinScale = 7.888609052210118e-31f;  // 2^-100
 
-// quantize_block_fast() of 8 values with packed products and one test of the
-// four bytes of a word: the codes of v * r_lo and v * r_hi agree and none is
-// 0x80 or NaN, or the block takes the exact divide.
+// RN(v / s) of two values from r = RN(1 / s): Newton steps on the quotient with
+// exact fma remainders. By Markstein's theorem (1990) the second one rounds
+// correctly, the first having come within an ulp; s within 2^+-60 keeps the
+// remainders of every quotient that matters clear of underflow.
+__device__ __forceinline__ void divide2(float &q0, float &q1, float v0, float v1, float s, float r) {
+    float e0, e1;
+    mul2(q0, q1, v0, v1, r, r);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        fma2(e0, e1, q0, q1, -s, -s, v0, v1);
+        fma2(q0, q1, e0, e1, r, r, q0, q1);
+    }
+}
+
+// Bytes 0x7f, 0xff (NaN) and 0x80 of a word of codes, in bit 7 of each byte.
+__device__ __forceinline__ uint32_t special_bytes(uint32_t w) {
+    const uint32_t m = w & 0x7f7f7f7fu;
+    return ((m + 0x01010101u) | (~(m + 0x7f7f7f7fu) & w)) & 0x80808080u;
+}
+
+// QuantizeLinear of 8 values, bit-identical to quantize1(). As
+// quantize_block_fast(): where the codes of v * r_lo and v * r_hi agree they
+// are the code of RN(v / s). 16-bit inputs meet a rounding boundary often (448
+// = 7 * 64: for a bf16 maximum with an even significand one significand in 128
+// divides to the midpoint 21/16), so a block with a disagreement is divided
+// correctly in place, and only one with NaN or 0x80 codes, or an unusual
+// scale, takes the scalar divide and the integer encoder.
 __device__ __forceinline__ void quantize8(const float *v, float s, float r, bool s_ok, uint32_t *w) {
     const float r_lo = r * 0.99999952316284180f;  // 1 - 2^-21
     const float r_hi = r * 1.00000047683715820f;  // 1 + 2^-21
-    uint32_t odd = 0;
+    uint32_t other[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         float lo[4], hi[4];
@@ -114,12 +138,18 @@ __device__ __forceinline__ void quantize8(const float *v, float s, float r, bool
             fma2(hi[k], hi[k + 1], v[4 * j + k], v[4 * j + k + 1], r_hi, r_hi, 0.0f, 0.0f);
         }
         w[j] = cvt_e4m3x2(lo[0], lo[1]) | (cvt_e4m3x2(lo[2], lo[3]) << 16);
-        const uint32_t other = cvt_e4m3x2(hi[0], hi[1]) | (cvt_e4m3x2(hi[2], hi[3]) << 16);
-        // 0x7f + 1 and 0xff + 1 set bit 7 of the low seven bits' sum; a zero magnitude plus 0x7f does not
-        const uint32_t m = w[j] & 0x7f7f7f7fu;
-        odd |= (w[j] ^ other) | ((m + 0x01010101u) & 0x80808080u) | (~(m + 0x7f7f7f7fu) & w[j] & 0x80808080u);
+        other[j] = cvt_e4m3x2(hi[0], hi[1]) | (cvt_e4m3x2(hi[2], hi[3]) << 16);
     }
-    if (odd != 0 || !s_ok) {
+    if (((w[0] ^ other[0]) | (w[1] ^ other[1])) != 0) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            float q[4];
+            divide2(q[0], q[1], v[4 * j], v[4 * j + 1], s, r);
+            divide2(q[2], q[3], v[4 * j + 2], v[4 * j + 3], s, r);
+            w[j] = cvt_e4m3x2(q[0], q[1]) | (cvt_e4m3x2(q[2], q[3]) << 16);
+        }
+    }
+    if ((special_bytes(w[0]) | special_bytes(w[1])) != 0 || !s_ok) {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
             w[j] = quantize1(v[4 * j], s) | (quantize1(v[4 * j + 1], s) << 8) | (quantize1(v[4 * j + 2], s) << 16) | (quantize1(v[4 * j + 3], s) << 24);
@@ -216,7 +246,7 @@ __global__ void __launch_bounds__(THREADS) k_kv_cache_write(WriteArgs a) {
         s = fmaxf(s, had);
         const float div = s > 0.0f ? s : 1.0f;
         const float r = __frcp_rn(div);
-        const bool ok = scale_fast_ok(div, r);
+        const bool ok = div >= 8.673617379884035e-19f && div <= 1.152921504606847e18f;  // 2^+-60: divide2()
 #pragma unroll
         for (int j = 0; j < kVpt; ++j) {
             const int i = threadIdx.x + j * blockDim.x;
