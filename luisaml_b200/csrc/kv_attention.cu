@@ -42,7 +42,19 @@ constexpr int kMinRange = 32;      // steps a CTA takes at least
 constexpr int kWholeSteps = 64;    // up to here splitting a segment costs more than it gains
 constexpr int kPad = 24;           // what a segment's set-up and join cost, in steps
 constexpr int kMaxBatch = 1024;    // sequences per launch (the plan's table in shared memory)
-constexpr int kTcRows = 128;       // rows of a sequence from which the tensor-core kernel takes it
+
+// Which kernel: the streaming one takes 1.0 us of an SM for 16 rows and 128
+// keys (0.7 at head_dim 64), the tensor-core one 1.9 us for up to 256 rows, but
+// it splits no keys: with fewer units than SMs the rest of the machine idles.
+// Both are proportional to the keys, so the lengths, which the host does not
+// know, cancel out: the tensor-core kernel wins from `rows` rows a unit or SM,
+// whichever are more. 8 cache heads, streaming / tensor-core in us:
+//   head_dim 128, 64 sequences of 4096: 16 rows 135 / 249, 32 250 / 256, 64 484 / 256
+//     8 sequences of 32768: 32 rows 228 / 420, 64 433 / 420, 96 634 / 445
+//     1 sequence of 32768: 256 rows 204 / 497, 512 392 / 500
+//   head_dim 64, 64 of 4096: 32 rows 169 / 217, 64 318 / 219
+//     8 of 32768: 64 rows 274 / 380, 96 404 / 380
+constexpr int tc_rows(int head_dim) { return head_dim == 64 ? 40 : 28; }
 
 // RG: groups of 8 rows per tile. One CTA per SM with a deep ring, two at
 // head_dim 64 (two CTAs of 128-register threads at 128 leave the ring two
@@ -949,11 +961,21 @@ int lcml_kv_attention(const lcml_kv_attention_desc *d, lcml_stream_t stream) {
     const bool fits = kv_attention_tc_fits(d);
     LCML_CHECK_ARG(d->variant != 2 || fits, "lcml_kv_attention: variant 2 does not serve this call");
     const int64_t most = (d->max_tokens < d->batch->total_tokens ? d->max_tokens : d->batch->total_tokens) * a.group;
-    int min_rows = fits && d->variant != 1 ? (d->variant == 2 ? 0 : kTcRows) : 0x7fffffff;
-    if (most < min_rows) min_rows = 0x7fffffff;
+    int min_rows = 0x7fffffff;
+    if (d->variant == 2) {
+        min_rows = 0;
+    } else if (fits && d->variant == 0) {
+        const int rows = tc_rows(d->cache->head_dim);
+        const int64_t all = d->batch->total_tokens * a.group;
+        // units of the sequences with at least `rows` rows, at most
+        const int64_t units = (all / kTcBlockRows + (d->batch->batch < all / rows ? d->batch->batch : all / rows)) * d->cache->kv_heads;
+        if (most >= rows && all * d->cache->kv_heads >= rows * (units > sm_count() ? units : sm_count())) min_rows = rows;
+    }
     if (min_rows != 0x7fffffff) {
         const int rc2 = kv_attention_tc(d, a, min_rows, st);
-        if (rc2 != LCML_OK || min_rows == 0 || d->batch->batch == 1) return rc2;
+        // the shortest sequence has at least what the others, at max_tokens each, leave
+        const int64_t least = (d->batch->total_tokens - (d->batch->batch - 1) * static_cast<int64_t>(d->max_tokens)) * a.group;
+        if (rc2 != LCML_OK || min_rows == 0 || least >= min_rows) return rc2;
     }
     const int max_rows = min_rows == 0x7fffffff ? min_rows : min_rows - 1;
     const Plan p = make_plan(d, max_rows);

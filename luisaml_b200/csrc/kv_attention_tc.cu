@@ -35,7 +35,8 @@ namespace lcml {
 namespace {
 
 constexpr int kTile = 128;                // rows per tile, keys per tile
-constexpr int kBlockRows = 2 * kTile;     // rows per CTA
+constexpr int kBlockRows = kTcBlockRows;  // rows per CTA: two tiles
+static_assert(kBlockRows == 2 * kTile, "two tiles");
 constexpr int kThreads = 512;
 constexpr int kGroups = kTile / 16;       // 16-token groups of a key tile: one pair of scales each
 constexpr int kInfoStages = 4;

@@ -106,6 +106,8 @@ __device__ __forceinline__ void split_q(uint32_t w0, uint32_t w1, const QScale<N
     }
 }
 
+constexpr int kTcBlockRows = 256;  // rows per CTA of the tensor-core kernel
+
 // The tensor-core path for long runs of queries (kv_attention_tc.cu).
 bool kv_attention_tc_fits(const lcml_kv_attention_desc *d);
 int kv_attention_tc(const lcml_kv_attention_desc *d, const AttnArgs &a, int min_rows, cudaStream_t st);
