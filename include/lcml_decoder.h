@@ -56,7 +56,10 @@ int lcml_rmsnorm_quantize(const lcml_rmsnorm_desc *desc, lcml_stream_t stream);
  * so a value is decode(code) * the scale of its block of scale_block tokens.
  * head_dim: 64, 128 or 256; scale_block: a multiple of 16 that divides
  * page_size, with scale_block * head_dim <= 32768. k and v are 16-byte
- * aligned.
+ * aligned; scales are finite and not negative, as lcml_kv_cache_write leaves
+ * them. kv_heads <= 4096, page_size <= 65536 and num_pages * kv_heads *
+ * page_size < 2^31 (a row of head_dim codes has a 32-bit index, an address 64
+ * bits).
  */
 typedef struct lcml_kv_cache {
     uint8_t *k, *v;
@@ -69,10 +72,11 @@ typedef struct lcml_kv_cache {
  * A ragged batch: sequence b owns tokens cu_tokens[b] .. cu_tokens[b + 1] - 1
  * of the packed token dimension (cu_tokens[0] = 0, cu_tokens[batch] <=
  * total_tokens), and position t of sequence b lives in slot t % page_size of
- * page block_table[b * table_stride + t / page_size]. An entry outside
- * [0, num_pages), or a position past the table's columns, is never
- * dereferenced: a write or read skips it, attention takes zeros, and the
- * device error word gets code 6 (lcml_device_error).
+ * page block_table[b * table_stride + t / page_size]; cu_tokens does not
+ * decrease. A table entry outside [0, num_pages), or a position past the
+ * table's columns, is never followed: a write or read skips it, attention
+ * leaves its tokens out (what it returns for that sequence means nothing), and
+ * the device error word (lcml_device_error) gets code 6.
  */
 typedef struct lcml_kv_batch {
     int32_t batch;
@@ -125,9 +129,10 @@ int lcml_kv_cache_read(const lcml_kv_cache *cache, const lcml_kv_batch *batch, v
  * weights enter the matrix products as 16-bit floats or, on the tensor-core
  * path, q as a sum of e4m3 parts that reproduce it. What the masked slots
  * hold (NaN codes included) does not matter.
- * max_tokens: an upper bound of the n (host side; picks the kernels). A
- * sequence with more queries, or longer than its block table reaches, is not
- * computed in full and sets the device error word to 7.
+ * max_tokens: an upper bound of the n (host side). It and the extents pick the
+ * kernels: the closer it is, the fewer launches (exact for a batch of equal
+ * lengths). A sequence with more queries, or longer than its block table
+ * reaches, is not computed in full and sets the device error word to 7.
  * workspace: lcml_kv_attention_workspace_size(desc) bytes, 16-byte aligned,
  * contents on entry do not matter (NULL when the size is 0).
  */

@@ -46,14 +46,7 @@ __device__ __forceinline__ float cap_score(float dot, float inv_cap, float cap) 
 // are zero) counts as 1.
 __device__ __forceinline__ float value_scale(float s) { return s >= 7.888609052210118e-31f ? s : 1.0f; }
 
-// Two e4m3 codes -> two halves (exact), low byte first.
-__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t b) {
-    uint32_t h;
-    asm("{\n\t.reg .b16 t;\n\tcvt.u16.u32 t, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(h) : "r"(b));
-    return h;
-}
-
-// The four codes of a word -> two pairs of halves.
+// The four codes of a word -> two pairs of halves (exact), low byte first.
 __device__ __forceinline__ void e4m3x4_to_half2(uint32_t w, uint32_t &lo, uint32_t &hi) {
     asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
         : "=r"(lo), "=r"(hi)

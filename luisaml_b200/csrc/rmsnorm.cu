@@ -221,7 +221,8 @@ extern "C" int lcml_rmsnorm_quantize(const lcml_rmsnorm_desc *d, lcml_stream_t s
     LCML_CHECK_ARG(d->weight_dtype == d->x_dtype || d->weight_dtype == LCML_DTYPE_FLOAT,
                    "lcml_rmsnorm_quantize: weight_dtype %d is neither x's type nor FLOAT", d->weight_dtype);
     LCML_CHECK_ARG(d->eps >= 0.0f, "lcml_rmsnorm_quantize: eps is negative or NaN");
-    if (d->rows == 0 || d->cols == 0) return LCML_OK;
+    if (d->rows == 0) return LCML_OK;
+    LCML_CHECK_ARG(d->cols > 0, "lcml_rmsnorm_quantize: rows without columns have no norm");
     LCML_CHECK_ARG((d->scale != nullptr) != (d->scale_out != nullptr),
                    "lcml_rmsnorm_quantize: give exactly one of scale and scale_out");
     LCML_CHECK_ARG(d->x && d->weight && d->q, "lcml_rmsnorm_quantize: null pointer");
