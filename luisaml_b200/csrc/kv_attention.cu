@@ -31,16 +31,20 @@
 // last). Where no sequence can be longer than kWholeSteps, a CTA takes whole
 // segments and there is nothing to join.
 //
-// Bound: HBM, 2 head_dim bytes per key and cache head.
+// Bound: HBM, 2 head_dim bytes per key and cache head (one token of a
+// 131072-token sequence, 8 cache heads of 128: 65 us, 4.2 of a copy's 6.5 TB/s:
+// 5.3 TB/s while it streams, the rest is the plan, the first copies and the
+// join; of 64 sequences of up to 4096: 77 us).
 #include "lcml_attention.cuh"
 
 namespace lcml {
 namespace {
 
 constexpr int kStep = 16;          // keys per warp step
-constexpr int kMinRange = 32;      // steps a CTA takes at least
-constexpr int kWholeSteps = 64;    // up to here splitting a segment costs more than it gains
-constexpr int kPad = 24;           // what a segment's set-up and join cost, in steps
+// Up to here splitting a segment costs more than it gains: 32 steps in one CTA
+// or split, one token of 64 sequences of 500: 25.9 and 27.2 us (head_dim 64:
+// 14.7 and 19.2), of 1 sequence 12.1 and 11.0.
+constexpr int kWholeSteps = 64;
 constexpr int kMaxBatch = 1024;    // sequences per launch (the plan's table in shared memory)
 
 // Which kernel: the streaming one takes 1.0 us of an SM for 16 rows and 128
@@ -56,15 +60,28 @@ constexpr int kMaxBatch = 1024;    // sequences per launch (the plan's table in 
 //     8 of 32768: 64 rows 274 / 380, 96 404 / 380
 constexpr int tc_rows(int head_dim) { return head_dim == 64 ? 40 : 28; }
 
-// RG: groups of 8 rows per tile. One CTA per SM with a deep ring, two at
-// head_dim 64 (two CTAs of 128-register threads at 128 leave the ring two
-// stages: 66 -> 70 us for 131072 tokens of 8 cache heads).
+// Warps per CTA and CTAs per SM: 8 warps an SM with deep rings of copies (16 at
+// head_dim 64). Two CTAs of four, so that one's set-up and join run under the
+// other's copies: one token of 200 sequences of 500, 8 cache heads, 85 us with
+// one CTA of eight, 64 here; of 64 x 500 34 and 26, of 64 x 4096 118 and 119, of
+// 8 x 300 10.9 and 12.7. Four CTAs of two: 59, 23, 121 and 14.7, but 14.8 for
+// one sequence of 500 (11.4 and 12.1). 16-row tiles at head_dim 64 keep two CTAs
+// of eight: their shares of O leave no room for four of four (4 tokens of 64
+// sequences of 1000: 41 and 57 us).
+constexpr int stream_warps(int head_dim, int groups) { return head_dim == 64 && groups == 2 ? 8 : 4; }
+constexpr int stream_ctas(int head_dim, int groups) { return head_dim == 64 && groups == 1 ? 4 : 2; }
+
 template <int D, int RG>
 struct Shape {
-    static constexpr int kWarps = 8;
+    static constexpr int kWarps = stream_warps(D, RG);
     static constexpr int kThreads = kWarps * 32;
     static constexpr int kRows = 8 * RG;                           // rows per tile
-    static constexpr int kCtasPerSm = D == 64 ? 2 : 1;
+    static constexpr int kCtasPerSm = stream_ctas(D, RG);
+    // Steps a CTA takes at least (one token of one sequence of 1000: 10.6 us,
+    // 11.4 with twice as many, 13.7 with four times), and what a segment's set-up
+    // and join cost in steps (of one sequence of 2000 11.7 us, 13.9 with none;
+    // of 200 sequences of 500 64.9, 63.5 with none, 67.3 with half as much again).
+    static constexpr int kMinRange = 2 * kWarps, kPad = 2 * kWarps;
     static constexpr int kStages = D == 256 ? 2 : 4;
     static constexpr int kStageBytes = 2 * kStep * D;              // per warp
     static constexpr int kRing = kWarps * kStages * kStageBytes;
@@ -101,9 +118,9 @@ struct Span {
 };
 
 // Sequence s; steps counts from lo over all the keys any of its queries sees,
-// and kPad empty ones: CTAs with many short segments would be late otherwise
+// and PAD empty ones: CTAs with many short segments would be late otherwise
 // (and a row without keys still gets its zeros).
-template <int ROWS>
+template <int ROWS, int PAD>
 __device__ __forceinline__ Span span_of(const AttnArgs &a, int s) {
     Span r;
     r.t0 = __ldg(a.b.cu_tokens + s);
@@ -115,7 +132,7 @@ __device__ __forceinline__ Span span_of(const AttnArgs &a, int s) {
     r.pos0 = r.len - n;
     const int64_t first = static_cast<int64_t>(r.pos0) - a.window + 1;  // the first query's oldest key
     r.lo = a.window > 0 && first > 0 ? static_cast<int>(first) & ~(kStep - 1) : 0;
-    r.steps = (r.len - r.lo + kStep - 1) / kStep + kPad;
+    r.steps = (r.len - r.lo + kStep - 1) / kStep + PAD;
     r.tiles = static_cast<int>((static_cast<int64_t>(r.n) * a.group + ROWS - 1) / ROWS);
     return r;
 }
@@ -229,7 +246,7 @@ __global__ void __launch_bounds__(Shape<D, RG>::kThreads, Shape<D, RG>::kCtasPer
             const int s = s0 + threadIdx.x;
             int64_t mine = 0;
             if (s < batch) {
-                const Span p = span_of<kRows>(a, s);
+                const Span p = span_of<kRows, S::kPad>(a, s);
                 if (p.cut && blockIdx.x == 0) record_device_error(a.err, kDevBadBatch);
                 if (static_cast<int64_t>(p.n) * a.group <= max_rows) mine = static_cast<int64_t>(p.tiles) * heads * p.steps;
                 plan_steps[s] = p.steps;
@@ -267,7 +284,7 @@ __global__ void __launch_bounds__(Shape<D, RG>::kThreads, Shape<D, RG>::kCtasPer
         return lo;
     };
     int64_t range = (total + gridDim.x - 1) / gridDim.x;
-    if (range < kMinRange && !whole) range = kMinRange;
+    if (range < S::kMinRange && !whole) range = S::kMinRange;
     int64_t from = range * blockIdx.x, to = min(from + range, total);
     if (whole && from < total) {  // segments that begin in the stretch, entirely
         auto up = [&](int64_t p) {  // the first segment boundary at or after p
@@ -305,7 +322,7 @@ __global__ void __launch_bounds__(Shape<D, RG>::kThreads, Shape<D, RG>::kCtasPer
             const int th = in <= 0x7fffffff ? static_cast<int>(in) / steps : static_cast<int>(in / steps);  // 64-bit division is slow
             const int st = static_cast<int>(in - static_cast<int64_t>(th) * steps);
             const int tile = th / heads, head = th - tile * heads;
-            const Span sp = span_of<kRows>(a, s);
+            const Span sp = span_of<kRows, S::kPad>(a, s);
             const int key = sp.lo + st * kStep;
             const int row_a = tile * kRows / a.group, row_z = (min(tile * kRows + kRows, sp.n * a.group) - 1) / a.group;
             const int hi = a.causal ? min(sp.pos0 + row_z, sp.len - 1) : sp.len - 1, lo = a.window > 0 ? sp.pos0 + row_a - a.window + 1 : 0;
@@ -378,7 +395,7 @@ __global__ void __launch_bounds__(Shape<D, RG>::kThreads, Shape<D, RG>::kCtasPer
             ++seq;
             th = 0;
         }
-        const Span sp = span_of<kRows>(a, seq);
+        const Span sp = span_of<kRows, S::kPad>(a, seq);
         const int tile = th / heads, head = th - tile * heads;
         const int seg = static_cast<int>(plan_first[seq] + static_cast<int64_t>(th) * sp.steps - from);  // the segment's first step
         const int end = min(seg + sp.steps, span);
@@ -869,7 +886,7 @@ Plan make_plan(const lcml_kv_attention_desc *d, int max_rows) {
     if (most < 1) most = 1;
     Plan p{};
     p.groups = most <= 8 || c->head_dim == 256 ? 1 : 2;
-    p.grid = sm_count() * (c->head_dim == 64 ? 2 : 1);
+    p.grid = sm_count() * stream_ctas(c->head_dim, p.groups);
     const int64_t reach = static_cast<int64_t>(d->batch->table_cols) * c->page_size;  // no sequence is longer
     p.whole = (reach + kStep - 1) / kStep <= kWholeSteps;
     if (p.whole) return p;
