@@ -8,7 +8,7 @@
 // together: one block reduction per row, not two.
 //
 // Bound: HBM (x + residual + h + 1 byte per element) for many rows (8191 x 5000
-// fp32: 39 us, 5.2 of a copy's 6.5 TB/s), the latency of one load, one block
+// fp32: 40 us, 5.1 of a copy's 6.5 TB/s), the latency of one load, one block
 // reduction and one store for few (1 x 4096: 2.1 us in a graph).
 #include "lcml_decoder.cuh"
 
@@ -44,6 +44,17 @@ __device__ __forceinline__ void block_sum_max(float &sum, float &mx) {
     mx = warp_max(l < nw ? red_m[l] : 0.0f);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+}
+
+// r / s for r ~ 1 / sqrt(ms), rounded about once: one Newton step for r, whose
+// correction c stays apart, then one for the quotient. All elements of a row share
+// this factor's error: of 8191 x 5000 fp32 values 48 had another code than in 64
+// bits without the steps, 33 have with them, 31 with the factor from 64 bits.
+__device__ __forceinline__ float norm_factor(float r, float ms, float s) {
+    const float u = r * ms, ue = fmaf(r, ms, -u);
+    const float c = 0.5f * r * (fmaf(-u, r, 1.0f) - ue * r);
+    const float inv = __frcp_rn(s), f = r * inv;
+    return fmaf(inv, fmaf(-f, s, r) + c, f);
 }
 
 // E elements per access (E = 1: rows of any alignment), VPT accesses per
@@ -106,7 +117,7 @@ __global__ void __launch_bounds__(1024) k_rmsnorm_quantize(NormArgs a) {
     // of the fused GEMM epilogues (quantize_block_rcp). It differs from a
     // division only where y / s lies within a few fp32 ulps of an e4m3
     // boundary, as y itself is uncertain by the order of its sum.
-    const float f = r * __frcp_rn(s);
+    const float f = norm_factor(r, sum / static_cast<float>(a.cols) + a.eps, s);
     const bool ok = scale_fast_ok(s, f);
     uint8_t *q = a.q + row * a.cols;
 #pragma unroll
