@@ -568,3 +568,19 @@ def test_bad_pages_are_not_followed(dev):
     assert _no_device_error() == 7
     lb.kv_cache_write(*cache.args(), k, k, cache.table, cu, long)
     assert _no_device_error() == 6
+
+
+@pytest.mark.parametrize("dim,dtype", [(128, "bf16"), (64, "f16")])
+def test_the_choice_of_kernel(dev, dim, dtype):
+    """many sequences that the automatic choice gives to the tensor-core kernel: all of them (no streaming launch), all
+    but the short ones (both launches, sequences of no query among them), and one row less than either side of the threshold"""
+    rows = {128: 28, 64: 40}[dim]
+    held = [200 + 3 * i for i in range(40)]
+    for new in ([30] * 40, [30] * 39 + [29], [30, 1, 30, 0] * 10, [rows // 4, rows // 4 - 1, 30, 30] * 10):
+        _attend(dev, new, held, 2, 4, dim, 32, 16, dtype)
+
+
+def test_many_sequences_of_one_token(dev):
+    """more segments than CTAs, whole and cut, and more sequences than one launch plans"""
+    _attend(dev, [1] * 300, [(7 * i) % 100 for i in range(300)], 2, 4, 128, 16, 16, "bf16")
+    _attend(dev, [1] * 1100, [(13 * i) % 40 for i in range(1099)] + [1500], 1, 2, 64, 16, 16, "f16")
