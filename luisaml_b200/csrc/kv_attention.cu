@@ -81,7 +81,9 @@ struct Shape {
     // 11.4 with twice as many, 13.7 with four times), and what a segment's set-up
     // and join cost in steps (of one sequence of 2000 11.7 us, 13.9 with none;
     // of 200 sequences of 500 64.9, 63.5 with none, 67.3 with half as much again).
-    static constexpr int kMinRange = 2 * kWarps, kPad = 2 * kWarps;
+    // 16-row tiles join twice as much: 4 tokens of 16 sequences of up to 2000, head_dim
+    // 64, 28.0 us, 29.7 with 2 kWarps (64 x 1000 at 128: 52.7 and 51.7).
+    static constexpr int kMinRange = 2 * kWarps, kPad = (RG == 1 ? 2 : 3) * kWarps;
     static constexpr int kStages = D == 256 ? 2 : 4;
     static constexpr int kStageBytes = 2 * kStep * D;              // per warp
     static constexpr int kRing = kWarps * kStages * kStageBytes;

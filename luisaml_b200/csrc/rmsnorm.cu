@@ -8,7 +8,7 @@
 // together: one block reduction per row, not two.
 //
 // Bound: HBM (x + residual + h + 1 byte per element) for many rows (8191 x 5000
-// fp32: 40 us, 5.1 of a copy's 6.5 TB/s), the latency of one load, one block
+// fp32: 41 us, 5.0 of a copy's 6.5 TB/s), the latency of one load, one block
 // reduction and one store for few (1 x 4096: 2.1 us in a graph).
 #include "lcml_decoder.cuh"
 
