@@ -11,7 +11,7 @@
 //
 // Bound: the read by HBM (32 x 2000 tokens, 8 heads of 128, to bf16: 61 us, 4.8
 // of a copy's 6.5 TB/s; three quarters of its bytes are writes); the write of
-// prompts by the instructions of the exact rounding, about 30 an element (5
+// prompts by the instructions of the exact rounding, 23 an element (5
 // prompts of 4000 tokens, f16: 38 us, 2.8 TB/s); decode steps by the chain of
 // dependent look-ups (cu -> length -> page -> codes and scales) of a few L2
 // latencies (one token of 64 sequences: 9 us).
