@@ -131,8 +131,9 @@ int lcml_kv_cache_read(const lcml_kv_cache *cache, const lcml_kv_batch *batch, v
  * hold (NaN codes included) does not matter.
  * max_tokens: an upper bound of the n (host side). It and the extents pick the
  * kernels: the closer it is, the fewer launches (exact for a batch of equal
- * lengths). A sequence with more queries, or longer than its block table
- * reaches, is not computed in full and sets the device error word to 7.
+ * lengths). Where total_tokens is padded, the padded total picks, and every
+ * query is computed. A sequence with more queries, or longer than its block
+ * table reaches, is not computed in full and sets the device error word to 7.
  * workspace: lcml_kv_attention_workspace_size(desc) bytes, 16-byte aligned,
  * contents on entry do not matter (NULL when the size is 0).
  */

@@ -982,7 +982,7 @@ int lcml_kv_attention(const lcml_kv_attention_desc *d, lcml_stream_t stream) {
     const int64_t most = (d->max_tokens < d->batch->total_tokens ? d->max_tokens : d->batch->total_tokens) * a.group;
     int min_rows = 0x7fffffff;
     if (d->variant == 2) {
-        min_rows = 0;
+        min_rows = 1;
     } else if (fits && d->variant == 0) {
         const int rows = tc_rows(d->cache->head_dim);
         const int64_t all = d->batch->total_tokens * a.group;
@@ -991,10 +991,14 @@ int lcml_kv_attention(const lcml_kv_attention_desc *d, lcml_stream_t stream) {
         if (most >= rows && all * d->cache->kv_heads >= rows * (units > sm_count() ? units : sm_count())) min_rows = rows;
     }
     if (min_rows != 0x7fffffff) {
-        const int rc2 = kv_attention_tc(d, a, min_rows, st);
-        // the shortest sequence has at least what the others, at max_tokens each, leave
+        // If cu_tokens[batch] is total_tokens, the shortest sequence has at
+        // least what the others, at max_tokens each, leave. A padded batch may
+        // hold shorter ones all the same, so the kernel that runs alone takes
+        // every sequence, however few its rows.
         const int64_t least = (d->batch->total_tokens - (d->batch->batch - 1) * static_cast<int64_t>(d->max_tokens)) * a.group;
-        if (rc2 != LCML_OK || min_rows == 0 || least >= min_rows) return rc2;
+        const bool alone = d->variant == 2 || least >= min_rows;
+        const int rc2 = kv_attention_tc(d, a, alone ? 0 : min_rows, st);
+        if (rc2 != LCML_OK || alone) return rc2;
     }
     const int max_rows = min_rows == 0x7fffffff ? min_rows : min_rows - 1;
     const Plan p = make_plan(d, max_rows);

@@ -48,3 +48,59 @@ def test_a_score_far_above_the_earlier_ones(dev, nats, dim, dtype, variant):
         scale = nats / dim
         out = lb.kv_attention(q, *cache.args(), cache.table, _cu([n], dev), cache.lens, max_tokens=n, scale=scale, lse=lse, variant=variant)
         _check_attention(cache, q, [n], [length], out, lse, scale=scale)
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, "f16"), (128, "bf16")])
+@pytest.mark.parametrize("new,total,most", [([3], 512, 512), ([5, 0, 2], 700, 300), ([100, 3], 200, 100), ([0, 0], 400, 200), ([30] * 40, 1500, 30),
+                                            ([260, 40], 600, 300), ([1] * 30, 240, 8), ([1] * 64, 2000, 1)])
+def test_padded_queries(dev, new, total, most, dim, dtype):
+    """a packed dimension longer than cu_tokens[batch]: every query is computed, the padding is left alone"""
+    import luisaml_b200 as lb
+    heads, group = 8, 4
+    lens = [n + 150 + 31 * (i % 5) for i, n in enumerate(new)]
+    cache = Cache(dev, lens, max(lens) + 5, heads, dim, 32, 16)
+    q = torch.randn(total, heads * group, dim, device=dev).to(TYPES[dtype])
+    out, lse = torch.full_like(q, 7.0), torch.full((total, heads * group), 7.0, device=dev)
+    lb.kv_attention(q, *cache.args(), cache.table, _cu(new, dev), cache.lens, max_tokens=most, out=out, lse=lse)
+    _check_attention(cache, q, new, lens, out, lse)
+    assert (out[sum(new):] == 7).all() and (lse[sum(new):] == 7).all()
+
+
+def test_a_captured_batch_replayed_with_fewer_tokens(dev):
+    import luisaml_b200 as lb
+    heads, group, dim = 2, 4, 128
+    new = [100] * 40
+    cache = Cache(dev, [300] * 40, 300, heads, dim, 32, 16)
+    q = torch.randn(sum(new), heads * group, dim, device=dev).bfloat16()
+    out, lse = torch.empty_like(q), torch.empty(sum(new), heads * group, device=dev)
+    cu = _cu(new, dev)
+    call = lambda: lb.kv_attention(q, *cache.args(), cache.table, cu, cache.lens, max_tokens=100, out=out, lse=lse, workspace=ws)  # noqa: E731
+    ws = torch.empty(lb.kv_attention_workspace_size(q, *cache.args(), cache.table, cu, cache.lens, max_tokens=100), dtype=torch.uint8, device=dev)
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+        with torch.cuda.graph(graph, stream=side):
+            call()
+    torch.cuda.current_stream().wait_stream(side)
+    for new, lens in (([100] * 40, [300] * 40), ([1] * 40, [300] * 40), ([(7 * i) % 30 for i in range(40)], [200 + i for i in range(40)])):
+        cu.copy_(_cu(new, dev))
+        cache.lens.copy_(torch.tensor(lens, dtype=torch.int32))
+        out.fill_(7.0)
+        lse.fill_(7.0)
+        graph.replay()
+        _check_attention(cache, q, new, lens, out, lse)
+        assert (out[sum(new):] == 7).all()
+
+
+def test_padded_writes_and_reads(dev):
+    import luisaml_b200 as lb
+    start, new, total = [3, 0, 40], [20, 5, 1], 100
+    cache = Cache(dev, start, 80, 2, 64, 32, 16)
+    k, v = (torch.randn(total, 2, 64, device=dev).bfloat16() for _ in range(2))
+    cu = _cu(new, dev)
+    _check_write(cache, start, new, k, v, lambda lb: lb.kv_cache_write(*cache.args(), k, v, cache.table, cu, cache.lens))
+    got = lb.kv_cache_read(*cache.args(), cache.table, cu, cache.lens, total=total, dtype=torch.float32)
+    for a, which in zip(got, "kv"):
+        want = torch.cat([cache.tokens(which, b, s + n)[:, s:].transpose(0, 1) for b, (s, n) in enumerate(zip(start, new))])
+        assert torch.equal(a[:sum(new)], want.float())
