@@ -36,18 +36,24 @@ struct Elem<__nv_bfloat16> {
 };
 
 // E consecutive elements of T as one aligned access of E * sizeof(T) bytes
-// (two for 32 bytes), widened to or rounded from fp32.
-template <typename T, int E>
+// (two for 32 bytes), widened to or rounded from fp32. kReadOnly: nothing writes
+// the memory while the kernel runs.
+template <typename T, int E, bool kReadOnly = true>
 __device__ __forceinline__ void load_vec(const T *p, float *v) {
     constexpr int B = E * static_cast<int>(sizeof(T));
     alignas(16) T t[E];
+    auto get = [&](auto *dst, int i) {
+        const auto *src = reinterpret_cast<decltype(dst)>(const_cast<T *>(p)) + i;
+        if constexpr (kReadOnly) dst[i] = __ldg(src);
+        else dst[i] = *src;
+    };
     if constexpr (B == 32) {
-        reinterpret_cast<uint4 *>(t)[0] = __ldg(reinterpret_cast<const uint4 *>(p));
-        reinterpret_cast<uint4 *>(t)[1] = __ldg(reinterpret_cast<const uint4 *>(p) + 1);
+        get(reinterpret_cast<uint4 *>(t), 0);
+        get(reinterpret_cast<uint4 *>(t), 1);
     } else if constexpr (B == 16) {
-        *reinterpret_cast<uint4 *>(t) = __ldg(reinterpret_cast<const uint4 *>(p));
+        get(reinterpret_cast<uint4 *>(t), 0);
     } else if constexpr (B == 8) {
-        *reinterpret_cast<uint2 *>(t) = __ldg(reinterpret_cast<const uint2 *>(p));
+        get(reinterpret_cast<uint2 *>(t), 0);
     } else {
 #pragma unroll
         for (int i = 0; i < E; ++i) t[i] = p[i];

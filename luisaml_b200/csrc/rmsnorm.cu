@@ -65,17 +65,19 @@ __global__ void __launch_bounds__(1024) k_rmsnorm_quantize(NormArgs a) {
     const int64_t row = blockIdx.x;
     const int nv = static_cast<int>(a.cols / E);
     // A thread past the row's end reads the last access again and drops it:
-    // loads and arithmetic without branches.
+    // loads and arithmetic without branches. What it reads may be h already,
+    // where h_out is x or residual, so it counts neither in the sum nor in the
+    // maximum; the owner's own load comes before its store.
     float v[VPT * E];
     griddep_wait();
     const T *x = static_cast<const T *>(a.x) + row * a.ldx;
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) load_vec<T, E>(x + static_cast<int64_t>(min(static_cast<int>(threadIdx.x + j * blockDim.x), nv - 1)) * E, v + j * E);
+    for (int j = 0; j < VPT; ++j) load_vec<T, E, false>(x + static_cast<int64_t>(min(static_cast<int>(threadIdx.x + j * blockDim.x), nv - 1)) * E, v + j * E);
     if (a.residual != nullptr) {
         const T *r = static_cast<const T *>(a.residual) + row * a.ldr;
         float t[VPT * E];
 #pragma unroll
-        for (int j = 0; j < VPT; ++j) load_vec<T, E>(r + static_cast<int64_t>(min(static_cast<int>(threadIdx.x + j * blockDim.x), nv - 1)) * E, t + j * E);
+        for (int j = 0; j < VPT; ++j) load_vec<T, E, false>(r + static_cast<int64_t>(min(static_cast<int>(threadIdx.x + j * blockDim.x), nv - 1)) * E, t + j * E);
 #pragma unroll
         for (int k = 0; k < VPT * E; ++k) v[k] += t[k];
     }
@@ -93,21 +95,22 @@ __global__ void __launch_bounds__(1024) k_rmsnorm_quantize(NormArgs a) {
         const int i = threadIdx.x + j * blockDim.x;
         float w[E];
         load_vec<W, E>(static_cast<const W *>(a.weight) + static_cast<int64_t>(min(i, nv - 1)) * E, w);
-        float s0 = 0.0f, s1 = 0.0f;
+        float s0 = 0.0f, s1 = 0.0f, top = 0.0f;
         if constexpr (E == 1) {
             s0 = v[j] * v[j];
             v[j] *= w[0];
-            mx = fmaxf(mx, fabsf(v[j]));  // (an element twice does not change the maximum)
+            top = fabsf(v[j]);
         } else {
 #pragma unroll
             for (int e = 0; e < E; e += 2) {
                 float &v0 = v[j * E + e], &v1 = v[j * E + e + 1];
                 fma2(s0, s1, v0, v1, v0, v1, s0, s1);
                 mul2(v0, v1, v0, v1, w[e], w[e + 1]);
-                mx = fmaxf(fmaxf(mx, fabsf(v0)), fabsf(v1));
+                top = fmaxf(fmaxf(top, fabsf(v0)), fabsf(v1));
             }
         }
         sum += i < nv ? s0 + s1 : 0.0f;
+        mx = fmaxf(mx, i < nv ? top : 0.0f);
     }
     block_sum_max(sum, mx);
     const float r = rsqrtf(sum / static_cast<float>(a.cols) + a.eps);

@@ -104,3 +104,24 @@ def test_padded_writes_and_reads(dev):
     for a, which in zip(got, "kv"):
         want = torch.cat([cache.tokens(which, b, s + n)[:, s:].transpose(0, 1) for b, (s, n) in enumerate(zip(start, new))])
         assert torch.equal(a[:sum(new)], want.float())
+
+
+@pytest.mark.parametrize("dtype,cols", [("bf16", 5376), ("bf16", 4104), ("bf16", 2304), ("f16", 3848), ("f32", 2304), ("f32", 5376), ("bf16", 433), ("f32", 33000)])
+@pytest.mark.parametrize("rows", [3, 400])
+def test_norm_in_place(dev, rows, cols, dtype):
+    """h_out = x and h_out = residual, at widths whose last vectors do not fill the threads: bit for bit as with an output of its own"""
+    import luisaml_b200 as lb
+    g = torch.Generator(device=dev).manual_seed(cols)
+    x = torch.randn(rows, cols, generator=g, device=dev)
+    r = torch.randn(rows, cols, generator=g, device=dev)
+    # the row's maximum lies in what the surplus threads would read, and would grow with another addition
+    x[:, -32:], r[:, -32:] = 4.0, 4.0
+    x, r = x.to(TYPES[dtype]), r.to(TYPES[dtype])
+    w = torch.ones(cols, device=dev)
+    want = lb.rmsnorm_quantize(x, w, r)
+    _check_norm(x, w, r, 1e-6, *want)
+    for turn in range(30):
+        for alias in ("x", "residual"):
+            a, b = x.clone(), r.clone()
+            got = lb.rmsnorm_quantize(a, w, b, h_out=a if alias == "x" else b)
+            assert all(torch.equal(p, q) for p, q in zip(got, want)), (turn, alias)
