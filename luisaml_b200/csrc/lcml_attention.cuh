@@ -42,9 +42,13 @@ __device__ __forceinline__ float cap_score(float dot, float inv_cap, float cap) 
 
 // The scale of a block of values takes part in the softmax's exponent: with
 // a_j = x_j + log2(s_j) the weights 2^(a_j - m) multiply codes, and the sum
-// takes 2^(a_j - m) / s_j. A scale below 2^-100 (an all-zero block, whose codes
-// are zero) counts as 1.
-__device__ __forceinline__ float value_scale(float s) { return s >= 7.888609052210118e-31f ? s : 1.0f; }
+// takes 2^(a_j - m) / s_j. A block of scale 0 adds nothing to the output but its
+// share of the sum, so any scale small enough does: 2^-80 keeps its keys out of
+// the reference maximum m (as 1 they would push the other weights by their
+// scales, e.g. 2^-16 for values of 0.01, into subnormal halves), and its weights
+// only flush to 0 (2^-126) where they are 2^-46 of the largest over the largest
+// scale. Scales below 2^-100 do not occur in a written cache and count as 0.
+__device__ __forceinline__ float value_scale(float s) { return s >= 7.888609052210118e-31f ? s : 8.271806125530277e-25f; }
 
 // The four codes of a word -> two pairs of halves (exact), low byte first.
 __device__ __forceinline__ void e4m3x4_to_half2(uint32_t w, uint32_t &lo, uint32_t &hi) {

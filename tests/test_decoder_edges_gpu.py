@@ -125,3 +125,81 @@ def test_norm_in_place(dev, rows, cols, dtype):
             a, b = x.clone(), r.clone()
             got = lb.rmsnorm_quantize(a, w, b, h_out=a if alias == "x" else b)
             assert all(torch.equal(p, q) for p, q in zip(got, want)), (turn, alias)
+
+
+def _check_rows(cache, q, new, lens, out, dtype, share=0.05):
+    """Attention against 64 bits with a bound taken row by row from the weights p and value scales s: a weight enters the
+    product as a half of p_j s_j over a reference that is at most the row's largest, so beside the relative terms (fp32
+    scores, 2^-11, the sum, the output's type) it is off by 2^-25 of max_j(p_j s_j), for every code it multiplies.
+    `share`: the bound may not be more of the row's largest output, so a wrong value shows."""
+    group, at = q.shape[1] // cache.heads, 0
+    half = 2.0 ** -8 if dtype == "bf16" else 2.0 ** -11
+    for b, (n, length) in enumerate(zip(new, lens)):
+        k, v = cache.tokens("k", b, length), cache.tokens("v", b, length)
+        s = cache.vs[cache.table[b].long()].double().transpose(0, 1).reshape(cache.heads, -1).repeat_interleave(cache.block, 1)[:, :length]
+        codes = cache.v[cache.table[b].long()].view(torch.float8_e4m3fn).double().transpose(0, 1).reshape(cache.heads, -1, cache.dim)[:, :length].abs()
+        pos = torch.arange(length - n, length, device=q.device)
+        for h in range(q.shape[1]):
+            qq, c = q[at:at + n, h].double(), h // group
+            ref, lse, weighted, reach = _attention64(qq, k[c], v[c], pos, length, cache.dim ** -0.5, True, 0, 0.0)
+            x = (qq @ k[c].T * cache.dim ** -0.5).masked_fill(torch.arange(length, device=q.device) > pos[:, None], -float("inf"))
+            p = torch.exp(x - lse[:, None])
+            least = 2.0 ** -25 * (p * s[c]).amax(1, keepdim=True) * codes[c].sum(0)
+            off = 2 * ((cache.dim + 8) * 2.0 ** -24 * float(reach) + 2.0 ** -20)
+            bound = half * ref.abs() + (2.0 ** -25 if dtype == "f16" else 0.0) + (1 + half) * (weighted * (off + 2.0 ** -11 + (length + 16) * 2.0 ** -24) + least)
+            assert (bound.amax(1) <= share * ref.abs().amax(1)).all(), "the bound would hide a wrong value"
+            err = (out[at:at + n, h].double() - ref).abs()
+            assert (err <= bound).all(), (b, h, float((err / ref.abs().amax(1, keepdim=True)).max()), float((err / bound).max()))
+        at += n
+
+
+@pytest.mark.parametrize("variant", [0, 1, 2])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("size", [1e-2, 1e-4, 1e-8, 1.0, 100.0])
+def test_a_block_of_zero_values_beside_small_ones(dev, size, dim, variant):
+    """A value block of scale 0 counts in the softmax's sum and nowhere else, however small the other values are; whatever
+    its codes say."""
+    import luisaml_b200 as lb
+    new, lens, heads, group = [1, 40], [600, 333], 2, 2
+    for code in (0x00, 0x7e, 0xfe):  # the last two: what an infinity alone in its block leaves behind
+        cache = Cache(dev, lens, 600, heads, dim, 32, 16)
+        cache.vs *= size
+        for b in range(2):
+            p = int(cache.table[b, 1])
+            cache.v[p, :, 16:] = code
+            cache.vs[p, :, 1] = 0
+        q = (torch.randn(sum(new), heads * group, dim, device=dev) * 1.5).bfloat16()
+        out = lb.kv_attention(q, *cache.args(), cache.table, _cu(new, dev), cache.lens, max_tokens=40, variant=variant)
+        _check_rows(cache, q, new, lens, out, "bf16")
+
+
+@pytest.mark.parametrize("variant", [1, 2])
+@pytest.mark.parametrize("dim,dtype", [(64, "f16"), (128, "bf16")])
+def test_value_scales_far_apart(dev, dim, dtype, variant):
+    """blocks 2^20 apart, zero blocks among them, several queries a sequence"""
+    import luisaml_b200 as lb
+    new, lens, heads, group = [30, 1], [500, 200], 2, 2
+    cache = Cache(dev, lens, 500, heads, dim, 32, 16)
+    g = torch.Generator(device=dev).manual_seed(11)
+    cache.vs *= torch.exp2(torch.randint(-10, 11, cache.vs.shape, device=dev, generator=g).float())
+    for b in range(2):
+        cache.v[int(cache.table[b, 2]), :, :16], cache.vs[int(cache.table[b, 2]), :, 0] = 0, 0
+    q = (torch.randn(sum(new), heads * group, dim, device=dev, generator=g) * 1.5).to(TYPES[dtype])
+    out = lb.kv_attention(q, *cache.args(), cache.table, _cu(new, dev), cache.lens, max_tokens=30, variant=variant)
+    _check_rows(cache, q, new, lens, out, dtype)
+
+
+def test_a_sink_without_values(dev):
+    """a first block of zero values that takes nearly the whole softmax: the rest is small and still right"""
+    import luisaml_b200 as lb
+    for dim in (64, 128):
+        for variant in (1, 2):
+            cache = Cache(dev, [400], 400, 1, dim, 32, 16)
+            p = int(cache.table[0, 0])
+            cache.v[p, :, :16], cache.vs[p, :, 0] = 0, 0
+            cache.k[p, :, :16] = 0x48  # 4.0
+            cache.ks[p, :, 0] = 1.0
+            cache.vs *= 1e-3
+            q = (torch.randn(20, 2, dim, device=dev) * 0.3 + 8.0 / (4.0 * dim ** 0.5)).bfloat16()  # the sink's score is about 8
+            out = lb.kv_attention(q, *cache.args(), cache.table, _cu([20], dev), cache.lens, max_tokens=20, variant=variant)
+            _check_rows(cache, q, [20], [400], out, "bf16")
