@@ -78,7 +78,9 @@ __device__ __forceinline__ Unit find_unit(const lcml_kv_cache &c, const lcml_kv_
     const int start = __ldg(b.lengths + s);
     const int64_t i = u - (t0 / blk + 2 * static_cast<int64_t>(s));  // the sequence's i-th block
     const int64_t first = (static_cast<int64_t>(start) / blk + i) * blk;
-    if (t0 < 0 || start < 0 || first >= static_cast<int64_t>(start) + (t1 - t0)) return r;
+    // A sequence without tokens is not looked at further: its table may hold
+    // anything, and its last page may be another sequence's to write.
+    if (t0 < 0 || t1 <= t0 || start < 0 || first >= static_cast<int64_t>(start) + (t1 - t0)) return r;
     r.first = static_cast<int>(first);
     r.lo = max(0, start - r.first);
     r.hi = static_cast<int>(min(static_cast<int64_t>(blk), start + static_cast<int64_t>(t1 - t0) - first));

@@ -203,3 +203,26 @@ def test_a_sink_without_values(dev):
             q = (torch.randn(20, 2, dim, device=dev) * 0.3 + 8.0 / (4.0 * dim ** 0.5)).bfloat16()  # the sink's score is about 8
             out = lb.kv_attention(q, *cache.args(), cache.table, _cu([20], dev), cache.lens, max_tokens=20, variant=variant)
             _check_rows(cache, q, [20], [400], out, "bf16")
+
+
+def test_sequences_without_new_tokens_are_not_touched(dev):
+    """An idle sequence in the middle of a block: its table is not followed, and a page it shares with a sequence that
+    writes belongs to that one alone."""
+    import luisaml_b200 as lb
+    start, new = [5, 21, 40], [0, 1, 0]
+    cache = Cache(dev, start, 64, 2, 64, 32, 16)
+    k, v = (torch.randn(1, 2, 64, device=dev) * 50 for _ in range(2))
+    table = cache.table.clone()
+    table[0] = -1  # no pages any more
+    cache.table = cache.table[1:2]  # for the oracle: the sequence that writes, alone
+    _check_write(cache, start[1:2], new[1:2], k, v, lambda lb: lb.kv_cache_write(*cache.args(), k, v, table, _cu(new, dev), cache.lens))
+    lb.kv_cache_read(*cache.args(), table, _cu(new, dev), cache.lens, total=1)
+
+
+def test_idle_sequences_on_a_shared_page(dev):
+    start, new = [21] + [20] * 60, [1] + [0] * 60
+    for turn in range(20):
+        cache = Cache(dev, start, 64, 4, 64, 32, 16, seed=turn)
+        cache.table[1:] = cache.table[0]
+        k, v = (torch.randn(1, 4, 64, device=dev) * 50 for _ in range(2))
+        _check_write(cache, start, new, k, v, lambda lb: lb.kv_cache_write(*cache.args(), k, v, cache.table, _cu(new, dev), cache.lens))
