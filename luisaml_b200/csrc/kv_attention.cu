@@ -967,11 +967,14 @@ int lcml_kv_attention(const lcml_kv_attention_desc *d, lcml_stream_t stream) {
     const int64_t need = make_plan(d, 0x7fffffff).bytes;
     LCML_CHECK_ARG(need == 0 || (d->workspace && aligned(d->workspace, 16)), "lcml_kv_attention: needs a 16-byte aligned workspace of %lld bytes",
                    (long long)need);
+    // No sequence is longer than its table reaches: a window of that many hides
+    // nothing, and without it the kernels' position - window keeps to 32 bits.
+    const int64_t reach = static_cast<int64_t>(d->batch->table_cols) * d->cache->page_size;
     AttnArgs a{*d->cache,         *d->batch,          d->q,
                d->out,            d->q_token_stride,  d->q_head_stride,
                d->out_token_stride, d->out_head_stride, d->lse,
                d->q_heads / d->cache->kv_heads, d->dtype == LCML_DTYPE_BFLOAT16, d->softmax_scale * kLog2e,
-               d->softcap,        d->softcap > 0.0f ? d->softmax_scale / d->softcap : 0.0f, d->window,
+               d->softcap,        d->softcap > 0.0f ? d->softmax_scale / d->softcap : 0.0f, d->window < reach ? d->window : 0,
                d->causal ? 1 : 0, d->max_tokens,      device_error_word()};
     cudaStream_t st = to_cuda(stream);
     // Rows a sequence must have for the tensor-core kernel; the streaming

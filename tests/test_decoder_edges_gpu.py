@@ -226,3 +226,11 @@ def test_idle_sequences_on_a_shared_page(dev):
         cache.table[1:] = cache.table[0]
         k, v = (torch.randn(1, 4, 64, device=dev) * 50 for _ in range(2))
         _check_write(cache, start, new, k, v, lambda lb: lb.kv_cache_write(*cache.args(), k, v, cache.table, _cu(new, dev), cache.lens))
+
+
+@pytest.mark.parametrize("variant", [0, 1, 2])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 2, 5000, 100])
+def test_windows_longer_than_any_sequence(dev, window, variant):
+    """with queries before the first token among them"""
+    for new, lens in (([12], [4]), ([40, 3], [30, 200])):
+        _attend(dev, new, lens, 2, 2, 64, 16, 16, "bf16", variant=variant, window=window)
