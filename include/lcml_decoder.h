@@ -70,9 +70,10 @@ typedef struct lcml_kv_cache {
 
 /*
  * A ragged batch: sequence b owns tokens cu_tokens[b] .. cu_tokens[b + 1] - 1
- * of the packed token dimension (cu_tokens[0] = 0, cu_tokens[batch] <=
- * total_tokens), and position t of sequence b lives in slot t % page_size of
- * page block_table[b * table_stride + t / page_size]; cu_tokens does not
+ * of the packed token dimension (cu_tokens[0] >= 0, more where the call takes a
+ * part of a longer batch; cu_tokens[batch] <= total_tokens), and position t of
+ * sequence b lives in slot t % page_size of page
+ * block_table[b * table_stride + t / page_size]; cu_tokens does not
  * decrease. A table entry outside [0, num_pages), or a position past the
  * table's columns, is never followed: a write or read skips it, attention
  * leaves its tokens out (what it returns for that sequence means nothing), and

@@ -244,7 +244,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
         w.pos0 = w.len - w.n;
         const int64_t block = u - (static_cast<int64_t>(w.t0) * a.group / kBlockRows + w.seq);
         const int64_t all = static_cast<int64_t>(w.n) * a.group;
-        if (block * kBlockRows >= all || all < min_rows || w.t0 < 0) return;  // the whole CTA
+        // the whole CTA (block < 0: a unit before the first sequence's, where cu_tokens[0] > 0)
+        if (block < 0 || block * kBlockRows >= all || all < min_rows || w.t0 < 0) return;
         w.row0 = static_cast<int>(block * kBlockRows);
         w.rows = static_cast<int>(min(static_cast<int64_t>(kBlockRows), all - w.row0));
         const int qa = w.row0 / a.group, qz = (w.row0 + w.rows - 1) / a.group;

@@ -234,3 +234,32 @@ def test_windows_longer_than_any_sequence(dev, window, variant):
     """with queries before the first token among them"""
     for new, lens in (([12], [4]), ([40, 3], [30, 200])):
         _attend(dev, new, lens, 2, 2, 64, 16, 16, "bf16", variant=variant, window=window)
+
+
+def test_a_part_of_a_batch(dev):
+    """cu_tokens of sequences 2 .. 4 of a longer batch: the packed tokens keep their places"""
+    import luisaml_b200 as lb
+    new, lens = [300, 5, 70, 0, 40, 9], [300, 50, 100, 30, 333, 60]
+    heads, group, dim = 2, 4, 64
+    for variant in (0, 1, 2):
+        cache = Cache(dev, lens, 340, heads, dim, 32, 16)
+        cu = _cu(new, dev)
+        q = torch.randn(sum(new), heads * group, dim, device=dev).bfloat16()
+        out = torch.full_like(q, 7.0)
+        lb.kv_attention(q, *cache.args(), cache.table[2:5], cu[2:6], cache.lens[2:5], max_tokens=70, variant=variant, out=out)
+        lo, hi = sum(new[:2]), sum(new[:5])
+        whole = Cache(dev, lens, 340, heads, dim, 32, 16)  # the same one
+        whole.table = cache.table[2:5]
+        _check_attention(whole, q[lo:hi], new[2:5], lens[2:5], out[lo:hi])
+        assert (out[:lo] == 7).all() and (out[hi:] == 7).all()
+    start = [n - m for n, m in zip(lens, new)]
+    first = torch.tensor(start, dtype=torch.int32, device=dev)
+    k, v = lb.kv_cache_read(*cache.args(), cache.table[2:5], cu[2:6], first[2:5], total=sum(new), dtype=torch.float32)
+    want = torch.cat([cache.tokens("k", b, lens[b])[:, start[b]:].transpose(0, 1) for b in range(2, 5)])
+    assert torch.equal(k[lo:hi], want.float())
+    x, y = (torch.randn(sum(new), heads, dim, device=dev) * 3 for _ in range(2))
+    other = Cache(dev, start, 340, heads, dim, 32, 16, seed=1)
+    twin = Cache(dev, start, 340, heads, dim, 32, 16, seed=1)
+    lb.kv_cache_write(*other.args(), x, y, other.table[2:5], cu[2:6], first[2:5])
+    lb.kv_cache_write(*twin.args(), x[lo:hi].clone(), y[lo:hi].clone(), twin.table[2:5], _cu(new[2:5], dev), first[2:5])
+    assert all(torch.equal(a.nan_to_num(), b.nan_to_num()) for a, b in zip(other.args(), twin.args()))
