@@ -77,7 +77,8 @@ typedef struct lcml_kv_cache {
  * decrease. A table entry outside [0, num_pages), or a position past the
  * table's columns, is never followed: a write or read skips it, attention
  * leaves its tokens out (what it returns for that sequence means nothing), and
- * the device error word (lcml_device_error) gets code 6.
+ * the device error word (lcml_device_error) gets code 6. A negative length sets
+ * it to 7: a write or read skips the sequence's tokens, to attention it holds none.
  */
 typedef struct lcml_kv_batch {
     int32_t batch;

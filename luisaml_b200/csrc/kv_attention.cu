@@ -116,7 +116,7 @@ struct Span {
     int n, len, lo, steps, tiles;
     int t0;    // first packed token
     int pos0;  // position of query 0 (negative: queries before the first token see nothing)
-    bool cut;  // longer than the call's bounds
+    bool cut;  // longer than the call's bounds, or of negative length
 };
 
 // Sequence s; steps counts from lo over all the keys any of its queries sees,
@@ -127,10 +127,11 @@ __device__ __forceinline__ Span span_of(const AttnArgs &a, int s) {
     Span r;
     r.t0 = __ldg(a.b.cu_tokens + s);
     const int t1 = static_cast<int>(min(static_cast<int64_t>(__ldg(a.b.cu_tokens + s + 1)), a.b.total_tokens));
-    const int n = r.t0 >= 0 ? max(0, t1 - r.t0) : 0, len = max(0, __ldg(a.b.lengths + s));
+    const int held = __ldg(a.b.lengths + s);
+    const int n = r.t0 >= 0 ? max(0, t1 - r.t0) : 0, len = max(0, held);
     r.n = static_cast<int>(min(static_cast<int64_t>(n), a.max_tokens));
     r.len = static_cast<int>(min(static_cast<int64_t>(len), static_cast<int64_t>(a.b.table_cols) * a.c.page_size));
-    r.cut = r.n < n || r.len < len;
+    r.cut = r.n < n || r.len < len || held < 0;
     r.pos0 = r.len - n;
     const int64_t first = static_cast<int64_t>(r.pos0) - a.window + 1;  // the first query's oldest key
     r.lo = a.window > 0 && first > 0 ? static_cast<int>(first) & ~(kStep - 1) : 0;

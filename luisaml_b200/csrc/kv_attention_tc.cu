@@ -237,10 +237,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
         w.seq = find_sequence(a.b.cu_tokens, a.b.batch, u, a.group, kBlockRows, 1);
         w.t0 = __ldg(a.b.cu_tokens + w.seq);
         const int t1 = static_cast<int>(min(static_cast<int64_t>(__ldg(a.b.cu_tokens + w.seq + 1)), a.b.total_tokens));
-        const int len = max(0, __ldg(a.b.lengths + w.seq));
+        const int held = __ldg(a.b.lengths + w.seq), len = max(0, held);
         w.n = w.t0 >= 0 ? max(0, t1 - w.t0) : 0;
         w.len = static_cast<int>(min(static_cast<int64_t>(len), static_cast<int64_t>(a.b.table_cols) * a.c.page_size));
-        if ((w.len < len || w.n > a.max_tokens) && threadIdx.x == 0) record_device_error(a.err, kDevBadBatch);
+        if ((w.len < len || held < 0 || w.n > a.max_tokens) && threadIdx.x == 0) record_device_error(a.err, kDevBadBatch);
         w.pos0 = w.len - w.n;
         const int64_t block = u - (static_cast<int64_t>(w.t0) * a.group / kBlockRows + w.seq);
         const int64_t all = static_cast<int64_t>(w.n) * a.group;

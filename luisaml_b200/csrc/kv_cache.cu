@@ -81,7 +81,10 @@ __device__ __forceinline__ Unit find_unit(const lcml_kv_cache &c, const lcml_kv_
     // A sequence without tokens is not looked at further: its table may hold
     // anything, and its last page may be another sequence's to write.
     // i < 0: a unit before the first sequence's, where cu_tokens[0] > 0.
-    if (i < 0 || t0 < 0 || t1 <= t0 || start < 0 || first >= static_cast<int64_t>(start) + (t1 - t0)) return r;
+    if (i < 0 || t0 < 0 || t1 <= t0 || start < 0 || first >= static_cast<int64_t>(start) + (t1 - t0)) {
+        if (t1 > t0 && start < 0 && threadIdx.x == 0) record_device_error(err, kDevBadBatch);
+        return r;
+    }
     r.first = static_cast<int>(first);
     r.lo = max(0, start - r.first);
     r.hi = static_cast<int>(min(static_cast<int64_t>(blk), start + static_cast<int64_t>(t1 - t0) - first));

@@ -13,7 +13,7 @@ namespace lcml {
 
 // Join the codes of DeviceError. A page number outside the cache or a position
 // past the block table (the access is skipped), and a sequence longer than
-// the call's bounds (its surplus is not computed).
+// the call's bounds (its surplus is not computed) or of negative length.
 constexpr int kDevBadPage = 6;
 constexpr int kDevBadBatch = 7;
 

@@ -263,3 +263,24 @@ def test_a_part_of_a_batch(dev):
     lb.kv_cache_write(*other.args(), x, y, other.table[2:5], cu[2:6], first[2:5])
     lb.kv_cache_write(*twin.args(), x[lo:hi].clone(), y[lo:hi].clone(), twin.table[2:5], _cu(new[2:5], dev), first[2:5])
     assert all(torch.equal(a.nan_to_num(), b.nan_to_num()) for a, b in zip(other.args(), twin.args()))
+
+
+def test_negative_lengths_are_reported(dev):
+    """and count as a sequence that holds nothing (attention) or is not followed (write, read)"""
+    import luisaml_b200 as lb
+    cache = Cache(dev, [20, 30], 64, 2, 64, 32, 16)
+    before = [t.clone() for t in cache.args()]
+    cu = _cu([1, 1], dev)
+    bad = torch.tensor([-3, 30], dtype=torch.int32, device=dev)
+    q = torch.randn(2, 4, 64, device=dev).half()
+    for variant in (1, 2):
+        out = lb.kv_attention(q, *cache.args(), cache.table, cu, bad, max_tokens=1, variant=variant)
+        assert _device_error() == 7
+        assert (out[0] == 0).all()
+    lb.kv_cache_read(*cache.args(), cache.table, cu, bad, total=2)
+    assert _device_error() == 7
+    k = torch.randn(2, 2, 64, device=dev)
+    lb.kv_cache_write(*cache.args(), k, k, cache.table, cu, bad)
+    assert _device_error() == 7
+    p = cache.table[0].long()
+    assert all(torch.equal(a[p].nan_to_num(), b[p].nan_to_num()) for a, b in zip(before, cache.args()))
