@@ -144,7 +144,7 @@ typedef struct lcml_kv_attention_desc {
     const lcml_kv_batch *batch;
     const void *q;            /* [total_tokens, q_heads, head_dim], strides in elements */
     int64_t q_token_stride, q_head_stride;
-    void *out;                /* same shape and type */
+    void *out;                /* same shape and type, rows that do not overlap */
     int64_t out_token_stride, out_head_stride;
     float *lse;               /* optional, dense [total_tokens, q_heads] */
     int32_t q_heads;

@@ -965,6 +965,12 @@ int lcml_kv_attention(const lcml_kv_attention_desc *d, lcml_stream_t stream) {
     LCML_CHECK_ARG(aligned(d->q, 2) && aligned(d->out, 2) && aligned(d->lse, 4), "lcml_kv_attention: a pointer is not aligned to its element size");
     LCML_CHECK_ARG(d->q_token_stride >= 0 && d->q_head_stride >= 0 && d->out_token_stride >= 0 && d->out_head_stride >= 0,
                    "lcml_kv_attention: negative stride");
+    // Rows of out are written by different CTAs: either stride covers the rows of the other.
+    const int64_t tokens = d->batch->total_tokens, heads = d->q_heads, dim = d->cache->head_dim;
+    const int64_t ts = d->out_token_stride, hs = d->out_head_stride;
+    LCML_CHECK_ARG((tokens == 1 || ts >= dim) && (heads == 1 || hs >= dim) &&
+                       (tokens == 1 || heads == 1 || ts >= (heads - 1) * hs + dim || hs >= (tokens - 1) * ts + dim),
+                   "lcml_kv_attention: rows of out overlap (strides %lld and %lld)", (long long)ts, (long long)hs);
     const int64_t need = make_plan(d, 0x7fffffff).bytes;
     LCML_CHECK_ARG(need == 0 || (d->workspace && aligned(d->workspace, 16)), "lcml_kv_attention: needs a 16-byte aligned workspace of %lld bytes",
                    (long long)need);

@@ -284,3 +284,19 @@ def test_negative_lengths_are_reported(dev):
     assert _device_error() == 7
     p = cache.table[0].long()
     assert all(torch.equal(a[p].nan_to_num(), b[p].nan_to_num()) for a, b in zip(before, cache.args()))
+
+
+def test_layouts_of_the_output(dev):
+    """heads first, one head, one token, rows apart"""
+    import luisaml_b200 as lb
+    for new, lens, heads in (([5, 1], [60, 9], 2), ([1], [40], 2), ([6], [33], 1)):
+        cache = Cache(dev, lens, 60, heads, 64, 16, 16)
+        n = sum(new)
+        q = torch.randn(n, heads, 64, device=dev).half()
+        for out in (torch.empty(heads, n, 64, device=dev).half().transpose(0, 1), torch.empty(n, heads, 64, device=dev).half(),
+                    torch.empty(n, 2 * heads + 1, 70, device=dev).half()[:, ::2, 3:67][:, :heads]):
+            lb.kv_attention(q, *cache.args(), cache.table, _cu(new, dev), cache.lens, max_tokens=max(new), out=out)
+            _check_attention(cache, q, new, lens, out)
+        if n > 1:
+            with pytest.raises(lb.LcmlError):
+                lb.kv_attention(q, *cache.args(), cache.table, _cu(new, dev), cache.lens, out=torch.empty(1, heads, 64, device=dev).half().expand(n, -1, -1))
