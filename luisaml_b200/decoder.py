@@ -8,6 +8,7 @@ tensors' device and neither synchronise nor read lengths back: the lengths of a
 ragged batch stay on the device. Codes are uint8 e4m3 as everywhere in this
 package. Refused arguments raise ValueError or LcmlError; a page or length out
 of range is never followed and shows in :func:`luisaml_b200.device_error`.
+Inference only: in grad mode an input that requires a gradient is refused.
 
 A cache is four tensors that the caller keeps::
 

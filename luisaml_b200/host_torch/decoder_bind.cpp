@@ -10,6 +10,7 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -89,6 +90,13 @@ c10::Device device_of(const at::Tensor &first, const Ts *...rest) {
     return d;
 }
 
+// The operators have no backward: a graph through them would end without a word.
+template <typename... Ts>
+void no_gradient(const Ts *...t) {
+    if (at::GradMode::is_enabled())
+        need(((t == nullptr || !t->requires_grad()) && ...), "no gradient flows through this operator: detach its inputs or call it under torch.no_grad()");
+}
+
 at::Tensor empty(at::IntArrayRef size, at::ScalarType t, c10::Device d) { return at::detail::empty_cuda(size, t, d, std::nullopt); }
 
 PyObject *wrap(const at::Tensor &t) {
@@ -149,6 +157,7 @@ PyObject *rmsnorm_quantize(PyObject *const *o) {
     const at::Tensor *r = maybe(o[2], "residual"), *s = maybe(o[4], "scale"), *out = maybe(o[5], "out"), *s_out = maybe(o[6], "scale_out"),
                      *h_out = maybe(o[7], "h_out");
     need(x.dim() == 2, "rmsnorm_quantize: x is [rows, cols]");
+    no_gradient(&x, &w, r, s);
     const c10::Device dev = device_of(x, &w, r, s, out, s_out, h_out);
     lcml_rmsnorm_desc d{};
     const int64_t rows = d.rows = x.size(0), cols = d.cols = x.size(1);
@@ -215,6 +224,7 @@ PyObject *kv_cache_write(PyObject *const *o) {
     const at::Tensor &kc = tensor(o[0], "k_cache"), &vc = tensor(o[1], "v_cache"), &ks = tensor(o[2], "k_scale"), &vs = tensor(o[3], "v_scale"),
                      &k = tensor(o[4], "k"), &v = tensor(o[5], "v"), &table = tensor(o[6], "block_table"), &cu = tensor(o[7], "cu_tokens"),
                      &start = tensor(o[8], "start");
+    no_gradient(&k, &v, &ks, &vs);
     const c10::Device dev = device_of(kc, &vc, &ks, &vs, &k, &v, &table, &cu, &start);
     const lcml_kv_cache c = cache_of(kc, vc, ks, vs);
     const int dt = dtype_of(k, "k");
@@ -237,6 +247,7 @@ PyObject *kv_cache_read(PyObject *const *o) {
     const int dt = dtype_code(t);
     need(dt != 0, "kv_cache_read: dtype is float32, float16 or bfloat16");
     need(total >= 0, "kv_cache_read: negative total");
+    no_gradient(&ks, &vs);
     const c10::Device dev = device_of(kc, &vc, &ks, &vs, &table, &cu, &start);
     const lcml_kv_cache c = cache_of(kc, vc, ks, vs);
     const lcml_kv_batch b = batch_of(table, cu, start, total);
@@ -256,6 +267,7 @@ PyObject *kv_attention(PyObject *const *o) {
     const at::Tensor &q = tensor(o[0], "q"), &kc = tensor(o[1], "k_cache"), &vc = tensor(o[2], "v_cache"), &ks = tensor(o[3], "k_scale"),
                      &vs = tensor(o[4], "v_scale"), &table = tensor(o[5], "block_table"), &cu = tensor(o[6], "cu_tokens"), &len = tensor(o[7], "kv_len");
     const at::Tensor *out = maybe(o[13], "out"), *lse = maybe(o[14], "lse"), *ws = maybe(o[15], "workspace");
+    no_gradient(&q, &ks, &vs);
     const c10::Device dev = device_of(q, &kc, &vc, &ks, &vs, &table, &cu, &len, out, lse, ws);
     const lcml_kv_cache c = cache_of(kc, vc, ks, vs);
     need(q.dim() == 3 && q.size(2) == c.head_dim && q.stride(2) == 1, "kv_attention: q is [tokens, q_heads, head_dim] with contiguous rows");
