@@ -30,7 +30,14 @@ __all__ = [*_DECODER, "lib", "check", "LcmlError", "quantize", "quantize_from_am
 
 def __getattr__(name):
     if name in _DECODER:  # luisaml_b200.decoder imports torch, which this module does only when a call needs it
-        from . import decoder
+        try:
+            from . import decoder
+        except Exception as e:  # no torch or no binding: for the call to say, so that `import *` needs neither
+            why = e
+
+            def missing(*args, **kwargs):
+                raise ImportError(f"luisaml_b200.{name}: {why}") from why
+            return missing
         globals().update({n: getattr(decoder, n) for n in _DECODER})
         return globals()[name]
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

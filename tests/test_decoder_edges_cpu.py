@@ -1,8 +1,11 @@
 """Refusals of the decoder-layer operators that need no GPU, beyond those of test_decoder_cpu.py."""
 import ctypes
+import subprocess
+import sys
 
 import pytest
 
+from conftest import ROOT
 from test_decoder_cpu import _attention, _batch, _cache, capi  # noqa: F401
 
 
@@ -29,3 +32,13 @@ def test_inputs_that_require_a_gradient_are_refused(capi):
             call()
         with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):  # the next check: these are host tensors
             call()
+
+
+def test_star_import_without_torch():
+    """the names are there, and the call says what is missing"""
+    code = ("import sys; sys.modules['torch'] = None\n"
+            "from luisaml_b200 import *\n"
+            "assert quantize and check\n"
+            "try:\n    kv_attention(None)\nexcept ImportError as e:\n    assert 'kv_attention' in str(e) and 'torch' in str(e); print('said so')")
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=ROOT)
+    assert out.returncode == 0 and "said so" in out.stdout, out.stderr
