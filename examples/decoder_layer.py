@@ -3,7 +3,7 @@ different lengths, then token by token from a CUDA graph.
 
     python examples/decoder_layer.py [--batch 16] [--prompt 500] [--steps 64]
 
-One step is eight calls of luisaml_b200: norm (with the residual's addition) ->
+One step is ten calls of luisaml_b200: norm (with the residual's addition) ->
 QKV GEMM -> cache write -> attention -> row quantization -> output GEMM -> norm
 -> FFN up (SiLU(gate) * up in the GEMM) -> row quantization -> FFN down. The
 prompt's and the steps' outputs are checked against the same layer in plain

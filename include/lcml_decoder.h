@@ -127,10 +127,13 @@ int lcml_kv_cache_read(const lcml_kv_cache *cache, const lcml_kv_batch *batch, v
  *   x_j = softmax_scale * q . k_j;  softcap > 0: x_j = softcap * tanh(x_j / softcap)
  *   out = sum_j softmax(x)_j v_j,   lse = log sum_j exp(x_j)
  * A query that sees nothing gets zeros and lse -inf. Scores, the softmax's
- * maximum and sum, and the output accumulate in fp32; q and the softmax's
- * weights enter the matrix products as 16-bit floats or, on the tensor-core
- * path, q as a sum of e4m3 parts that reproduce it. What the masked slots
- * hold (NaN codes included) does not matter.
+ * maximum and sum, and the output accumulate in fp32. The softmax's weights enter
+ * the product with the values as halves (11 significant bits: FLOAT16 outputs
+ * measured 2.9e-4 off, 2.1e-4 of it their own rounding), q as it is or, on the
+ * tensor-core path, as a sum of e4m3 parts: exact for elements above 2^-9
+ * (BFLOAT16) or 2^-6 (FLOAT16) of the row's largest, within 2^-17 of that one
+ * for smaller ones. A value block of scale 0 counts in the sum alone. What the
+ * masked slots hold (NaN codes included) does not matter.
  * max_tokens: an upper bound of the n (host side). It and the extents pick the
  * kernels: the closer it is, the fewer launches (exact for a batch of equal
  * lengths). Where total_tokens is padded, the padded total picks, and every

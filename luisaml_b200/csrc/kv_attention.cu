@@ -22,7 +22,9 @@
 // takes e4m3 operands too, but converts them itself for every use: measured
 // slower); the block scales multiply the scores (keys) and join the exponent
 // (values, value_scale()). P^T reaches its operand layout by one movmatrix per
-// 8 keys.
+// 8 keys. The weights are rounded to halves for their product, 2^-11 of each: codes
+// are exact in halves and both operands of the MMA have one type; in tf32 (the
+// same 11 bits) the product would take twice the instructions. Sums keep fp32.
 //
 // At a segment's end each warp leaves its (m, l, O) in shared memory and goes
 // on; the last of them joins and writes. A segment that lies in several CTAs
@@ -34,16 +36,20 @@
 // Bound: HBM, 2 head_dim bytes per key and cache head (one token of a
 // 131072-token sequence, 8 cache heads of 128: 65 us, 4.2 of a copy's 6.5 TB/s:
 // 5.3 TB/s while it streams, the rest is the plan, the first copies and the
-// join; of 64 sequences of up to 4096: 77 us).
+// join; of 64 sequences of up to 4096: 77 us). Several tokens at head_dim 256 have
+// no other kernel than this one's tiles of 8 rows, which copy and convert the keys
+// once per tile: 4 tokens of 16 sequences of 2000 66 us (floor 20), a prompt of
+// 4096 5.6 ms (floor 166 us).
 #include "lcml_attention.cuh"
 
 namespace lcml {
 namespace {
 
 constexpr int kStep = 16;          // keys per warp step
-// Up to here splitting a segment costs more than it gains: 32 steps in one CTA
-// or split, one token of 64 sequences of 500: 25.9 and 27.2 us (head_dim 64:
-// 14.7 and 19.2), of 1 sequence 12.1 and 11.0.
+// Up to here segments are not split. With many of them that is faster: 32 steps
+// in one CTA or split, one token of 64 sequences of 500 25.9 and 27.2 us
+// (head_dim 64: 14.7 and 19.2). With few it is not, 12.1 and 11.0 for 1
+// sequence: the number of segments, which the host can bound, is not looked at yet.
 constexpr int kWholeSteps = 64;
 constexpr int kMaxBatch = 1024;    // sequences per launch (the plan's table in shared memory)
 

@@ -12,7 +12,8 @@
 // no key is converted.
 // Values are converted to halves (exact) by one warpgroup, from global memory
 // into the MN-major 128-byte-swizzled layout of the B operand: the weights
-// need more range than e4m3 has.
+// need more range than e4m3 has. They are rounded to halves, 2^-11 of each: A and
+// B of the MMA have one type, and tf32 would halve its rate for the same 11 bits.
 //
 // Roles (16 warps): 0-3 and 4-7 softmax of tile 0 and 1 (a row per thread, no
 // shuffles), 8-11 value conversion, 12 look-ups and TMA of the keys, 13 MMA
@@ -22,7 +23,8 @@
 // Bound: the tensor cores (4 head_dim FLOP per visible pair) and the
 // exponentials, 16 a clock per SM: equal at head_dim 128, twice the products'
 // time at 64. Measured at 128 (two prompts of up to 4096, 32 heads over 8, bf16):
-// 235 us, 0.75 PFLOP/s. A pair of key tiles takes 3450 clocks, of which the
+// 236 us, 0.75 PFLOP/s (both of 4096: 327; with capped scores, which take every
+// tile in the two passes of the masked ones, 613). A pair of key tiles takes 3450 clocks, of which the
 // MMAs run 2048 and the weights of one row tile 1650. What was tried beside:
 // P V of the first 64 keys under the weights of the others (one row tile 3360 ->
 // 2860 clocks, two 3760 -> 3940), scores of 64 keys at a time (an MMA of half

@@ -11,10 +11,13 @@
 //
 // Bound: the read by HBM (32 x 2000 tokens, 8 heads of 128, to bf16: 61 us, 4.8
 // of a copy's 6.5 TB/s; three quarters of its bytes are writes); the write of
-// prompts by the instructions of the exact rounding, 23 an element (5
-// prompts of 4000 tokens, f16: 38 us, 2.8 TB/s); decode steps by the chain of
-// dependent look-ups (cu -> length -> page -> codes and scales) of a few L2
-// latencies (one token of 64 sequences: 9 us).
+// prompts by latency at low occupancy, of loads and of the exact rounding's
+// 23 instructions an element (5 prompts of up to 4000 tokens, f16: 38 us, 2.8 TB/s;
+// 54 % of the issue slots used, 23 % of the warps active: 64-thread CTAs of 123
+// registers); decode steps by the chain of dependent look-ups (cu -> length ->
+// page -> codes and scales) of a few L2 latencies, the write's also by the four
+// items a CTA takes in turn (one token of 64 sequences, in a graph: write 9.1 us,
+// read 5.5).
 #include "lcml_decoder.cuh"
 
 namespace lcml {

@@ -61,8 +61,9 @@ __device__ __forceinline__ void e4m3x4_to_half2(uint32_t w, uint32_t &lo, uint32
 // comes to [128, 256); part 1 is the nearest e4m3 value of that, part 2 the
 // nearest of what is left, and so on. e4m3 has 4 significant bits and the rest
 // has a sign, so two parts are a bf16 (8 bits) exactly and three an fp16 (11),
-// but for elements so small that e4m3's least step (2^-9) rounds them: an
-// error of 2^-10, 2^-17 of the row's largest element. A row with an infinity
+// but for elements whose last bit is below e4m3's least step (2^-9; those less
+// than 2^-9, for fp16 2^-6, of the row's largest): an error of 2^-10, 2^-17 of the
+// row's largest element. A row with an infinity
 // or NaN becomes NaN.
 template <int NP>
 struct QScale {
