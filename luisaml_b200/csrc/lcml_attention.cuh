@@ -46,7 +46,7 @@ __device__ __forceinline__ float cap_score(float dot, float inv_cap, float cap) 
 // share of the sum, so any scale small enough does: 2^-80 keeps its keys out of
 // the reference maximum m (as 1 they would push the other weights by their
 // scales, e.g. 2^-16 for values of 0.01, into subnormal halves), and its weights
-// only flush to 0 (2^-126) where they are 2^-46 of the largest over the largest
+// only flush to 0 (2^-126) below about 2^-46 of the largest weight times its
 // scale. Scales below 2^-100 do not occur in a written cache and count as 0.
 __device__ __forceinline__ float value_scale(float s) { return s >= 7.888609052210118e-31f ? s : 8.271806125530277e-25f; }
 
