@@ -9,7 +9,8 @@ Layers:
   call the C ABI;
 * ``decoder``             the operators of a decoder layer around the FP8 GEMMs
   (``include/lcml_decoder.h``): RMS norm with an e4m3 output, the paged e4m3
-  key/value cache and the attention over it;
+  key/value cache and the attention over it; the plan of a batch, rotation and
+  sampling of its step (``include/lcml_decode_step.h``);
 * this module: torch-tensor helpers over the C ABI (device memory, streams)
   used by tests and bench.py. PyTorch is plumbing here, not the product.
 """
@@ -21,7 +22,8 @@ from . import _capi
 from ._capi import (TENSOR_DYNAMIC_WORKSPACE_BYTES, DTYPE_BFLOAT16, DTYPE_E4M3, DTYPE_FLOAT, EPI_NONE, EPI_RELU, EPI_SILU_MUL, SCALE_AXIS,
                     SCALE_COL, SCALE_ROW, SCALE_TENSOR, GemmDesc, LcmlError, check)
 
-_DECODER = ("rmsnorm_quantize", "kv_cache_write", "kv_cache_read", "kv_attention", "kv_attention_workspace_size")
+_DECODER = ("rmsnorm_quantize", "kv_cache_write", "kv_cache_read", "kv_attention", "kv_attention_workspace_size", "kv_plan",
+            "qk_norm_rope", "sample")
 
 __all__ = [*_DECODER, "lib", "check", "LcmlError", "quantize", "quantize_from_amax", "quantize_rows_dynamic",
            "quantize_tensor_dynamic", "amax", "dequantize", "transpose_u8", "gemm", "gemm_rowquant", "launch_count",

@@ -1,5 +1,5 @@
-"""ctypes binding of the C ABI in include/lcml_fp8.h and include/lcml_decoder.h
-(liblcml_fp8.so).
+"""ctypes binding of the C ABI in include/lcml_fp8.h, include/lcml_decoder.h and
+include/lcml_decode_step.h (liblcml_fp8.so).
 
 This is the binding a Python caller of the reference's operator path would
 add; tests and bench.py go through it so every GPU number is measured across
@@ -125,6 +125,39 @@ class KvAttentionDesc(ctypes.Structure):
     ]
 
 
+class KvPlanDesc(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int32), ("page_size", ctypes.c_int32), ("table_cols", ctypes.c_int32),
+        ("table_stride", ctypes.c_int64), ("block_table", ctypes.c_void_p), ("new_tokens", ctypes.c_void_p),
+        ("held", ctypes.c_void_p), ("ended", ctypes.c_void_p), ("free_pages", ctypes.c_void_p),
+        ("free_capacity", ctypes.c_int64), ("free_count", ctypes.c_void_p), ("total_tokens", ctypes.c_int64),
+        ("cu_tokens", ctypes.c_void_p), ("start", ctypes.c_void_p), ("kv_len", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p), ("slots", ctypes.c_void_p), ("free_count_out", ctypes.c_void_p),
+    ]
+
+
+class QkNormRopeDesc(ctypes.Structure):
+    _fields_ = [
+        ("tokens", ctypes.c_int64), ("q_heads", ctypes.c_int32), ("k_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("rotary", ctypes.c_int32), ("dtype", ctypes.c_int), ("interleaved", ctypes.c_int),
+        ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("q_token_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64),
+        ("k_token_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64), ("q_out", ctypes.c_void_p),
+        ("k_out", ctypes.c_void_p), ("q_out_token_stride", ctypes.c_int64), ("q_out_head_stride", ctypes.c_int64),
+        ("k_out_token_stride", ctypes.c_int64), ("k_out_head_stride", ctypes.c_int64), ("q_weight", ctypes.c_void_p),
+        ("k_weight", ctypes.c_void_p), ("weight_dtype", ctypes.c_int), ("eps", ctypes.c_float),
+        ("positions", ctypes.c_void_p), ("inv_freq", ctypes.c_void_p), ("inv_freq_dtype", ctypes.c_int),
+    ]
+
+
+class SampleDesc(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64), ("vocab", ctypes.c_int64), ("logits", ctypes.c_void_p), ("ld", ctypes.c_int64),
+        ("dtype", ctypes.c_int), ("uniform", ctypes.c_void_p), ("temperature", ctypes.c_void_p),
+        ("top_k", ctypes.c_void_p), ("top_p", ctypes.c_void_p), ("min_p", ctypes.c_void_p), ("tokens", ctypes.c_void_p),
+        ("logprob", ctypes.c_void_p),
+    ]
+
+
 _c_i64 = ctypes.c_int64
 _vp = ctypes.c_void_p
 _ci = ctypes.c_int
@@ -190,6 +223,10 @@ PROTOTYPES = {
     "lcml_kv_cache_read": [ctypes.POINTER(KvCache), ctypes.POINTER(KvBatch), _vp, _vp, _ci, _vp],
     "lcml_kv_attention_workspace_size": [ctypes.POINTER(KvAttentionDesc)],
     "lcml_kv_attention": [ctypes.POINTER(KvAttentionDesc), _vp],
+    "lcml_kv_plan": [ctypes.POINTER(KvPlanDesc), _vp],
+    "lcml_qk_norm_rope": [ctypes.POINTER(QkNormRopeDesc), _vp],
+    "lcml_kv_attention_sinks": [ctypes.POINTER(KvAttentionDesc), ctypes.c_int32, _vp],
+    "lcml_sample": [ctypes.POINTER(SampleDesc), _vp],
 }
 _RESTYPES = {
     "lcml_last_error": ctypes.c_char_p,

@@ -42,6 +42,8 @@
 // 4096 5.6 ms (floor 166 us).
 #include "lcml_attention.cuh"
 
+#include "../../include/lcml_decode_step.h"
+
 namespace lcml {
 namespace {
 
@@ -118,19 +120,24 @@ struct JoinItem {
     int pad[3];
 };
 
+template <bool SINKS>
 struct Span {
     int n, len, lo, steps, tiles;
+    int sink_steps;  // steps over the first keys, before those from lo on (SINKS)
     int t0;    // first packed token
     int pos0;  // position of query 0 (negative: queries before the first token see nothing)
     bool cut;  // longer than the call's bounds, or of negative length
+    __device__ __forceinline__ int key(int step) const {
+        return SINKS ? (step < sink_steps ? step * kStep : lo + (step - sink_steps) * kStep) : lo + step * kStep;
+    }
 };
 
-// Sequence s; steps counts from lo over all the keys any of its queries sees,
-// and PAD empty ones: CTAs with many short segments would be late otherwise
+// Sequence s; steps counts over all the keys any of its queries sees, the sinks
+// below lo and those from lo on, and PAD empty ones: CTAs with many short segments would be late otherwise
 // (and a row without keys still gets its zeros).
-template <int ROWS, int PAD>
-__device__ __forceinline__ Span span_of(const AttnArgs &a, int s) {
-    Span r;
+template <int ROWS, int PAD, bool SINKS>
+__device__ __forceinline__ Span<SINKS> span_of(const AttnArgs &a, int s) {
+    Span<SINKS> r;
     r.t0 = __ldg(a.b.cu_tokens + s);
     const int t1 = static_cast<int>(min(static_cast<int64_t>(__ldg(a.b.cu_tokens + s + 1)), a.b.total_tokens));
     const int held = __ldg(a.b.lengths + s);
@@ -141,7 +148,8 @@ __device__ __forceinline__ Span span_of(const AttnArgs &a, int s) {
     r.pos0 = r.len - n;
     const int64_t first = static_cast<int64_t>(r.pos0) - a.window + 1;  // the first query's oldest key
     r.lo = a.window > 0 && first > 0 ? static_cast<int>(first) & ~(kStep - 1) : 0;
-    r.steps = (r.len - r.lo + kStep - 1) / kStep + PAD;
+    r.sink_steps = SINKS ? min((a.sinks + kStep - 1) / kStep, r.lo / kStep) : 0;
+    r.steps = r.sink_steps + (r.len - r.lo + kStep - 1) / kStep + PAD;
     r.tiles = static_cast<int>((static_cast<int64_t>(r.n) * a.group + ROWS - 1) / ROWS);
     return r;
 }
@@ -219,7 +227,7 @@ __device__ __forceinline__ uint32_t nan_cleared(uint32_t w) {
     return w & ~((m >> 7) * 0xffu);
 }
 
-template <int D, int RG, bool BF16, bool CAP>
+template <int D, int RG, bool BF16, bool CAP, bool SINKS>
 __global__ void __launch_bounds__(Shape<D, RG>::kThreads, Shape<D, RG>::kCtasPerSm) k_kv_attention(AttnArgs a, int max_rows, bool whole, int part_rows,
                                                                                           JoinItem *join_items, float *part_ml, float *part_o) {
     using S = Shape<D, RG>;
@@ -243,6 +251,7 @@ __global__ void __launch_bounds__(Shape<D, RG>::kThreads, Shape<D, RG>::kCtasPer
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, c = lane & 3;
     const int heads = a.c.kv_heads, batch = a.b.batch;
+    const int sinks = SINKS ? a.sinks : 0;
 
     // The plan: where each sequence's steps begin in the list, and the steps
     // of its segments. Sequences of more than max_rows rows are left to the
@@ -255,7 +264,7 @@ __global__ void __launch_bounds__(Shape<D, RG>::kThreads, Shape<D, RG>::kCtasPer
             const int s = s0 + threadIdx.x;
             int64_t mine = 0;
             if (s < batch) {
-                const Span p = span_of<kRows, S::kPad>(a, s);
+                const auto p = span_of<kRows, S::kPad, SINKS>(a, s);
                 if (p.cut && blockIdx.x == 0) record_device_error(a.err, kDevBadBatch);
                 if (static_cast<int64_t>(p.n) * a.group <= max_rows) mine = static_cast<int64_t>(p.tiles) * heads * p.steps;
                 plan_steps[s] = p.steps;
@@ -331,11 +340,11 @@ __global__ void __launch_bounds__(Shape<D, RG>::kThreads, Shape<D, RG>::kCtasPer
             const int th = in <= 0x7fffffff ? static_cast<int>(in) / steps : static_cast<int>(in / steps);  // 64-bit division is slow
             const int st = static_cast<int>(in - static_cast<int64_t>(th) * steps);
             const int tile = th / heads, head = th - tile * heads;
-            const Span sp = span_of<kRows, S::kPad>(a, s);
-            const int key = sp.lo + st * kStep;
+            const auto sp = span_of<kRows, S::kPad, SINKS>(a, s);
+            const int key = sp.key(st);
             const int row_a = tile * kRows / a.group, row_z = (min(tile * kRows + kRows, sp.n * a.group) - 1) / a.group;
             const int hi = a.causal ? min(sp.pos0 + row_z, sp.len - 1) : sp.len - 1, lo = a.window > 0 ? sp.pos0 + row_a - a.window + 1 : 0;
-            if (key <= hi && key + kStep > lo) {
+            if (key <= hi && (key + kStep > lo || (SINKS && key < sinks))) {
                 const int col = key / page_size, slot = key - col * page_size;
                 const int64_t page = __ldg(a.b.block_table + s * a.b.table_stride + col);  // key < len <= the table's reach
                 if (page >= 0 && page < a.c.num_pages) {
@@ -404,7 +413,7 @@ __global__ void __launch_bounds__(Shape<D, RG>::kThreads, Shape<D, RG>::kCtasPer
             ++seq;
             th = 0;
         }
-        const Span sp = span_of<kRows, S::kPad>(a, seq);
+        const auto sp = span_of<kRows, S::kPad, SINKS>(a, seq);
         const int tile = th / heads, head = th - tile * heads;
         const int seg = static_cast<int>(plan_first[seq] + static_cast<int64_t>(th) * sp.steps - from);  // the segment's first step
         const int end = min(seg + sp.steps, span);
@@ -504,7 +513,7 @@ __global__ void __launch_bounds__(Shape<D, RG>::kThreads, Shape<D, RG>::kCtasPer
             st = st == (kStages - 1) * S::kStageBytes ? 0 : st + S::kStageBytes;
             const float ks = __shfl_sync(0xffffffffu, cur.k, i & 31), vs = __shfl_sync(0xffffffffu, cur.v, i & 31);
             if (vs == 0.0f) continue;
-            const int key = sp.lo + (warp + i * kWarps - seg) * kStep;
+            const int key = sp.key(warp + i * kWarps - seg);
             // scores: keys g, g + 8 x rows 2c, 2c + 1 (+ 8)
             float x[RG][4];
 #pragma unroll
@@ -523,7 +532,7 @@ __global__ void __launch_bounds__(Shape<D, RG>::kThreads, Shape<D, RG>::kCtasPer
                 }
             }
             const float lvs = __log2f(vs), inv_vs = __fdividef(1.0f, vs);
-            const bool edge = key < all_lo || key + kStep - 1 > all_hi;
+            const bool edge = (key < all_lo && (!SINKS || key + kStep > sinks)) || key + kStep - 1 > all_hi;
             float e[RG][2][2], rows_sum[RG][2];  // weights [row][key g, g + 8]
             // Weights against the running reference maximum, which moves only
             // when a weight passes 2^8 (halves have room for that): no exchange
@@ -556,7 +565,7 @@ __global__ void __launch_bounds__(Shape<D, RG>::kThreads, Shape<D, RG>::kCtasPer
                         for (int k = 0; k < 2; ++k) {
                             const float y = CAP ? cap_score(x[rg][2 * k + r], f, a.cap) + lvs : fmaf(x[rg][2 * k + r], f, lvs);
                             const int at_key = key + g + 8 * k;
-                            e[rg][r][k] = at_key <= last[rg][r] && at_key >= first[rg][r] ? y : -INFINITY;
+                            e[rg][r][k] = at_key <= last[rg][r] && (at_key >= first[rg][r] || (SINKS && at_key < sinks)) ? y : -INFINITY;
                         }
                         float t = fmaxf(e[rg][r][0], e[rg][r][1]);
                         t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 4));
@@ -651,7 +660,7 @@ __global__ void __launch_bounds__(Shape<D, RG>::kThreads, Shape<D, RG>::kCtasPer
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
                             const int at_key = key + 2 * c + (k & 1) + (k >> 1) * 8;
-                            see[k] = at_key <= hi && at_key >= lo ? 1.0f : 0.0f;
+                            see[k] = at_key <= hi && (at_key >= lo || (SINKS && at_key < sinks)) ? 1.0f : 0.0f;
                         }
                         const uint32_t s0 = half2_bits(see[0], see[1]), s1 = half2_bits(see[2], see[3]);
 #pragma unroll
@@ -908,6 +917,14 @@ Plan make_plan(const lcml_kv_attention_desc *d, int max_rows) {
     return p;
 }
 
+// A kernel with sinks and one without: their tests cost 4 tokens of 16 sequences, which
+// have none, 1.2 us of 28.4.
+template <int D, int RG, bool SINKS>
+auto stream_kernel(const AttnArgs &a) {
+    return a.bf16 ? (a.cap != 0.0f ? k_kv_attention<D, RG, true, true, SINKS> : k_kv_attention<D, RG, true, false, SINKS>)
+                  : (a.cap != 0.0f ? k_kv_attention<D, RG, false, true, SINKS> : k_kv_attention<D, RG, false, false, SINKS>);
+}
+
 template <int D, int RG>
 int launch_stream(const lcml_kv_attention_desc *d, const AttnArgs &args, const Plan &p, int max_rows, cudaStream_t st) {
     using S = Shape<D, RG>;
@@ -915,8 +932,7 @@ int launch_stream(const lcml_kv_attention_desc *d, const AttnArgs &args, const P
     JoinItem *items = p.whole ? nullptr : reinterpret_cast<JoinItem *>(ws + p.items);
     float *ml = p.whole ? nullptr : reinterpret_cast<float *>(ws + p.ml);
     float *o = p.whole ? nullptr : reinterpret_cast<float *>(ws + p.o);
-    auto kern = args.bf16 ? (args.cap != 0.0f ? k_kv_attention<D, RG, true, true> : k_kv_attention<D, RG, true, false>)
-                          : (args.cap != 0.0f ? k_kv_attention<D, RG, false, true> : k_kv_attention<D, RG, false, false>);
+    auto kern = args.sinks > 0 ? stream_kernel<D, RG, true>(args) : stream_kernel<D, RG, false>(args);
     int rc = ensure_max_smem(reinterpret_cast<const void *>(kern), S::kSmem, "kv_attention");
     for (int64_t b0 = 0; rc == LCML_OK && b0 < d->batch->batch; b0 += kMaxBatch) {
         AttnArgs a = args;
@@ -957,15 +973,18 @@ using namespace lcml;
 
 extern "C" {
 
+int lcml_kv_attention(const lcml_kv_attention_desc *d, lcml_stream_t stream) { return lcml_kv_attention_sinks(d, 0, stream); }
+
 int64_t lcml_kv_attention_workspace_size(const lcml_kv_attention_desc *d) {
     if (check_attention(d) != LCML_OK) return -1;
     if (d->batch->batch == 0 || d->batch->total_tokens == 0) return 0;
     return make_plan(d, 0x7fffffff).bytes;
 }
 
-int lcml_kv_attention(const lcml_kv_attention_desc *d, lcml_stream_t stream) {
+int lcml_kv_attention_sinks(const lcml_kv_attention_desc *d, int32_t sinks, lcml_stream_t stream) {
     const int rc = check_attention(d);
     if (rc != LCML_OK) return rc;
+    LCML_CHECK_ARG(sinks >= 0, "lcml_kv_attention: sinks is negative");
     if (d->batch->batch == 0 || d->batch->total_tokens == 0) return LCML_OK;
     LCML_CHECK_ARG(d->q && d->out, "lcml_kv_attention: null pointer");
     LCML_CHECK_ARG(aligned(d->q, 2) && aligned(d->out, 2) && aligned(d->lse, 4), "lcml_kv_attention: a pointer is not aligned to its element size");
@@ -981,14 +1000,17 @@ int lcml_kv_attention(const lcml_kv_attention_desc *d, lcml_stream_t stream) {
     LCML_CHECK_ARG(need == 0 || (d->workspace && aligned(d->workspace, 16)), "lcml_kv_attention: needs a 16-byte aligned workspace of %lld bytes",
                    (long long)need);
     // No sequence is longer than its table reaches: a window of that many hides
-    // nothing, and without it the kernels' position - window keeps to 32 bits.
+    // nothing, and without it the kernels' position - window keeps to 32 bits. No
+    // more sinks than that, so the kernels round them up to whole steps.
     const int64_t reach = static_cast<int64_t>(d->batch->table_cols) * d->cache->page_size;
+    const int window = d->window < reach ? d->window : 0;
+    const int64_t most_sinks = reach < 0x7fff0000 ? reach : 0x7fff0000;
     AttnArgs a{*d->cache,         *d->batch,          d->q,
                d->out,            d->q_token_stride,  d->q_head_stride,
                d->out_token_stride, d->out_head_stride, d->lse,
                d->q_heads / d->cache->kv_heads, d->dtype == LCML_DTYPE_BFLOAT16, d->softmax_scale * kLog2e,
-               d->softcap,        d->softcap > 0.0f ? d->softmax_scale / d->softcap : 0.0f, d->window < reach ? d->window : 0,
-               d->causal ? 1 : 0, d->max_tokens,      device_error_word()};
+               d->softcap,        d->softcap > 0.0f ? d->softmax_scale / d->softcap : 0.0f, window,
+               d->causal ? 1 : 0, d->max_tokens,      device_error_word(), window == 0 ? 0 : static_cast<int>(sinks < most_sinks ? sinks : most_sinks)};
     cudaStream_t st = to_cuda(stream);
     // Rows a sequence must have for the tensor-core kernel; the streaming
     // kernel takes the others. One launch where the bound or the variant says

@@ -210,14 +210,18 @@ __device__ __forceinline__ float sum16(const float *x) {
 }
 
 // The CTA's work, known to every thread.
+template <bool SINKS>
 struct Work {
     int seq, head, rows;      // rows in this block (<= kBlockRows)
     int row0;                 // first row within the sequence
     int t0, n, len, pos0;     // packed first token, queries, tokens held, position of query 0
-    int tile_lo, tiles;       // first key tile and how many
+    int lo, hi;               // the keys that some row sees (and the sinks)
+    int tile_lo, tiles;       // first key tile of the window, and how many in all
+    int sink_tiles;           // of which over the first keys, before the window's (SINKS)
+    __device__ __forceinline__ int tile(int j) const { return SINKS && j < sink_tiles ? j : tile_lo + (SINKS ? j - sink_tiles : j); }
 };
 
-template <int D, int NP, bool CAP>
+template <int D, int NP, bool CAP, bool SINKS>
 __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_constant__ CUtensorMap k_map, AttnArgs a, int box_rows,
                                                                  int min_rows) {
     using S = Shape<D, NP>;
@@ -232,7 +236,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
 
     // Units are handed out from the last one: within a sequence the last rows
     // see the most keys, and the longest units should not start last.
-    Work w;
+    Work<SINKS> w;
+    const int sinks = SINKS ? a.sinks : 0;
     {
         w.head = blockIdx.x % a.c.kv_heads;
         const int64_t u = (gridDim.x - 1 - blockIdx.x) / a.c.kv_heads;
@@ -254,7 +259,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
         const int hi = a.causal ? min(w.pos0 + qz, w.len - 1) : w.len - 1;  // the last key any row sees
         const int lo = a.window > 0 ? max(0, w.pos0 + qa - a.window + 1) : 0;
         w.tile_lo = lo / kTile;
-        w.tiles = hi >= lo ? hi / kTile - w.tile_lo + 1 : 0;
+        w.sink_tiles = SINKS ? min((sinks + kTile - 1) / kTile, w.tile_lo) : 0;
+        w.tiles = hi >= lo ? hi / kTile - w.tile_lo + 1 + w.sink_tiles : 0;
+        w.lo = lo;
+        w.hi = hi;
     }
     const bool two = w.rows > kTile;
 
@@ -300,14 +308,19 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
             // Look-ups run two tiles ahead of their use: table entries for
             // j + 2 and scales for j + 1 are in flight while j is published.
             const int32_t *table = a.b.block_table + w.seq * a.b.table_stride;
+            const int groups_per_box = box_rows / 16;
+            // position of group `lane` of tile j, -1: no token (or, with sinks, in a box that no row sees)
+            auto place = [&](int j) -> int64_t {
+                const int64_t pos = static_cast<int64_t>(w.tile(j)) * kTile + lane * 16, box = pos - lane % groups_per_box * 16;
+                return lane >= kGroups || j >= n || pos >= w.len || (SINKS && (box > w.hi || (box + box_rows <= w.lo && box >= sinks))) ? -1 : pos;
+            };
             auto entry = [&](int j) -> int {  // page of group `lane` of tile j, -1: none
-                const int64_t pos = static_cast<int64_t>(w.tile_lo + j) * kTile + lane * 16;
-                if (lane >= kGroups || j >= n || pos >= w.len) return -1;
-                return __ldg(table + pos / a.c.page_size);
+                const int64_t pos = place(j);
+                return pos < 0 ? -1 : __ldg(table + pos / a.c.page_size);
             };
             auto row_of = [&](int j, int page) -> int {
-                const int64_t pos = static_cast<int64_t>(w.tile_lo + j) * kTile + lane * 16;
-                if (lane >= kGroups || j >= n || pos >= w.len) return -1;
+                const int64_t pos = place(j);
+                if (pos < 0) return -1;
                 if (page < 0 || page >= a.c.num_pages) {
                     record_device_error(a.err, kDevBadPage);
                     return -1;
@@ -317,7 +330,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
             int row = row_of(0, entry(0));
             float ks = row >= 0 ? __ldg(a.c.k_scale + row / a.c.scale_block) : 0.0f, vs = row >= 0 ? __ldg(a.c.v_scale + row / a.c.scale_block) : 1.0f;
             int next_page = entry(1);
-            const int groups_per_box = box_rows / 16;
             int issued = 0;
             for (int j = 0; j < n; ++j) {
                 const int later_page = entry(j + 2);
@@ -430,13 +442,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
         auto fetch = [&](int j) -> bool {
             const int st = j % kInfoStages;
             if (!__all_sync(0xffffffffu, mbar_wait(&sh.info_full[st], (j / kInfoStages) & 1, a.err, kDevTimeoutProducer))) return false;
-            const int64_t base = static_cast<int64_t>(w.tile_lo + j) * kTile;
+            const int64_t base = static_cast<int64_t>(w.tile(j)) * kTile;
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
                 const int tok = tok0 + i * kRowsPer;
                 const int row = sh.info[st][tok >> 4].row;
                 codes[i] = make_uint4(0, 0, 0, 0);
-                if (row >= 0 && base + tok < w.len)
+                // with sinks: a slot that no row sees may hold NaN, which would cost a pass over the cache
+                if (row >= 0 && base + tok < w.len && (!SINKS || (base + tok <= w.hi && (base + tok >= w.lo || base + tok < sinks))))
                     codes[i] = __ldg(reinterpret_cast<const uint4 *>(a.c.v + (static_cast<int64_t>(row) + (tok & 15)) * D) + ch);
             }
             __syncwarp();
@@ -449,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
             ok = __all_sync(0xffffffffu, mbar_wait(&sh.v_empty[vst], ((j / kVStages) & 1) ^ 1, a.err, kDevTimeoutProducer));
             if (!ok) break;
             const uint32_t vb = smem + S::kOffV + vst * S::kV;
-            const int base = (w.tile_lo + j) * kTile;
+            const int base = w.tile(j) * kTile;
             uint32_t nan = 0;
             if (base < all_lo || base + kTile - 1 > all_hi) {  // elsewhere a NaN reaches only rows that see it
 #pragma unroll
@@ -571,8 +584,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tc_fence_after();
-                const int base = (w.tile_lo + j) * kTile;
-                const bool plain = !CAP && __all_sync(0xffffffffu, first <= base && last >= base + kTile - 1);
+                const int base = w.tile(j) * kTile;
+                const bool plain = !CAP && __all_sync(0xffffffffu, (first <= base || (SINKS && base + kTile <= sinks)) && last >= base + kTile - 1);
                 const GroupInfo *info = sh.info[st];
                 uint32_t sr[2][32], p[64];
                 // Weights of the tile against the reference maximum, 32 scores
@@ -638,7 +651,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
                             const int k = base + q * 32 + e;
                             const float x = __uint_as_float(r[e]), f = gi.x * factor;
                             const float y = CAP ? cap_score(x, f, a.cap) + gi.y : fmaf(x, f, gi.y);
-                            r[e] = __float_as_uint(k >= first && k <= last ? y : -INFINITY);
+                            r[e] = __float_as_uint((k >= first || (SINKS && k < sinks)) && k <= last ? y : -INFINITY);
                         }
                         top = max3(top, max16(r), max16(r + 16));
                         tmem_st_32x32b_x32(ts + q * 32, r);
@@ -740,7 +753,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
         const int32_t *table = a.b.block_table + w.seq * a.b.table_stride;
         uint16_t *out = static_cast<uint16_t *>(a.out) + (w.t0 + static_cast<int64_t>(row / a.group)) * a.out_token_stride +
                         (w.head * a.group + row % a.group) * a.out_head_stride;
-        for (int k = first; k <= last; ++k) {
+        for (int k = min(first, sinks) > 0 ? 0 : first; k <= last; ++k) {
+            if (SINKS && k == sinks && k < first) k = first;
             const int64_t page = __ldg(table + k / a.c.page_size);
             if (page < 0 || page >= a.c.num_pages) continue;
             const uint32_t *v = reinterpret_cast<const uint32_t *>(a.c.v + ((page * a.c.kv_heads + w.head) * a.c.page_size + k % a.c.page_size) * D);
@@ -791,7 +805,8 @@ int launch_tc(const lcml_kv_attention_desc *d, const AttnArgs &a, int min_rows, 
                           D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return set_error(LCML_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
-    auto kern = k_kv_attention_tc<D, NP, CAP>;
+    // without sinks two prompts of 4096 take 232 us, with their tests in the kernel 240
+    auto kern = a.sinks > 0 ? k_kv_attention_tc<D, NP, CAP, true> : k_kv_attention_tc<D, NP, CAP, false>;
     const int rc = ensure_max_smem(reinterpret_cast<const void *>(kern), S::kSmem, "kv_attention_tc");
     if (rc != LCML_OK) return rc;
     const int64_t units = (d->batch->total_tokens * a.group / kBlockRows + d->batch->batch) * d->cache->kv_heads;

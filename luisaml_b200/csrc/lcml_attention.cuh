@@ -19,6 +19,7 @@ struct AttnArgs {
     int window, causal;
     int64_t max_tokens;
     int *err;
+    int sinks;  // first positions that stay visible behind the window (0 without one)
 };
 
 constexpr float kLog2e = 1.4426950408889634f;

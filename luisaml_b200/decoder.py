@@ -1,7 +1,9 @@
 """The operators of a decoder layer around the FP8 GEMMs, over the C ABI of
 ``include/lcml_decoder.h``: RMS norm with the residual's addition and an e4m3
 output, the paged e4m3 key/value cache (quantizing write, read back) and the
-attention over it.
+attention over it; and what a step needs beside them (``include/lcml_decode_step.h``):
+the plan of a ragged batch from request lengths, the norm and rotation of queries
+and keys, attention with sinks, the sampling of the next token.
 
 All of them take CUDA tensors, enqueue on torch's current stream of the
 tensors' device and neither synchronise nor read lengths back: the lengths of a
@@ -24,6 +26,7 @@ cu_tokens[b + 1] - 1) and a length per sequence.
 from __future__ import annotations
 
 import os
+import typing
 
 import torch
 
@@ -70,20 +73,74 @@ def kv_attention_workspace_size(q, k_cache, v_cache, k_scale, v_scale, block_tab
                                 max_tokens=None, window=0, variant=0):
     """Bytes of scratch the same call of :func:`kv_attention` needs (0: none)."""
     return _bind.kv_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_tokens, kv_len, max_tokens, None,
-                              True, window, 0.0, None, None, None, variant, True)
+                              True, window, 0.0, None, None, None, variant, True, 0)
 
 
 def kv_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_tokens, kv_len, *, max_tokens=None, scale=None,
-                 causal=True, window=0, softcap=0.0, out=None, lse=None, workspace=None, variant=0):
+                 causal=True, window=0, softcap=0.0, out=None, lse=None, workspace=None, variant=0, sinks=0):
     """Attention of the packed queries ``q`` [tokens, q_heads, head_dim] (float16 or bfloat16)
     over the cache; returns ``out`` of q's shape and type.
 
     Sequence b holds ``kv_len[b]`` tokens, its queries the last of them (written before this
     call). ``max_tokens``: an upper bound of one sequence's queries, known on the host (default:
     all of q's). ``scale``: 1 / sqrt(head_dim) by default; ``window``: how many positions up to
-    its own a query sees (0: all); ``softcap``: scores become softcap * tanh(score / softcap).
+    its own a query sees (0: all), ``sinks``: how many first positions it sees besides (the pages
+    between are not looked at: their table entries may be anything); ``softcap``: scores become softcap * tanh(score / softcap).
     A query that sees nothing gets zeros. ``lse``: optional float32 [tokens, q_heads] output.
     ``workspace``: scratch of :func:`kv_attention_workspace_size` bytes (default: allocated).
     """
     return _bind.kv_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_tokens, kv_len, max_tokens, scale,
-                              causal, window, softcap, out, lse, workspace, variant, False)
+                              causal, window, softcap, out, lse, workspace, variant, False, sinks)
+
+
+class KvPlan(typing.NamedTuple):
+    """What :func:`kv_plan` returns: int32 tensors on the batch's device."""
+    cu_tokens: torch.Tensor   # [batch + 1]
+    start: torch.Tensor       # [batch]: tokens each row holds before the step (start of kv_cache_write)
+    kv_len: torch.Tensor      # [batch]: and after it (kv_len of kv_attention)
+    positions: torch.Tensor   # [total]: each packed token's position, -1 past the last one
+    slots: torch.Tensor       # [total]: page * page_size + slot, -1 where it has none
+    free_count: torch.Tensor  # [1]: pages left on the free list
+
+
+def kv_plan(new_tokens, held, block_table, free_pages, free_count, *, page_size, total, ended=None, kv_len=None, free_count_out=None):
+    """Plans a step of a ragged batch on the device: row b holds ``held[b]`` tokens and brings
+    ``new_tokens[b]`` more (int32 [batch]).
+
+    Takes the pages that the new tokens need from the end of the free list (``free_pages`` int32
+    [capacity], of which the first ``free_count`` [1] are free) and enters them into ``block_table``,
+    in place. ``ended`` (bool [batch]): rows whose request is over; their pages go back onto the
+    list first and ``new_tokens`` is the row's new request's. ``total``: length of the packed maps, at
+    least the batch's new tokens. ``kv_len`` and ``free_count_out``: outputs, which may be ``held`` and
+    ``free_count`` themselves, so that a captured step moves on with each replay.
+    Returns a :class:`KvPlan`. An empty free list shows in :func:`luisaml_b200.device_error` as 8,
+    lengths that do not fit as 7; what has no page gets -1 and is never followed.
+    """
+    return KvPlan(*_bind.kv_plan(new_tokens, held, block_table, free_pages, free_count, ended, page_size, total, kv_len, free_count_out))
+
+
+def qk_norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, *, eps=1e-6, interleaved=False, q_out=None, k_out=None):
+    """RMS norm of every head of ``q`` and ``k`` [tokens, heads, head_dim] (float32, float16 or bfloat16;
+    tokens and heads may be strided), then their rotation by ``positions`` (int32 [tokens]; a token of
+    negative position is not touched).
+
+    ``inv_freq`` (float64 or float32 [rotary / 2]): radians per position of each pair of the first rotary
+    elements, (i, i + rotary / 2) or, ``interleaved``, (2 i, 2 i + 1). ``q_weight``, ``k_weight`` [head_dim], q's type or
+    float32; None: no norm. head_dim is even and at most 512. Returns (q_out, k_out), new tensors by
+    default; they may be ``q`` and ``k`` themselves.
+    """
+    return _bind.qk_norm_rope(q, k, positions, inv_freq, q_weight, k_weight, eps, interleaved, q_out, k_out)
+
+
+def sample(logits, uniform, *, temperature=None, top_k=None, top_p=None, min_p=None, out=None, logprob=None):
+    """Draws a token of every row of ``logits`` [rows, vocab] (float32, float16 or bfloat16) with the numbers
+    ``uniform`` (float32 [rows], in [0, 1)); returns int32 [rows].
+
+    Parameters are tensors of one value a row: ``temperature`` (0: the largest logit), ``top_k`` int32 (0: all),
+    ``top_p`` of what top_k keeps (1: all), ``min_p`` of the largest probability (0: all). The draw is among the
+    tokens that all of them keep, equal logits in the order of their indices, and takes the lowest index at
+    which their probabilities, summed by rising index, pass ``uniform``. Probabilities are held in 64 bits and
+    the order of every sum is fixed: equal inputs give equal tokens. ``logprob``: optional float32 [rows]
+    output, the log of the token's probability among the kept ones. A row of -infinity alone gives -1.
+    """
+    return _bind.sample(logits, uniform, temperature, top_k, top_p, min_p, out, logprob)

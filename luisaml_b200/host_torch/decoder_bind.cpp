@@ -1,4 +1,4 @@
-// Python binding of include/lcml_decoder.h for torch tensors
+// Python binding of include/lcml_decoder.h and include/lcml_decode_step.h for torch tensors
 // (luisaml_b200._decoder_bind, called by luisaml_b200/decoder.py).
 //
 // A decode step's kernels take a few microseconds; reading shapes, strides and
@@ -19,7 +19,7 @@
 
 #include <string>
 
-#include "lcml_decoder.h"
+#include "lcml_decode_step.h"
 
 namespace {
 
@@ -262,7 +262,7 @@ PyObject *kv_cache_read(PyObject *const *o) {
 }
 
 // kv_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, cu_tokens, kv_len, max_tokens, scale, causal, window, softcap, out, lse,
-//              workspace, variant, size_only)
+//              workspace, variant, size_only, sinks)
 PyObject *kv_attention(PyObject *const *o) {
     const at::Tensor &q = tensor(o[0], "q"), &kc = tensor(o[1], "k_cache"), &vc = tensor(o[2], "v_cache"), &ks = tensor(o[3], "k_scale"),
                      &vs = tensor(o[4], "v_scale"), &table = tensor(o[5], "block_table"), &cu = tensor(o[6], "cu_tokens"), &len = tensor(o[7], "kv_len");
@@ -290,6 +290,8 @@ PyObject *kv_attention(PyObject *const *o) {
     d.window = static_cast<int32_t>(window);
     d.softcap = static_cast<float>(number(o[12]));
     d.variant = static_cast<int>(integer(o[16]));
+    const int64_t sinks = integer(o[18]);
+    need(sinks >= 0 && sinks <= INT32_MAX, "kv_attention: sinks is negative or exceeds 32 bits");
     c10::cuda::CUDAGuard guard(dev);
     const int64_t bytes = lcml_kv_attention_workspace_size(&d);
     if (bytes < 0) throw Failed{LCML_ERR_INVALID_ARGUMENT};
@@ -317,8 +319,168 @@ PyObject *kv_attention(PyObject *const *o) {
         need(ws->is_contiguous() && static_cast<int64_t>(ws->nbytes()) >= bytes, "kv_attention: the workspace is too small");
         d.workspace = ws->data_ptr();
     }
-    check(lcml_kv_attention(&d, stream_of(dev)));
+    check(lcml_kv_attention_sinks(&d, static_cast<int32_t>(sinks), stream_of(dev)));
     return made.defined() ? wrap(made) : same(o[13]);
+}
+
+// An int32 output of n values: the one given, or a new one.
+at::Tensor int_output(const at::Tensor *given, int64_t n, c10::Device dev, const char *what) {
+    if (given == nullptr) return empty({n}, at::kInt, dev);
+    need(given->dim() == 1 && given->size(0) == n && given->scalar_type() == at::kInt && given->is_contiguous(), what);
+    return *given;
+}
+
+// kv_plan(new_tokens, held, block_table, free_pages, free_count, ended, page_size, total, kv_len, free_count_out)
+// -> (cu_tokens, start, kv_len, positions, slots, free_count)
+PyObject *kv_plan(PyObject *const *o) {
+    const at::Tensor &fresh = tensor(o[0], "new_tokens"), &held = tensor(o[1], "held"), &table = tensor(o[2], "block_table"), &free = tensor(o[3], "free_pages"),
+                     &count = tensor(o[4], "free_count");
+    const at::Tensor *ended = maybe(o[5], "ended"), *len_out = maybe(o[8], "kv_len"), *count_out = maybe(o[9], "free_count_out");
+    const c10::Device dev = device_of(fresh, &held, &table, &free, &count, ended, len_out, count_out);
+    const int64_t page_size = integer(o[6]), total = integer(o[7]), batch = fresh.dim() == 1 ? fresh.size(0) : -1;
+    need(batch >= 0 && fresh.scalar_type() == at::kInt && held.scalar_type() == at::kInt && held.dim() == 1 && held.size(0) == batch && fresh.is_contiguous() &&
+             held.is_contiguous(),
+         "kv_plan: new_tokens and held are int32 [batch], contiguous");
+    need(table.scalar_type() == at::kInt && table.dim() == 2 && table.size(0) == batch && (table.size(1) <= 1 || table.stride(1) == 1) &&
+             (batch <= 1 || table.stride(0) >= table.size(1)),
+         "kv_plan: block_table is int32 [batch, columns] with contiguous rows");
+    need(free.scalar_type() == at::kInt && free.dim() == 1 && free.is_contiguous() && count.scalar_type() == at::kInt && count.numel() == 1,
+         "kv_plan: free_pages is int32 [pages], contiguous, and free_count one int32");
+    need(ended == nullptr || ((ended->scalar_type() == at::kBool || ended->scalar_type() == at::kByte) && ended->dim() == 1 && ended->size(0) == batch && ended->is_contiguous()),
+         "kv_plan: ended is bool or uint8 [batch], contiguous");
+    need(page_size > 0 && page_size <= INT32_MAX && total >= 0 && table.size(1) <= INT32_MAX && batch <= INT32_MAX, "kv_plan: an extent is negative or exceeds 32 bits");
+    c10::cuda::CUDAGuard guard(dev);
+    const at::Tensor cu = empty({batch + 1}, at::kInt, dev), start = empty({batch}, at::kInt, dev), positions = empty({total}, at::kInt, dev),
+                     slots = empty({total}, at::kInt, dev);
+    const at::Tensor len = int_output(len_out, batch, dev, "kv_plan: kv_len is int32 [batch], contiguous"),
+                     left = int_output(count_out, 1, dev, "kv_plan: free_count_out is int32 [1]");
+    lcml_kv_plan_desc d{};
+    d.batch = static_cast<int32_t>(batch);
+    d.page_size = static_cast<int32_t>(page_size);
+    d.table_cols = static_cast<int32_t>(table.size(1));
+    d.table_stride = batch > 1 ? table.stride(0) : table.size(1);
+    d.block_table = static_cast<int32_t *>(table.data_ptr());
+    d.new_tokens = static_cast<const int32_t *>(fresh.data_ptr());
+    d.held = static_cast<const int32_t *>(held.data_ptr());
+    d.ended = ended ? static_cast<const uint8_t *>(ended->data_ptr()) : nullptr;
+    d.free_pages = static_cast<int32_t *>(free.data_ptr());
+    d.free_capacity = free.size(0);
+    d.free_count = static_cast<const int32_t *>(count.data_ptr());
+    d.total_tokens = total;
+    d.cu_tokens = static_cast<int32_t *>(cu.data_ptr());
+    d.start = static_cast<int32_t *>(start.data_ptr());
+    d.kv_len = static_cast<int32_t *>(len.data_ptr());
+    d.positions = static_cast<int32_t *>(positions.data_ptr());
+    d.slots = static_cast<int32_t *>(slots.data_ptr());
+    d.free_count_out = static_cast<int32_t *>(left.data_ptr());
+    check(lcml_kv_plan(&d, stream_of(dev)));
+    const at::Tensor *out[6] = {&cu, &start, &len, &positions, &slots, &left};
+    PyObject *t = PyTuple_New(6);
+    if (t == nullptr) throw Raised{};
+    for (int i = 0; i < 6; ++i) {
+        PyObject *x = i == 2 && len_out ? same(o[8]) : (i == 5 && count_out ? same(o[9]) : THPVariable_Wrap(*out[i]));
+        if (x == nullptr) {
+            Py_DECREF(t);
+            throw Raised{};
+        }
+        PyTuple_SET_ITEM(t, i, x);
+    }
+    return t;
+}
+
+// qk_norm_rope(q, k, positions, inv_freq, q_weight, k_weight, eps, interleaved, q_out, k_out) -> (q_out, k_out)
+PyObject *qk_norm_rope(PyObject *const *o) {
+    const at::Tensor &q = tensor(o[0], "q"), &k = tensor(o[1], "k"), &pos = tensor(o[2], "positions"), &freq = tensor(o[3], "inv_freq");
+    const at::Tensor *qw = maybe(o[4], "q_weight"), *kw = maybe(o[5], "k_weight"), *q_out = maybe(o[8], "q_out"), *k_out = maybe(o[9], "k_out");
+    no_gradient(&q, &k, &freq, qw, kw);
+    const c10::Device dev = device_of(q, &k, &pos, &freq, qw, kw, q_out, k_out);
+    lcml_qk_norm_rope_desc d{};
+    d.dtype = dtype_of(q, "q");
+    need(q.dim() == 3 && k.dim() == 3 && q.size(0) == k.size(0) && q.size(2) == k.size(2) && q.scalar_type() == k.scalar_type() && q.size(1) <= INT32_MAX &&
+             k.size(1) <= INT32_MAX && q.size(2) <= INT32_MAX,
+         "qk_norm_rope: q and k are [tokens, heads, head_dim] of one type");
+    const int64_t dim = q.size(2);
+    need(pos.scalar_type() == at::kInt && pos.dim() == 1 && pos.size(0) == q.size(0) && pos.is_contiguous(), "qk_norm_rope: positions is int32 [tokens], contiguous");
+    need((freq.scalar_type() == at::kFloat || freq.scalar_type() == at::kDouble) && freq.dim() == 1 && freq.is_contiguous() && freq.size(0) <= dim / 2,
+         "qk_norm_rope: inv_freq is float32 or float64 [rotary / 2], contiguous, rotary at most head_dim");
+    d.weight_dtype = LCML_DTYPE_FLOAT;
+    for (const at::Tensor *w : {qw, kw}) {
+        if (w == nullptr) continue;
+        need(w->dim() == 1 && w->size(0) == dim && w->is_contiguous() && (w->scalar_type() == q.scalar_type() || w->scalar_type() == at::kFloat),
+             "qk_norm_rope: q_weight and k_weight are [head_dim], contiguous, of q's type or float32");
+        d.weight_dtype = dtype_of(*w, "weight");
+    }
+    need(qw == nullptr || kw == nullptr || qw->scalar_type() == kw->scalar_type(), "qk_norm_rope: q_weight and k_weight have one type");
+    c10::cuda::CUDAGuard guard(dev);
+    at::Tensor made_q, made_k;
+    if (!q_out) {
+        made_q = empty(q.sizes(), q.scalar_type(), dev);
+        q_out = &made_q;
+    }
+    if (!k_out) {
+        made_k = empty(k.sizes(), k.scalar_type(), dev);
+        k_out = &made_k;
+    }
+    need(q_out->sizes() == q.sizes() && q_out->scalar_type() == q.scalar_type() && k_out->sizes() == k.sizes() && k_out->scalar_type() == k.scalar_type(),
+         "qk_norm_rope: q_out and k_out have the shape and type of q and k");
+    for (const at::Tensor *t : {&q, &k, q_out, k_out}) need(dim <= 1 || t->stride(2) == 1, "qk_norm_rope: heads are contiguous");
+    d.tokens = q.size(0);
+    d.q_heads = static_cast<int32_t>(q.size(1));
+    d.k_heads = static_cast<int32_t>(k.size(1));
+    d.head_dim = static_cast<int32_t>(dim);
+    d.rotary = static_cast<int32_t>(2 * freq.size(0));
+    d.interleaved = truth(o[7]);
+    d.q = q.data_ptr();
+    d.k = k.data_ptr();
+    d.q_token_stride = q.stride(0), d.q_head_stride = q.stride(1), d.k_token_stride = k.stride(0), d.k_head_stride = k.stride(1);
+    d.q_out = q_out->data_ptr();
+    d.k_out = k_out->data_ptr();
+    d.q_out_token_stride = q_out->stride(0), d.q_out_head_stride = q_out->stride(1), d.k_out_token_stride = k_out->stride(0), d.k_out_head_stride = k_out->stride(1);
+    d.q_weight = qw ? qw->data_ptr() : nullptr;
+    d.k_weight = kw ? kw->data_ptr() : nullptr;
+    d.eps = static_cast<float>(number(o[6]));
+    d.positions = static_cast<const int32_t *>(pos.data_ptr());
+    d.inv_freq = freq.data_ptr();
+    d.inv_freq_dtype = freq.scalar_type() == at::kDouble ? LCML_DTYPE_DOUBLE : LCML_DTYPE_FLOAT;
+    check(lcml_qk_norm_rope(&d, stream_of(dev)));
+    PyObject *a = made_q.defined() ? wrap(made_q) : same(o[8]), *b = made_k.defined() ? wrap(made_k) : same(o[9]);
+    PyObject *t = PyTuple_New(2);
+    PyTuple_SET_ITEM(t, 0, a);
+    PyTuple_SET_ITEM(t, 1, b);
+    return t;
+}
+
+// sample(logits, uniform, temperature, top_k, top_p, min_p, out, logprob) -> tokens
+PyObject *sample(PyObject *const *o) {
+    const at::Tensor &x = tensor(o[0], "logits"), &u = tensor(o[1], "uniform");
+    const at::Tensor *t = maybe(o[2], "temperature"), *k = maybe(o[3], "top_k"), *p = maybe(o[4], "top_p"), *m = maybe(o[5], "min_p"), *out = maybe(o[6], "out"),
+                     *lp = maybe(o[7], "logprob");
+    no_gradient(&x, &u, t, p, m);
+    const c10::Device dev = device_of(x, &u, t, k, p, m, out, lp);
+    lcml_sample_desc d{};
+    d.dtype = dtype_of(x, "logits");
+    need(x.dim() == 2, "sample: logits is [rows, vocab]");
+    const int64_t rows = x.size(0);
+    need((x.size(1) <= 1 || x.stride(1) == 1) && (rows <= 1 || x.stride(0) >= x.size(1)), "sample: rows of logits are contiguous and do not overlap");
+    auto row_values = [&](const at::Tensor *v, at::ScalarType type, const char *what) {
+        need(v == nullptr || (v->dim() == 1 && v->size(0) == rows && v->scalar_type() == type && v->is_contiguous()), what);
+        return v == nullptr ? nullptr : v->data_ptr();
+    };
+    d.rows = rows;
+    d.vocab = x.size(1);
+    d.logits = x.data_ptr();
+    d.ld = rows > 1 ? x.stride(0) : x.size(1);
+    d.uniform = static_cast<const float *>(row_values(&u, at::kFloat, "sample: uniform is float32 [rows], contiguous"));
+    d.temperature = static_cast<const float *>(row_values(t, at::kFloat, "sample: temperature is float32 [rows], contiguous"));
+    d.top_k = static_cast<const int32_t *>(row_values(k, at::kInt, "sample: top_k is int32 [rows], contiguous"));
+    d.top_p = static_cast<const float *>(row_values(p, at::kFloat, "sample: top_p is float32 [rows], contiguous"));
+    d.min_p = static_cast<const float *>(row_values(m, at::kFloat, "sample: min_p is float32 [rows], contiguous"));
+    d.logprob = static_cast<float *>(row_values(lp, at::kFloat, "sample: logprob is float32 [rows], contiguous"));
+    c10::cuda::CUDAGuard guard(dev);
+    const at::Tensor tokens = int_output(out, rows, dev, "sample: out is int32 [rows], contiguous");
+    d.tokens = static_cast<int32_t *>(tokens.data_ptr());
+    check(lcml_sample(&d, stream_of(dev)));
+    return out ? same(o[6]) : wrap(tokens);
 }
 
 // Runs F on exactly N positional arguments; every error becomes a Python one.
@@ -360,11 +522,14 @@ PyMethodDef methods[] = {
     {"rmsnorm_quantize", fast<rmsnorm_quantize, 8>(), METH_FASTCALL, nullptr},
     {"kv_cache_write", fast<kv_cache_write, 9>(), METH_FASTCALL, nullptr},
     {"kv_cache_read", fast<kv_cache_read, 9>(), METH_FASTCALL, nullptr},
-    {"kv_attention", fast<kv_attention, 18>(), METH_FASTCALL, nullptr},
+    {"kv_attention", fast<kv_attention, 19>(), METH_FASTCALL, nullptr},
+    {"kv_plan", fast<kv_plan, 10>(), METH_FASTCALL, nullptr},
+    {"qk_norm_rope", fast<qk_norm_rope, 10>(), METH_FASTCALL, nullptr},
+    {"sample", fast<sample, 8>(), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 
-PyModuleDef module = {PyModuleDef_HEAD_INIT, "_decoder_bind", "Binding of lcml_decoder.h for torch tensors.", -1, methods, nullptr, nullptr, nullptr, nullptr};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_decoder_bind", "Binding of lcml_decoder.h and lcml_decode_step.h for torch tensors.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }// namespace
 
