@@ -19,31 +19,52 @@ namespace {
 
 constexpr int kDevNoPages = 8;  // joins the codes of DeviceError: the free list ran out
 constexpr int kMaxRows = 16384;
-constexpr int kThreads = 1024;
+constexpr int kThreads = 1024;  // at most
 constexpr int kWarps = kThreads / 32;
 constexpr int kCluster = 8;
+constexpr unsigned kAll = 0xffffffffu;
 
-__device__ __forceinline__ int64_t add_up(int64_t v, int lane) {  // inclusive sums of a warp
+// Exclusive sums of two values a thread over the block; the totals are added to `tokens` and `entries`.
+struct Scan {
+    int64_t tokens[kWarps];
+    int32_t entries[kWarps];
+};
+__device__ __forceinline__ void block_scan(Scan &sh, int64_t &a, int32_t &b, int64_t &tokens, int32_t &entries) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    int64_t x = a;
+    int32_t y = b;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int64_t x = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += x;
+        const int64_t p = __shfl_up_sync(kAll, x, o);
+        const int32_t q = __shfl_up_sync(kAll, y, o);
+        if (lane >= o) {
+            x += p;
+            y += q;
+        }
     }
-    return v;
-}
-
-// Exclusive sums of one value a thread over the block; `total` gets the block's.
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t *warp_sums, int64_t &total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t incl = add_up(v, lane);
-    if (lane == 31) warp_sums[warp] = incl;
+    if (lane == 31) {
+        sh.tokens[warp] = x;
+        sh.entries[warp] = y;
+    }
     __syncthreads();
-    const int64_t of = lane < (blockDim.x >> 5) ? warp_sums[lane] : 0;
-    const int64_t upto = add_up(of, lane);
-    total = __shfl_sync(0xffffffffu, upto, 31);
-    const int64_t before = __shfl_sync(0xffffffffu, upto - of, warp);
+    // every warp sums the warps' sums
+    int64_t before = lane < warps ? sh.tokens[lane] : 0, all = before;
+    int32_t before_e = lane < warps ? sh.entries[lane] : 0;
+    const int32_t all_e = __reduce_add_sync(kAll, before_e);
+    before = lane < warp ? before : 0;
+    before_e = __reduce_add_sync(kAll, lane < warp ? before_e : 0);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        before += __shfl_xor_sync(kAll, before, o);
+        all += __shfl_xor_sync(kAll, all, o);
+    }
+    before += tokens;
+    before_e += entries;
     __syncthreads();
-    return before + incl - v;
+    a = before + x - a;
+    b = before_e + y - b;
+    tokens += all;
+    entries += all_e;
 }
 
 // The last i in [0, n) with first[i] <= x; first[0] <= x, not decreasing.
@@ -59,16 +80,17 @@ __device__ __forceinline__ int last_at_or_below(const int32_t *first, int n, int
 
 __global__ void __launch_bounds__(kThreads) k_kv_plan(lcml_kv_plan_desc a, int *err) {
     extern __shared__ int32_t smem[];
-    __shared__ int64_t warp_sums[kWarps];
+    __shared__ Scan scan;
     const int batch = a.batch;
-    int32_t *cu = smem;                    // [batch + 1]
-    int32_t *shift = smem + batch + 1;     // [batch]: a token's position less its packed index
-    int32_t *pages = shift + batch;        // [batch + 1]: new entries of the rows before; at first, pages given back
+    int32_t *cu = smem;                  // [batch + 1]
+    int32_t *shift = smem + batch + 1;   // [batch]: a token's position less its packed index
+    int32_t *pages = shift + batch;      // [batch + 1]: new entries of the rows before; at first, pages given back
     const int lane = threadIdx.x & 31;
     const int ctas = gridDim.x, rank = blockIdx.x;
     const int stride = ctas * blockDim.x, me = rank * blockDim.x + threadIdx.x;
-    const int ps = a.page_size;
+    const uint32_t ps = a.page_size;
     const int64_t reach = static_cast<int64_t>(a.table_cols) * ps;
+    const int total = static_cast<int>(a.total_tokens);
     bool bad = false;
 
     griddep_launch_dependents();
@@ -78,8 +100,8 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(lcml_kv_plan_desc a, int *
     int64_t count = listed < 0 ? 0 : (listed < capacity ? listed : capacity);
     bad |= count != listed;
 
-    auto columns = [&](int64_t tokens) -> int {  // columns of the table that hold this many
-        return static_cast<int>(tokens < reach ? (tokens + ps - 1) / ps : a.table_cols);
+    auto columns = [&](int tokens) -> int {  // columns of the table that hold this many (>= 0)
+        return static_cast<int>(min((static_cast<uint32_t>(tokens) + ps - 1) / ps, static_cast<uint32_t>(a.table_cols)));
     };
     if (a.ended != nullptr) {
         // a warp per row, the rows dealt to the cluster's warps; a count goes to every CTA
@@ -87,10 +109,13 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(lcml_kv_plan_desc a, int *
         const int warps = stride >> 5, w = me >> 5;
         cluster_sync_all();  // every CTA has started
         for (int b = w; b < batch; b += warps) {
+            const int held = a.held[b];
             int n = 0;
             if (a.ended[b] != 0) {
-                const int cols = columns(max(0, a.held[b]));
-                for (int c0 = 0; c0 < cols; c0 += 32) n += __popc(__ballot_sync(0xffffffffu, row_entry(b, c0 + lane, cols) >= 0));
+                const int cols = columns(max(0, held));
+#pragma unroll 4
+                for (int c0 = 0; c0 < cols; c0 += 32) n += row_entry(b, c0 + lane, cols) >= 0;
+                n = __reduce_add_sync(kAll, n);
             }
             if (lane < ctas) {
                 const uint32_t to = mapa_shared(smem_u32(pages + b), lane);
@@ -98,22 +123,24 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(lcml_kv_plan_desc a, int *
             }
         }
         cluster_sync_all();
-        int64_t back = 0;
+        int64_t unused = 0;
+        int32_t back = 0;
         for (int b0 = 0; b0 < batch; b0 += blockDim.x) {
             const int b = b0 + threadIdx.x;
-            int64_t sum;
-            const int64_t before = block_scan(b < batch ? pages[b] : 0, warp_sums, sum);
-            if (b < batch) pages[b] = static_cast<int32_t>(back + before);
-            back += sum;
+            int64_t none = 0;
+            int32_t mine = b < batch ? pages[b] : 0;
+            block_scan(scan, none, mine, unused, back);
+            if (b < batch) pages[b] = mine;
         }
         __syncthreads();
         for (int b = w; b < batch; b += warps) {
             if (a.ended[b] == 0) continue;
             const int cols = columns(max(0, a.held[b]));
             int64_t at = count + pages[b];
+#pragma unroll 4
             for (int c0 = 0; c0 < cols; c0 += 32) {
                 const int p = row_entry(b, c0 + lane, cols);
-                const uint32_t have = __ballot_sync(0xffffffffu, p >= 0);
+                const uint32_t have = __ballot_sync(kAll, p >= 0);
                 const int64_t to = at + __popc(have & ((1u << lane) - 1));
                 if (p >= 0) {
                     if (to < capacity) a.free_pages[to] = p;
@@ -127,69 +154,95 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(lcml_kv_plan_desc a, int *
         cluster_sync_all();  // the free list is complete, and `pages` may be written again
     }
 
-    // sums of the tokens and of the new entries
-    int64_t tokens = 0, taken = 0;
-    for (int b0 = 0; b0 < batch; b0 += blockDim.x) {
-        const int b = b0 + threadIdx.x;
-        int n = 0, start = 0;
-        if (b < batch) {
-            n = a.new_tokens[b];
-            start = a.held[b];
-            bad |= n < 0 || start < 0;
-            n = max(n, 0);
-            start = a.ended != nullptr && a.ended[b] != 0 ? 0 : max(start, 0);
+    // Sums of the tokens and of the new entries; these again where tokens are left out.
+    int64_t tokens = 0;
+    int32_t taken = 0;
+    for (int turn = 0; turn < 2; ++turn) {
+        const int64_t limit = turn == 0 ? INT64_MAX : total;
+        tokens = 0;
+        taken = 0;
+        for (int b0 = 0; b0 < batch; b0 += blockDim.x) {
+            const int b = b0 + threadIdx.x;
+            int n = 0, start = 0;
+            if (b < batch) {
+                n = a.new_tokens[b];
+                start = a.held[b];
+                bad |= n < 0 || start < 0;
+                n = max(n, 0);
+                start = a.ended != nullptr && a.ended[b] != 0 ? 0 : max(start, 0);
+            }
+            int64_t first = n;
+            if (turn == 1) n = static_cast<int>(min(static_cast<int64_t>(cu[b < batch ? b : 0]) + n, limit) - cu[b < batch ? b : 0]);  // cu: of turn 0
+            const int64_t len = min(static_cast<int64_t>(start) + n, static_cast<int64_t>(0x7fffffff));
+            bad |= b < batch && len > reach;
+            int32_t entries = b < batch ? columns(static_cast<int>(len)) - columns(start) : 0;
+            block_scan(scan, first, entries, tokens, taken);
+            if (b < batch) {
+                cu[b] = static_cast<int32_t>(min(first, static_cast<int64_t>(total)));
+                shift[b] = start - cu[b];
+                pages[b] = entries;
+            }
         }
-        int64_t sum;
-        const int64_t first = tokens + block_scan(n, warp_sums, sum);
-        tokens += sum;
-        const int from = static_cast<int>(min(first, a.total_tokens)), to = static_cast<int>(min(first + n, a.total_tokens));
-        const int64_t len = min(static_cast<int64_t>(start) + (to - from), static_cast<int64_t>(0x7fffffff));
-        bad |= b < batch && (len > reach || to - from < n);
-        const int64_t entries = taken + block_scan(b < batch ? columns(len) - columns(start) : 0, warp_sums, sum);
-        taken += sum;
-        if (b < batch) {
-            cu[b] = from;
-            shift[b] = start - from;
-            pages[b] = static_cast<int32_t>(entries);
-        }
+        if (tokens <= total) break;
+        bad = true;
+        __syncthreads();
     }
-    if (threadIdx.x == 0) {
-        cu[batch] = static_cast<int32_t>(min(tokens, a.total_tokens));
-        pages[batch] = static_cast<int32_t>(taken);
-    }
+    if (threadIdx.x == 0) cu[batch] = static_cast<int32_t>(min(tokens, static_cast<int64_t>(total)));
     if (rank == 0 && bad) record_device_error(err, kDevBadBatch);
-    cluster_sync_all();  // every CTA has read held and free_count: kv_len and free_count_out may be the same memory
+    if (ctas > 1) cluster_sync_all();  // every CTA has read held and free_count: kv_len and free_count_out may be the same memory
+    else __syncthreads();
 
-    auto page_of = [&](int64_t i) -> int { return i < count ? a.free_pages[count - 1 - i] : -1; };
+    auto page_of = [&](int i) -> int { return i < count ? a.free_pages[count - 1 - i] : -1; };
     for (int b = me; b <= batch; b += stride) {
         a.cu_tokens[b] = cu[b];
         if (b < batch) {
-            const int64_t start = static_cast<int64_t>(shift[b]) + cu[b];
-            a.start[b] = static_cast<int32_t>(start);
-            a.kv_len[b] = static_cast<int32_t>(min(start + (cu[b + 1] - cu[b]), static_cast<int64_t>(0x7fffffff)));
+            const int start = shift[b] + cu[b];
+            a.start[b] = start;
+            a.kv_len[b] = static_cast<int32_t>(min(static_cast<int64_t>(start) + (cu[b + 1] - cu[b]), static_cast<int64_t>(0x7fffffff)));
         }
     }
-    for (int64_t i = me; i < taken; i += stride) {
-        const int b = last_at_or_below(pages, batch, static_cast<int>(i));
-        const int col = columns(static_cast<int64_t>(shift[b]) + cu[b]) + static_cast<int>(i - pages[b]);
-        a.block_table[b * a.table_stride + col] = page_of(i);
+    for (int i = me; i < taken; i += stride) {
+        const int b = last_at_or_below(pages, batch, i);
+        a.block_table[b * a.table_stride + columns(shift[b] + cu[b]) + (i - pages[b])] = page_of(i);
     }
+    // four tokens a thread, so that four pages are looked up at once
     const int packed = cu[batch];
-    for (int64_t t = me; t < a.total_tokens; t += stride) {
-        int pos = -1, slot = -1;
-        if (t < packed) {
-            const int b = last_at_or_below(cu, batch, static_cast<int>(t));
-            pos = static_cast<int>(min(static_cast<int64_t>(shift[b]) + t, static_cast<int64_t>(0x7fffffff)));
-            const int col = pos / ps;
-            if (pos < reach) {
-                const int held = columns(static_cast<int64_t>(shift[b]) + cu[b]);
-                const int page = col < held ? a.block_table[b * a.table_stride + col] : page_of(static_cast<int64_t>(pages[b]) + col - held);
-                const int64_t s = static_cast<int64_t>(page) * ps + (pos - col * ps);
-                slot = page >= 0 && s <= 0x7fffffff ? static_cast<int>(s) : -1;
+    const bool vec = aligned(a.positions, 16) && aligned(a.slots, 16);
+    for (int64_t t0 = 4 * static_cast<int64_t>(me); t0 < total; t0 += 4 * static_cast<int64_t>(stride)) {
+        int pos[4], slot[4], b = t0 < packed ? last_at_or_below(cu, batch, static_cast<int>(t0)) : 0;
+        const int32_t *from[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t t = t0 + j;
+            pos[j] = -1;
+            from[j] = nullptr;  // where the token's page is found
+            if (t >= packed) continue;
+            while (cu[b + 1] <= t) ++b;
+            pos[j] = static_cast<int>(min(static_cast<int64_t>(shift[b]) + t, static_cast<int64_t>(0x7fffffff)));
+            if (pos[j] < reach) {
+                const int col = static_cast<int>(static_cast<uint32_t>(pos[j]) / ps), held = columns(shift[b] + cu[b]), i = pages[b] + col - held;
+                if (col < held) from[j] = a.block_table + b * a.table_stride + col;
+                else if (i < count) from[j] = a.free_pages + (count - 1 - i);
             }
         }
-        a.positions[t] = pos;
-        a.slots[t] = slot;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) slot[j] = from[j] != nullptr ? *from[j] : -1;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t s = static_cast<int64_t>(slot[j]) * ps + static_cast<uint32_t>(pos[j]) % ps;
+            slot[j] = slot[j] >= 0 && s <= 0x7fffffff ? static_cast<int>(s) : -1;
+        }
+        if (vec && t0 + 4 <= total) {
+            *reinterpret_cast<int4 *>(a.positions + t0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+            *reinterpret_cast<int4 *>(a.slots + t0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (t0 + j < total) {
+                    a.positions[t0 + j] = pos[j];
+                    a.slots[t0 + j] = slot[j];
+                }
+        }
     }
     if (me == 0) {
         *a.free_count_out = static_cast<int32_t>(max(count - taken, static_cast<int64_t>(0)));
@@ -222,8 +275,12 @@ extern "C" int lcml_kv_plan(const lcml_kv_plan_desc *d, lcml_stream_t stream) {
     const int rc = ensure_max_smem(reinterpret_cast<const void *>(k_kv_plan), (3 * kMaxRows + 2) * 4, "kv_plan");
     if (rc != LCML_OK) return rc;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(kCluster);
-    cfg.blockDim = dim3(kThreads);
+    // One CTA where it has a few rows and tokens a thread, else a cluster of 512 threads each
+    // (rows of 7001 tokens: 7.5 us, with 256 threads 10.5, with 1024 9.0, as clusters of those start later).
+    const int64_t work = d->batch > (d->total_tokens + 3) / 4 ? d->batch : (d->total_tokens + 3) / 4;
+    const bool alone = work <= kThreads && d->ended == nullptr;
+    cfg.gridDim = dim3(alone ? 1 : kCluster);
+    cfg.blockDim = dim3(alone ? (work <= 128 ? 128 : static_cast<unsigned>((work + 31) / 32 * 32)) : 512);
     cfg.dynamicSmemBytes = static_cast<size_t>(smem);
     cfg.stream = to_cuda(stream);
     cudaLaunchAttribute attr[2];

@@ -116,7 +116,7 @@ def kv_plan(new_tokens, held, block_table, free_pages, free_count, *, page_size,
     Returns a :class:`KvPlan`. An empty free list shows in :func:`luisaml_b200.device_error` as 8,
     lengths that do not fit as 7; what has no page gets -1 and is never followed.
     """
-    return KvPlan(*_bind.kv_plan(new_tokens, held, block_table, free_pages, free_count, ended, page_size, total, kv_len, free_count_out))
+    return tuple.__new__(KvPlan, _bind.kv_plan(new_tokens, held, block_table, free_pages, free_count, ended, page_size, total, kv_len, free_count_out))
 
 
 def qk_norm_rope(q, k, positions, inv_freq, q_weight=None, k_weight=None, *, eps=1e-6, interleaved=False, q_out=None, k_out=None):

@@ -350,10 +350,18 @@ PyObject *kv_plan(PyObject *const *o) {
          "kv_plan: ended is bool or uint8 [batch], contiguous");
     need(page_size > 0 && page_size <= INT32_MAX && total >= 0 && table.size(1) <= INT32_MAX && batch <= INT32_MAX, "kv_plan: an extent is negative or exceeds 32 bits");
     c10::cuda::CUDAGuard guard(dev);
-    const at::Tensor cu = empty({batch + 1}, at::kInt, dev), start = empty({batch}, at::kInt, dev), positions = empty({total}, at::kInt, dev),
-                     slots = empty({total}, at::kInt, dev);
-    const at::Tensor len = int_output(len_out, batch, dev, "kv_plan: kv_len is int32 [batch], contiguous"),
-                     left = int_output(count_out, 1, dev, "kv_plan: free_count_out is int32 [1]");
+    // One allocation for all outputs that are not given: views of it cost a tenth of an allocation each.
+    const int64_t row = (batch + 4) / 4 * 4, tokens = (total + 3) / 4 * 4;
+    const at::Tensor all = empty({3 * row + 4 + 2 * tokens}, at::kInt, dev);
+    auto part = [&](int64_t from, int64_t n) {
+        at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), all.dtype());
+        t.unsafeGetTensorImpl()->set_storage_offset(from);
+        t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+        return t;
+    };
+    const at::Tensor cu = part(0, batch + 1), start = part(row, batch), positions = part(3 * row + 4, total), slots = part(3 * row + 4 + tokens, total);
+    const at::Tensor len = len_out ? int_output(len_out, batch, dev, "kv_plan: kv_len is int32 [batch], contiguous") : part(2 * row, batch),
+                     left = count_out ? int_output(count_out, 1, dev, "kv_plan: free_count_out is int32 [1]") : part(3 * row, 1);
     lcml_kv_plan_desc d{};
     d.batch = static_cast<int32_t>(batch);
     d.page_size = static_cast<int32_t>(page_size);
