@@ -20,6 +20,11 @@
 // issue. The MMA order PV_0(j) QK_0(j+1) PV_1(j) QK_1(j+1) lets one tile's
 // softmax run under the other's products.
 //
+// With sinks (SINKS) the key tiles are those over the first positions, then the
+// window's; a box of keys that no row sees is not looked up, its values are zeros.
+// Masked tiles are weighed in one pass there. A unit of a short window is mostly set-up:
+// 54,000 clocks for 6.5 key tiles, of which steady tiles would take 22,000.
+//
 // Bound: the tensor cores (4 head_dim FLOP per visible pair) and the
 // exponentials, 16 a clock per SM: equal at head_dim 128, twice the products'
 // time at 64. Measured at 128 (two prompts of up to 4096, 32 heads over 8, bf16):
@@ -208,6 +213,9 @@ __device__ __forceinline__ float sum16(const float *x) {
     add2(t[0], t[1], t[0], t[1], t[2], t[3]);
     return t[0] + t[1];
 }
+
+// Bits n .. 31.
+__device__ __forceinline__ uint32_t bits_from(int n) { return n <= 0 ? 0xffffffffu : (n >= 32 ? 0u : 0xffffffffu << n); }
 
 // The CTA's work, known to every thread.
 template <bool SINKS>
@@ -592,8 +600,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
                 // at a time and the next 32 on their way. Returns the largest
                 // sum of 16 weights, a bound of each. kRaw: S as the MMA left
                 // it, else in log2 units.
-                auto weights = [&](auto raw, float ref, float &sum) {
-                    constexpr bool kRaw = decltype(raw)::value;
+                // kMasked: with the row's mask.
+                auto weights = [&](auto raw, auto masked, float ref, float &sum) {
+                    constexpr bool kRaw = decltype(raw)::value, kMasked = decltype(masked)::value;
                     float most = 0.0f;
                     tmem_ld_32x32b_x32(ts, sr[0]);
 #pragma unroll
@@ -601,6 +610,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
                         const float4 g0 = *reinterpret_cast<const float4 *>(info + 2 * q), g1 = *reinterpret_cast<const float4 *>(info + 2 * q + 1);
                         tmem_wait_ld();
                         if (q < 3) tmem_ld_32x32b_x32(ts + (q + 1) * 32, sr[(q + 1) & 1]);
+                        // keys of these 32 that the row sees
+                        uint32_t seen = 0;
+                        if constexpr (kMasked) seen = (bits_from(first - base - q * 32) | ~bits_from(sinks - base - q * 32)) & ~bits_from(last + 1 - base - q * 32);
 #pragma unroll
                         for (int g = 0; g < 2; ++g) {
                             const float f = kRaw ? (g ? g1.x : g0.x) * factor : 1.0f, b = (kRaw ? (g ? g1.y : g0.y) : 0.0f) - ref;
@@ -608,7 +620,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
 #pragma unroll
                             for (int e = 0; e < 16; e += 2) {
                                 fma2(x[e], x[e + 1], __uint_as_float(sr[q & 1][g * 16 + e]), __uint_as_float(sr[q & 1][g * 16 + e + 1]), f, f, b, b);
-                                if (kRaw && e / 2 < kPolyPairs) {
+                                if constexpr (kMasked) {
+                                    x[e] = seen >> (g * 16 + e) & 1u ? x[e] : -INFINITY;
+                                    x[e + 1] = seen >> (g * 16 + e + 1) & 1u ? x[e + 1] : -INFINITY;
+                                }
+                                if (kRaw && !kMasked && e / 2 < kPolyPairs) {
                                     exp2_poly(x[e], x[e + 1]);
                                 } else {
                                     x[e] = exp2_approx(x[e]);
@@ -631,9 +647,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
                 // row of the warp) is done again below. S stays until P is
                 // known to be good.
                 bool done = false;
-                if (plain && __all_sync(0xffffffffu, m > -INFINITY)) {
-                    float sum = l;
-                    const float most = weights(std::true_type{}, m, sum);
+                if ((plain || (SINKS && !CAP)) && __all_sync(0xffffffffu, m > -INFINITY)) {
+                    float sum = l, most;
+                    if constexpr (SINKS && !CAP) {
+                        // Most tiles of a short window are masked: two prompts of 4096 with a window of 512 and 16
+                        // sinks take 169 us, in the two passes below 180; chunks of 1000 with 1500 and 37 77, 83.
+                        if (plain) most = weights(std::true_type{}, std::false_type{}, m, sum);
+                        else most = weights(std::true_type{}, std::true_type{}, m, sum);
+                    } else {
+                        most = weights(std::true_type{}, std::false_type{}, m, sum);
+                    }
                     done = !__any_sync(0xffffffffu, most > 256.0f);
                     if (done) l = sum;
                 }
@@ -675,7 +698,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
                             }
                         }
                     }
-                    weights(std::false_type{}, m == -INFINITY ? 0.0f : m, l);
+                    weights(std::false_type{}, std::false_type{}, m == -INFINITY ? 0.0f : m, l);
                 }
                 tmem_st_32x32b_x32(ts, reinterpret_cast<uint32_t(&)[32]>(p[0]));
                 tmem_st_32x32b_x32(ts + 32, reinterpret_cast<uint32_t(&)[32]>(p[32]));
