@@ -40,6 +40,7 @@ constexpr int kPairs = 256;  // of which so many by comparing each with each
 constexpr uint32_t kOneBits = 0x3ff00000u;  // the upper word of 1.0
 constexpr int kBinShift = 14;  // a bin of the weights' histogram: their upper words but for these bits
 constexpr unsigned kAll = 0xffffffffu;
+constexpr float kLowest = -3.402823466385288598e38f;  // the least finite float, which masks use
 
 struct SampleArgs {
     const void *logits;
@@ -675,7 +676,7 @@ struct Row {
         // The tokens lighter than (1 - top_p) of the mean weight weigh less than 1 - top_p together: the cut is above them.
         const double t = log2((1.0 - top_p) * whole / a.vocab) / weight.per;
         const double margin = 1e-6 * (fabs(weight.top) + fabs(t));
-        return slowly<false>(keep, fmaxf(least, static_cast<float>(fmax(weight.top + t - margin, -3.4e38))), static_cast<float>(weight.top), 0, target, whole);
+        return slowly<false>(keep, fmaxf(least, static_cast<float>(fmax(weight.top + t - margin, kLowest))), static_cast<float>(weight.top), 0, target, whole);
     }
 
     // cut_slow() apart, on a copy: its registers are not the quick ways' concern.
@@ -907,7 +908,7 @@ __global__ void __launch_bounds__(NT, NT == 1024 ? 1 : 3) k_sample(SampleArgs a)
         return;
     }
     const double per = 1.4426950408889634074 / temperature;
-    const float least = fmaxf(best - 693.147f * temperature, -3.4e38f);  // 2^-1000
+    const float least = fmaxf(best - 693.147f * temperature, kLowest);  // 2^-1000
     r.weight = Weight{best, per, least};
     const Weight &weight = r.weight;
 
@@ -937,13 +938,13 @@ __global__ void __launch_bounds__(NT, NT == 1024 ? 1 : 3) k_sample(SampleArgs a)
         // The least float whose weight is min_p or more: of 32 about the logarithm's, or where it is not among
         // them (weights round to min_p over many floats: a largest logit near 0), by halving.
         const double at_least = min_p < 1.0f ? min_p : 1.0;
-        const uint32_t k_top = key_of(best), about = key_of(fmaxf(best + log2f(static_cast<float>(at_least)) / static_cast<float>(per), -3.4e38f) + 0.0f);
+        const uint32_t k_top = key_of(best), about = key_of(fmaxf(best + log2f(static_cast<float>(at_least)) / static_cast<float>(per), kLowest) + 0.0f);
         uint32_t k = min(about + 8, k_top) - 31 + r.lane;
         const uint32_t reach = __ballot_sync(kAll, weight(value_of(k)) >= at_least);
         if ((reach & 1u) == 0 && reach != 0) {
             k = __shfl_sync(kAll, k, __ffs(reach) - 1);
         } else {
-            uint32_t under = key_of(-3.4e38f) - 1;
+            uint32_t under = key_of(kLowest) - 1;
             k = k_top;
             while (k - under > 1) {
                 const uint32_t mid = under + (k - under) / 2;
@@ -1109,6 +1110,7 @@ int launch_sample(const SampleArgs &a, int64_t rows, cudaStream_t st) {
 
 template <typename T>
 int dispatch_sample(SampleArgs a, int64_t rows, cudaStream_t st) {
+    LCML_CHECK_ARG(rows <= 0x7fffffff / kMaxCluster, "lcml_sample: too many rows for one call");
     constexpr int E = Row<T, true, 1024>::E;
     const int64_t length = static_cast<int64_t>(a.vocab) + E - 1;
     auto slice = [&](int ctas, int threads) {
@@ -1129,7 +1131,6 @@ int dispatch_sample(SampleArgs a, int64_t rows, cudaStream_t st) {
     }
     while (a.ctas < 4 && fits(2 * a.ctas) && slice(a.ctas, 1024) > 16384) a.ctas *= 2;
     a.slice = static_cast<int>(slice(a.ctas, 1024));
-    LCML_CHECK_ARG(rows * a.ctas <= 0x7fffffff, "lcml_sample: too many rows for one call");
     if (a.slice * static_cast<int64_t>(sizeof(T)) > kStageMost<1024>) return launch_sample<T, false, 1024>(a, rows, st);
     return launch_sample<T, true, 1024>(a, rows, st);
 }

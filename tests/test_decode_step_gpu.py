@@ -102,6 +102,14 @@ def test_plan(dev, batch, most, page, stride, ended):
     _check_plan(dev, new, held, over, page, cols, spare=batch * cols, total=sum(new) + 77, in_place=True)  # padded, in place
 
 
+def test_plan_of_the_most_rows(dev):
+    rng = random.Random(5)
+    held = [rng.randint(0, 60) for _ in range(16384)]
+    over = [rng.random() < 0.2 for _ in range(16384)]
+    _check_plan(dev, [rng.choice([0, 1, 1, 1, 9]) for _ in range(16384)], held, over, 16, 6, spare=16384)
+    _check_plan(dev, [1] * 16384, held, [False] * 16384, 16, 6, spare=16384, in_place=True)
+
+
 def test_plan_of_nothing(dev):
     import luisaml_b200 as lb
     none = _ints([], dev)
@@ -512,6 +520,22 @@ def test_sample_special_values(dev):
     u = torch.full((8,), 0.6, device=dev)
     for s in SETTINGS + [{"temperature": inf}, {"temperature": 1e-30, "top_p": 0.5}, {"temperature": 1e30, "top_p": 0.5}, {"temperature": 1e38, "min_p": 0.5}]:
         _check_sample(x, u, **{k: _all(dev, 8, v, torch.int32 if k == "top_k" else torch.float32) for k, v in s.items()})
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab", [700, 30001])
+def test_sample_masks_of_the_lowest_value(dev, vocab, dtype):
+    """rows whose mask is the type's lowest value: of all tokens, of all but one, of all but a few"""
+    x, u = _rows(dev, 5, vocab, dtype)
+    lowest = torch.finfo(x.dtype).min
+    x[0] = lowest
+    x[1, :vocab - 1] = lowest
+    x[2, 3:] = lowest
+    x[3, ::2] = lowest
+    x[4] = -math.inf
+    x[4, 5] = lowest
+    for s in SETTINGS:
+        _check_sample(x, u, **{k: _all(dev, 5, v, torch.int32 if k == "top_k" else torch.float32) for k, v in s.items()})
 
 
 def test_sample_uniform_at_its_ends(dev):
