@@ -300,12 +300,19 @@ struct Row {
     // them all, in the order of the tokens. The barrier also makes what was stored
     // into other CTAs before it visible there.
     __device__ __forceinline__ Told tell(unsigned long long v0, unsigned long long v1) {
+        say(v0, v1);
+        return hear();
+    }
+    __device__ __forceinline__ void say(unsigned long long v0, unsigned long long v1) {
         if (lane < a.ctas) {
             const uint32_t to = mapa_shared(smem_u32(&sh.slot[turn][rank * kWarps + warp][0]), lane);
             st_cluster(to, v0);
             st_cluster(to + 8, v1);
         }
-        cluster_sync_all();
+        asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    }
+    __device__ __forceinline__ Told hear() {
+        asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
         const Told got = sh.slot[turn];
         turn ^= 1;
         return got;
@@ -448,13 +455,24 @@ struct Row {
     __device__ __forceinline__ void list(float v, int i, bool in, int which) {
         const uint32_t m = __ballot_sync(kAll, in);
         if (m == 0) return;
+        const bool one = a.ctas == 1;  // CTA: without the way round by the cluster
         uint32_t at = 0;
-        if (lane == 0) at = add_cluster(mapa_shared(smem_u32(&sh.listed[which]), 0), __popc(m));
+        if (lane == 0) at = one ? atomicAdd(&sh.listed[which], __popc(m)) : add_cluster(mapa_shared(smem_u32(&sh.listed[which]), 0), __popc(m));
         at = __shfl_sync(kAll, at, 0) + __popc(m & ((1u << lane) - 1));
-        if (in && at < kList)
-            for (int r = 0; r < a.ctas; ++r) st_cluster(mapa_shared(smem_u32(&sh.list[0]), r) + at * 8, entry_of(v, i));
+        if (in && at < kList) {
+            if (one) {
+                sh.list[at] = entry_of(v, i);
+            } else {
+                for (int r = 0; r < a.ctas; ++r) st_cluster(mapa_shared(smem_u32(&sh.list[0]), r) + at * 8, entry_of(v, i));
+            }
+        }
     }
 
+    // A listed token's weight in units of 2^-52, at least one of what weighs anything.
+    __device__ __forceinline__ unsigned long long units_of(unsigned long long entry) const {
+        const double w = weight(value_of(static_cast<uint32_t>(entry >> 32)));
+        return max(static_cast<unsigned long long>(w * 0x1p52), w > 0.0 ? 1ull : 0ull);
+    }
     // The cut of the first `want` (kCount) of the n listed tokens and, top_p below 1, of the fewest first ones
     // of those whose weights sum to top_p of theirs; or (not kCount) of the fewest first ones whose
     // weights and `above` reach `target`. 0: none does, though there are n.
@@ -466,7 +484,7 @@ struct Row {
             // of 2^-52 (exact sums, whatever the list's order).
             const int q = threadIdx.x & 3;
             const uint32_t stays = min(want, n);
-            for (uint32_t i = threadIdx.x; i < n; i += NT) sh.part[i] = static_cast<unsigned long long>(weight(value_of(static_cast<uint32_t>(sh.list[i] >> 32))) * 0x1p52);
+            for (uint32_t i = threadIdx.x; i < n; i += NT) sh.part[i] = units_of(sh.list[i]);
             if (threadIdx.x == 0) sh.verdict = 0;
             __syncthreads();
             auto place = [&](uint32_t t, unsigned long long &before) {
@@ -564,6 +582,34 @@ struct Row {
         return sh.list[last];
     }
 
+    // Rank 0: the draw from n listed tokens, those up to the cut; four threads a token, as in cut_of_list().
+    __device__ __forceinline__ void draw_listed(uint32_t n, unsigned long long cut, float uniform, int64_t row) {
+        const int q = threadIdx.x & 3;
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < n; i += NT) sh.part[i] = sh.list[i] >= cut ? units_of(sh.list[i]) : 0;
+        __syncthreads();
+#pragma unroll 1
+        for (uint32_t t0 = 0; t0 < n; t0 += NT / 4) {
+            const uint32_t t = t0 + threadIdx.x / 4;
+            const unsigned long long mine = t < n ? sh.list[t] : 0, own = t < n ? sh.part[t] : 0;
+            unsigned long long before = 0, all = 0;
+            for (uint32_t j = q; j < n; j += 4) {
+                all += sh.part[j];
+                before += static_cast<uint32_t>(sh.list[j]) > static_cast<uint32_t>(mine) ? sh.part[j] : 0;  // a lower index
+            }
+#pragma unroll
+            for (int o = 1; o < 4; o *= 2) {
+                before += __shfl_xor_sync(kAll, before, o);
+                all += __shfl_xor_sync(kAll, all, o);
+            }
+            const double target = (uniform > 0.0f ? static_cast<double>(uniform) : 0.0) * static_cast<double>(all);
+            if (q == 0 && own > 0 && static_cast<double>(before) <= target && (static_cast<double>(before + own) > target || before + own == all)) {
+                a.tokens[row] = static_cast<int>(0xffffffffu - static_cast<uint32_t>(mine));
+                if (a.logprob != nullptr) a.logprob[row] = static_cast<float>(log(weight(value_of(static_cast<uint32_t>(mine >> 32))) / (static_cast<double>(all) * 0x1p-52)));
+            }
+        }
+    }
+
     // The first k tokens' cut (0: there are fewer, all stay). own: the thread's largest logit, low: the
     // least of these that counts, least: a bound of all that do. Where the first k are few, top_p (below 1) is applied to them too, and listed is
     // how many are in the list, all that stay among them.
@@ -593,9 +639,10 @@ struct Row {
     }
 
     // The cut of the fewest first tokens, of those that `keep` takes (all, but for `some`), whose weights sum to top_p of theirs. above: what the
-    // warp's tokens before the list sum to, listed: the tokens in the list (more than kList: neither holds).
+    // warp's tokens before the list sum to (all_listed: there are none), listed: the tokens in the list (more than
+    // kList: neither holds).
     template <typename F>
-    __device__ __forceinline__ unsigned long long cut_mass(F keep, bool some, float least, double top_p, double &above, uint32_t &listed) {
+    __device__ __forceinline__ unsigned long long cut_mass(F keep, bool some, float least, double top_p, double &above, uint32_t &listed, bool &all_listed) {
         clear_bins();
         double mass = 0.0;
         auto weigh = [&](const float(&v)[E], int i, auto some) {
@@ -616,11 +663,12 @@ struct Row {
         const double whole = sum_of(tell(__double_as_longlong(warp_sum(mass)), 0)), target = top_p * whole;
         // the bins before which the sum, 1e-4 of the whole more or less, does not reach the target
         {
-            float c[kPer], mine = 0.0f;
+            float c[kPer], mine = 0.0f, tokens = 0.0f;  // mass, and at most so many tokens (a unit sum is 2^14 to 2^15 each)
             all_bins(c);
             const int b = kPer * threadIdx.x;
 #pragma unroll
             for (int j = 0; j < kPer; ++j) {
+                tokens += c[j] * 0x1p-14f;
                 c[j] *= __int_as_float((127 - 14 - (b + j + 63) / 64) << 23);
                 mine += c[j];
             }
@@ -647,19 +695,30 @@ struct Row {
             if (first < kBins) atomicMin(&sh.first, first);
             if (last < kBins) atomicMin(&sh.last, last);
             __syncthreads();
+            // few tokens up to the last of these bins: they are all listed
+            tokens = b <= min(sh.last, kBins - 2) ? tokens : 0.0f;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) tokens += __shfl_xor_sync(kAll, tokens, o);
+            if (lane == 0) sh.scan_f[warp] = tokens;
+            __syncthreads();
+            tokens = lane < kWarps ? sh.scan_f[lane] : 0.0f;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) tokens += __shfl_xor_sync(kAll, tokens, o);
+            all_listed = tokens <= 0.75f * kList;
         }
         const int first = sh.first, last = min(sh.last, kBins - 2);
         listed = kList + 1;
         if (first < kBins - 1) {
             // what lies before them, exactly, and their tokens
-            const float from = edge_above(first), to = edge_above(last + 1);
+            const float from = all_listed ? INFINITY : edge_above(first), to = edge_above(last + 1);
             uint32_t count = 0;
             double sum = 0.0;
             pick([&](float v, int i) { return v >= to && (!some || keep(v, i)); }, [&](float y, int j, bool is) {
                 list(y, j, is && y <= from, 1);
+                count += is && y <= from;
+                if (all_listed) return;
                 const double w = weight(y);
                 sum += is && y > from ? w : 0.0;
-                count += is && y <= from;
             });
             above = warp_sum(sum);
             const Told got = tell(__double_as_longlong(above), __reduce_add_sync(kAll, count));
@@ -860,6 +919,7 @@ __global__ void __launch_bounds__(NT, NT == 1024 ? 1 : 3) k_sample(SampleArgs a)
 
     // the row into shared memory, and its largest
     float own = -INFINITY, best = -INFINITY, low = -INFINITY;  // low: the least of the threads' largest
+    double per;
     int best_at = -1;
     {
         int own_at = 0x7fffffff;
@@ -889,8 +949,10 @@ __global__ void __launch_bounds__(NT, NT == 1024 ? 1 : 3) k_sample(SampleArgs a)
         const uint32_t key = own_at != 0x7fffffff ? key_of(own + 0.0f) : 0u, most = __reduce_max_sync(kAll, key);
         const int first = __reduce_min_sync(kAll, key == most ? own_at : 0x7fffffff);
         asm volatile("barrier.cluster.wait.acquire;" ::: "memory");  // every CTA has started
-        const auto got = r.tell(static_cast<unsigned long long>(most) << 32 | (0xffffffffu - static_cast<uint32_t>(first)),
-                                __reduce_max_sync(kAll, key != 0 ? 0xffffffffu - key : 0u));
+        r.say(static_cast<unsigned long long>(most) << 32 | (0xffffffffu - static_cast<uint32_t>(first)),
+              __reduce_max_sync(kAll, key != 0 ? 0xffffffffu - key : 0u));
+        per = 1.4426950408889634074 / temperature;  // while the others arrive
+        const auto got = r.hear();
         const uint32_t top = r.largest(got, 0, 1);
         if (top != 0) {
             best = value_of(top);
@@ -907,7 +969,6 @@ __global__ void __launch_bounds__(NT, NT == 1024 ? 1 : 3) k_sample(SampleArgs a)
         }
         return;
     }
-    const double per = 1.4426950408889634074 / temperature;
     const float least = fmaxf(best - 693.147f * temperature, kLowest);  // 2^-1000
     r.weight = Weight{best, per, least};
     const Weight &weight = r.weight;
@@ -926,13 +987,12 @@ __global__ void __launch_bounds__(NT, NT == 1024 ? 1 : 3) k_sample(SampleArgs a)
     const bool has_k = top_k > 0 && top_k < a.vocab, has_p = top_p < 1.0f;
     uint32_t listed = kList + 1;  // where it is less, the kept tokens are in the list, but for those that `above` sums
     double above = 0.0;
-    bool summed = false;
+    bool all_listed = true;
     if (has_k) set_cut(r.cut_count(own, fmaxf(low, least), least, best, static_cast<uint32_t>(top_k), has_p ? static_cast<double>(top_p) : 1.0, listed));
     if (has_p && listed > kList) {
         const float cx = cut_x;
         const int ci = cut_i;
-        summed = true;
-        set_cut(r.cut_mass([=](float v, int i) { return v > cx || (v == cx && i <= ci); }, cut != 0, fmaxf(least, cx), static_cast<double>(top_p), above, listed));
+        set_cut(r.cut_mass([=](float v, int i) { return v > cx || (v == cx && i <= ci); }, cut != 0, fmaxf(least, cx), static_cast<double>(top_p), above, listed, all_listed));
     }
     if (min_p > 0.0f) {
         // The least float whose weight is min_p or more: of 32 about the logarithm's, or where it is not among
@@ -955,11 +1015,15 @@ __global__ void __launch_bounds__(NT, NT == 1024 ? 1 : 3) k_sample(SampleArgs a)
         const unsigned long long c = static_cast<unsigned long long>(k) << 32 | (0xffffffffu - 0x7fffffffu);
         if (c > cut) {
             set_cut(c);
-            if (summed) listed = kList + 1;  // it may lie among the tokens that `above` sums
+            if (!all_listed) listed = kList + 1;  // it may lie among the tokens that `above` sums
         }
     }
 
-    // the draw
+    // the draw: from the list, if that is short and all there is
+    if (listed <= kPairs && all_listed) {
+        if (r.rank == 0) r.draw_listed(listed, cut, uniform, row);
+        return;
+    }
     double mass;
     if (listed <= kList) {
         mass = 0.0;
@@ -969,7 +1033,7 @@ __global__ void __launch_bounds__(NT, NT == 1024 ? 1 : 3) k_sample(SampleArgs a)
                 const unsigned long long e = sh.list[j];
                 const float v = value_of(static_cast<uint32_t>(e >> 32));
                 const int i = static_cast<int>(0xffffffffu - static_cast<uint32_t>(e));
-                if (r.own_warp(i) && keep(v, i)) sum += static_cast<unsigned long long>(weight(v) * 0x1p52);
+                if (r.own_warp(i) && keep(v, i)) sum += r.units_of(e);
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
