@@ -704,7 +704,7 @@ struct Row {
             tokens = lane < kWarps ? sh.scan_f[lane] : 0.0f;
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) tokens += __shfl_xor_sync(kAll, tokens, o);
-            all_listed = tokens <= 0.75f * kList;
+            all_listed = tokens <= kPairs;
         }
         const int first = sh.first, last = min(sh.last, kBins - 2);
         listed = kList + 1;
