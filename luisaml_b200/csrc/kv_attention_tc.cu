@@ -22,13 +22,15 @@
 //
 // With sinks (SINKS) the key tiles are those over the first positions, then the
 // window's; a box of keys that no row sees is not looked up, its values are zeros.
-// Masked tiles are weighed in one pass there. A unit of a short window is mostly set-up:
-// 54,000 clocks for 6.5 key tiles, of which steady tiles would take 22,000.
+// Masked tiles are weighed in one pass there. A unit of a short window is mostly set-up
+// and end: of 42,700 clocks (window 512, 16 sinks, two row tiles of 32 + 8 heads of 128) 2,500
+// look-ups and allocation, 9,000 q's load and split (12,000 with a division per row), 5,000
+// the first tile's weights in two passes, 4,500 the output and the release.
 //
 // Bound: the tensor cores (4 head_dim FLOP per visible pair) and the
 // exponentials, 16 a clock per SM: equal at head_dim 128, twice the products'
 // time at 64. Measured at 128 (two prompts of up to 4096, 32 heads over 8, bf16):
-// 236 us, 0.75 PFLOP/s (both of 4096: 327; with capped scores, which take every
+// 225 us, 0.79 PFLOP/s (both of 4096: 318; with capped scores, which take every
 // tile in the two passes of the masked ones, 613). A pair of key tiles takes 3450 clocks, of which the
 // MMAs run 2048 and the weights of one row tile 1650. What was tried beside:
 // P V of the first 64 keys under the weights of the others (one row tile 3360 ->
@@ -525,15 +527,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
                 const bool vec = aligned(a.q, 16) && a.q_token_stride % 8 == 0 && a.q_head_stride % 8 == 0;
                 uint4 e8[kPasses];  // all loads at once: one latency
                 uint32_t mx[kPasses];
+                // the pass's row, RPW rows on each time: one division in all
+                int in_group = (w.row0 + r0) % a.group;
+                const int more_queries = RPW / a.group, more_heads = RPW % a.group;
+                const uint16_t *p = static_cast<const uint16_t *>(a.q) + (w.t0 + static_cast<int64_t>((w.row0 + r0) / a.group)) * a.q_token_stride +
+                                    (static_cast<int64_t>(w.head) * a.group + in_group) * a.q_head_stride + part_lane * 8;
+                const int64_t step = more_queries * a.q_token_stride + more_heads * a.q_head_stride, wrap = a.q_token_stride - a.group * a.q_head_stride;
 #pragma unroll
                 for (int u = 0; u < kPasses; ++u) {
                     const int r = r0 + u * RPW;
                     e8[u] = make_uint4(0, 0, 0, 0);
                     if (r < w.rows) {
-                        const int row = w.row0 + r;
-                        const int64_t off = (w.t0 + static_cast<int64_t>(row / a.group)) * a.q_token_stride +
-                                            (static_cast<int64_t>(w.head) * a.group + row % a.group) * a.q_head_stride + part_lane * 8;
-                        const uint16_t *p = static_cast<const uint16_t *>(a.q) + off;
                         if (vec) {
                             e8[u] = __ldg(reinterpret_cast<const uint4 *>(p));
                         } else {
@@ -542,6 +546,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
                             for (int i = 0; i < 4; ++i) h[i] = p[2 * i] | (static_cast<uint32_t>(p[2 * i + 1]) << 16);
                             e8[u] = make_uint4(h[0], h[1], h[2], h[3]);
                         }
+                    }
+                    p += step;
+                    in_group += more_heads;
+                    if (in_group >= a.group) {
+                        in_group -= a.group;
+                        p += wrap;
                     }
                 }
                 // a row's largest magnitude: 16-bit floats order like their bits (NaN above infinity)
@@ -583,6 +593,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
             const float factor = sh.row_factor[r] * (CAP ? a.inv_cap : a.scale_log2);  // this warp's own rows
             const uint32_t lane_base = static_cast<uint32_t>(warp & 3) << 21;  // TMEM lanes 32 (warp % 4) ..
             const uint32_t ts = tmem + lane_base + t * kTile, to = tmem + lane_base + 2 * kTile + t * D;
+            // which of 32 keys from k0 on the row sees
+            auto row_sees = [&](int k0) { return (bits_from(first - k0) | ~bits_from(sinks - k0)) & ~bits_from(last + 1 - k0); };
             float m = -INFINITY, l = 0.0f;
             bool ok = true;
             for (int j = 0; j < n; ++j) {
@@ -612,7 +624,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
                         if (q < 3) tmem_ld_32x32b_x32(ts + (q + 1) * 32, sr[(q + 1) & 1]);
                         // keys of these 32 that the row sees
                         uint32_t seen = 0;
-                        if constexpr (kMasked) seen = (bits_from(first - base - q * 32) | ~bits_from(sinks - base - q * 32)) & ~bits_from(last + 1 - base - q * 32);
+                        if constexpr (kMasked) {
+                            seen = row_sees(base + q * 32);
+                            if (!__any_sync(0xffffffffu, seen != 0)) {  // of no row of the warp
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) p[q * 16 + e] = 0;
+                                continue;
+                            }
+                        }
 #pragma unroll
                         for (int g = 0; g < 2; ++g) {
                             const float f = kRaw ? (g ? g1.x : g0.x) * factor : 1.0f, b = (kRaw ? (g ? g1.y : g0.y) : 0.0f) - ref;
@@ -650,8 +669,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
                 if ((plain || (SINKS && !CAP)) && __all_sync(0xffffffffu, m > -INFINITY)) {
                     float sum = l, most;
                     if constexpr (SINKS && !CAP) {
-                        // Most tiles of a short window are masked: two prompts of 4096 with a window of 512 and 16
-                        // sinks take 169 us, in the two passes below 180; chunks of 1000 with 1500 and 37 77, 83.
+                        // Most tiles of a short window are masked: of two prompts of 4096 with a window of 512 and 16
+                        // sinks this saves 11 of 180 us against the two passes below, of chunks of 1000 6 of 83.
                         if (plain) most = weights(std::true_type{}, std::false_type{}, m, sum);
                         else most = weights(std::true_type{}, std::true_type{}, m, sum);
                     } else {
@@ -666,6 +685,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_kv_attention_tc(const __grid_co
 #pragma unroll 1
                     for (int q = 0; q < 4; ++q) {
                         uint32_t(&r)[32] = sr[0];
+                        if constexpr (SINKS) {
+                            if (!__any_sync(0xffffffffu, row_sees(base + q * 32) != 0)) {
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(-INFINITY);
+                                tmem_st_32x32b_x32(ts + q * 32, r);
+                                continue;
+                            }
+                        }
                         tmem_ld_32x32b_x32(ts + q * 32, r);
                         tmem_wait_ld();
 #pragma unroll
@@ -828,7 +855,7 @@ int launch_tc(const lcml_kv_attention_desc *d, const AttnArgs &a, int min_rows, 
                           D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return set_error(LCML_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
-    // without sinks two prompts of 4096 take 232 us, with their tests in the kernel 240
+    // a kernel without the sinks' tests: they cost two prompts of 4096, which have none, 8 us of 232
     auto kern = a.sinks > 0 ? k_kv_attention_tc<D, NP, CAP, true> : k_kv_attention_tc<D, NP, CAP, false>;
     const int rc = ensure_max_smem(reinterpret_cast<const void *>(kern), S::kSmem, "kv_attention_tc");
     if (rc != LCML_OK) return rc;
