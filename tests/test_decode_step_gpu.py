@@ -258,6 +258,25 @@ def test_rope_far_positions_and_skipped_tokens(dev):
     assert ((a[6:].double() - want).abs() <= size * (2 * math.pi * 2.0 ** -20 + 32 * 2.0 ** -24)).all()
 
 
+def test_rope_strides(dev):
+    """heads before tokens, and tokens further apart than 32 bits count"""
+    import luisaml_b200 as lb
+    pos = torch.arange(7, dtype=torch.int32, device=dev) + 50
+    q, k = torch.randn(5, 7, 64, device=dev).half().transpose(0, 1), torch.randn(2, 7, 64, device=dev).half().transpose(0, 1)
+    w = torch.ones(64, device=dev)
+    out = torch.empty(5, 7, 64, device=dev, dtype=torch.float16).transpose(0, 1)
+    a, b = lb.qk_norm_rope(q, k, pos, _freq(64, dev), w, w, q_out=out)
+    assert a is out
+    _check_rope(q, pos, _freq(64, dev), w, 1e-6, False, a)
+    _check_rope(k, pos, _freq(64, dev), w, 1e-6, False, b)
+    big = torch.empty((1 << 31) + 1024, dtype=torch.bfloat16, device=dev)
+    q = big.as_strided((3, 4, 64), (1 << 30, 64, 1))
+    q.copy_(torch.randn(3, 4, 64, device=dev))
+    was = q.clone()
+    lb.qk_norm_rope(q, q[:, :0], pos[:3], _freq(64, dev), q_out=q)
+    _check_rope(was, pos[:3], _freq(64, dev), None, 1e-6, False, q)
+
+
 def test_rope_special_values(dev):
     """An infinity or NaN reaches its own pair (and with a norm its head), nothing else."""
     import luisaml_b200 as lb
@@ -562,7 +581,27 @@ def test_sample_strides_streams_and_outputs(dev):
         got = lb.sample(x, u, out=out)
     torch.cuda.current_stream().wait_stream(side)
     assert got is out and torch.equal(out, lb.sample(x, u))
+    # two captured calls, replayed in turn, on the same and on different rows
+    graphs, outs = [], []
+    for part in (x, x[2:], x):
+        outs.append(torch.empty(part.shape[0], dtype=torch.int32, device=dev))
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            lb.sample(part, u[:part.shape[0]], top_p=_all(dev, part.shape[0], 0.8), out=outs[-1])
+    for _ in range(3):
+        for g in graphs:
+            g.replay()
+    for part, o in zip((x, x[2:], x), outs):
+        assert torch.equal(o, lb.sample(part, u[:part.shape[0]], top_p=_all(dev, part.shape[0], 0.8)))
     assert lb.sample(x[:0], u[:0]).shape == (0,)
+
+
+def test_sample_rows_far_apart(dev):
+    x, u = _rows(dev, 3, 5000)
+    big = torch.empty((1 << 31) + 5000, dtype=torch.float32, device=dev)
+    far = big.as_strided((3, 5000), (1 << 30, 1))
+    far.copy_(x)
+    _check_sample(far, u, top_p=_all(dev, 3, 0.9))
 
 
 def test_sample_draws_by_the_probabilities(dev):
