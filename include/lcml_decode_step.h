@@ -127,7 +127,7 @@ int lcml_kv_attention_sinks(const lcml_kv_attention_desc *desc, int32_t sinks, l
  * (temperature: 1).
  */
 typedef struct lcml_sample_desc {
-    int64_t rows, vocab;       /* vocab < 2^31 */
+    int64_t rows, vocab;       /* vocab <= 2^31 - 65537 */
     const void *logits;        /* [rows, vocab], row stride ld elements */
     int64_t ld;
     int dtype;                 /* FLOAT, FLOAT16 or BFLOAT16 */

@@ -451,10 +451,17 @@ PyObject *qk_norm_rope(PyObject *const *o) {
     d.inv_freq = freq.data_ptr();
     d.inv_freq_dtype = freq.scalar_type() == at::kDouble ? LCML_DTYPE_DOUBLE : LCML_DTYPE_FLOAT;
     check(lcml_qk_norm_rope(&d, stream_of(dev)));
-    PyObject *a = made_q.defined() ? wrap(made_q) : same(o[8]), *b = made_k.defined() ? wrap(made_k) : same(o[9]);
     PyObject *t = PyTuple_New(2);
-    PyTuple_SET_ITEM(t, 0, a);
-    PyTuple_SET_ITEM(t, 1, b);
+    if (t == nullptr) throw Raised{};
+    for (int i = 0; i < 2; ++i) {
+        const at::Tensor &made = i ? made_k : made_q;
+        PyObject *x = made.defined() ? THPVariable_Wrap(made) : same(o[8 + i]);
+        if (x == nullptr) {
+            Py_DECREF(t);
+            throw Raised{};
+        }
+        PyTuple_SET_ITEM(t, i, x);
+    }
     return t;
 }
 
