@@ -93,6 +93,10 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(lcml_kv_plan_desc a, int *
     const int total = static_cast<int>(a.total_tokens);
     bool bad = false;
 
+    if (a.ended != nullptr) {
+        for (int b = threadIdx.x; b < batch; b += blockDim.x) pages[b] = 0;
+        asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    }
     griddep_launch_dependents();
     griddep_wait();
     const int listed = *a.free_count;
@@ -104,24 +108,31 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(lcml_kv_plan_desc a, int *
         return static_cast<int>(min((static_cast<uint32_t>(tokens) + ps - 1) / ps, static_cast<uint32_t>(a.table_cols)));
     };
     if (a.ended != nullptr) {
-        // a warp per row, the rows dealt to the cluster's warps; a count goes to every CTA
+        // The rows are dealt to the cluster's warps, which take their ended ones in turn; a count goes to every CTA.
         auto row_entry = [&](int b, int c, int n) -> int { return c < n ? a.block_table[b * a.table_stride + c] : -1; };
         const int warps = stride >> 5, w = me >> 5;
-        cluster_sync_all();  // every CTA has started
-        for (int b = w; b < batch; b += warps) {
-            const int held = a.held[b];
-            int n = 0;
-            if (a.ended[b] != 0) {
-                const int cols = columns(max(0, held));
-#pragma unroll 4
-                for (int c0 = 0; c0 < cols; c0 += 32) n += row_entry(b, c0 + lane, cols) >= 0;
-                n = __reduce_add_sync(kAll, n);
+        auto each_ended = [&](auto f) {
+            for (int b0 = w; b0 < batch; b0 += 32 * warps) {
+                const int b = b0 + lane * warps;
+                const bool in = b < batch;
+                const int cols = in ? columns(max(0, a.held[b])) : 0;
+                for (uint32_t m = __ballot_sync(kAll, in && a.ended[in ? b : 0] != 0); m != 0; m &= m - 1) {
+                    const int l = __ffs(m) - 1;
+                    f(b0 + l * warps, __shfl_sync(kAll, cols, l));
+                }
             }
+        };
+        asm volatile("barrier.cluster.wait.acquire;" ::: "memory");  // every CTA has started
+        each_ended([&](int b, int cols) {
+            int n = 0;
+#pragma unroll 4
+            for (int c0 = 0; c0 < cols; c0 += 32) n += row_entry(b, c0 + lane, cols) >= 0;
+            n = __reduce_add_sync(kAll, n);
             if (lane < ctas) {
                 const uint32_t to = mapa_shared(smem_u32(pages + b), lane);
                 asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(n) : "memory");
             }
-        }
+        });
         cluster_sync_all();
         int64_t unused = 0;
         int32_t back = 0;
@@ -133,9 +144,7 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(lcml_kv_plan_desc a, int *
             if (b < batch) pages[b] = mine;
         }
         __syncthreads();
-        for (int b = w; b < batch; b += warps) {
-            if (a.ended[b] == 0) continue;
-            const int cols = columns(max(0, a.held[b]));
+        each_ended([&](int b, int cols) {
             int64_t at = count + pages[b];
 #pragma unroll 4
             for (int c0 = 0; c0 < cols; c0 += 32) {
@@ -148,10 +157,10 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(lcml_kv_plan_desc a, int *
                 }
                 at += __popc(have);
             }
-        }
+        });
         bad |= count + back > capacity;
         count = count + back < capacity ? count + back : capacity;
-        cluster_sync_all();  // the free list is complete, and `pages` may be written again
+        __syncthreads();  // `pages` may be written again
     }
 
     // Sums of the tokens and of the new entries; these again where tokens are left out.
@@ -189,7 +198,8 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(lcml_kv_plan_desc a, int *
     }
     if (threadIdx.x == 0) cu[batch] = static_cast<int32_t>(min(tokens, static_cast<int64_t>(total)));
     if (rank == 0 && bad) record_device_error(err, kDevBadBatch);
-    if (ctas > 1) cluster_sync_all();  // every CTA has read held and free_count: kv_len and free_count_out may be the same memory
+    // The free list is complete, and every CTA has read held and free_count: kv_len and free_count_out may be the same memory.
+    if (ctas > 1) cluster_sync_all();
     else __syncthreads();
 
     auto page_of = [&](int i) -> int { return i < count ? a.free_pages[count - 1 - i] : -1; };
