@@ -10,6 +10,8 @@
 // entry and slots are computed apart, without a second pass over the table.
 //
 // Bound: latency. A step of 64 rows moves 2 KB.
+#include <type_traits>
+
 #include "lcml_decoder.cuh"
 
 #include "../../include/lcml_decode_step.h"
@@ -22,6 +24,7 @@ constexpr int kMaxRows = 16384;
 constexpr int kThreads = 1024;  // at most
 constexpr int kWarps = kThreads / 32;
 constexpr int kCluster = 8;
+constexpr int kEntries = 8;  // of an ended row, that a lane loads at once
 constexpr unsigned kAll = 0xffffffffu;
 
 // Exclusive sums of two values a thread over the block; the totals are added to `tokens` and `entries`.
@@ -69,16 +72,25 @@ __device__ __forceinline__ void block_scan(Scan &sh, int64_t &a, int32_t &b, int
 
 // The last i in [0, n) with first[i] <= x; first[0] <= x, not decreasing.
 __device__ __forceinline__ int last_at_or_below(const int32_t *first, int n, int x) {
-    int lo = 0, hi = n - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (first[mid] <= x) lo = mid;
-        else hi = mid - 1;
-    }
+    int lo = 0;
+    for (int step = 1 << (31 - __clz(n | 1)); step > 0; step >>= 1)
+        if (lo + step < n && first[lo + step] <= x) lo += step;
     return lo;
 }
 
-__global__ void __launch_bounds__(kThreads) k_kv_plan(lcml_kv_plan_desc a, int *err) {
+// n / page_size for n below 2^31: (n factor) >> shift, where 2^shift is 2^31 times the least power of two
+// that is page_size or more and factor = floor(2^shift / page_size) + 1, too large by page_size / 2^shift at most.
+struct PageDivision {
+    uint32_t factor;
+    int shift;
+    explicit PageDivision(uint32_t page_size) : shift(31) {
+        while ((1u << (shift - 31)) < page_size) ++shift;
+        factor = static_cast<uint32_t>((uint64_t{1} << shift) / page_size + 1);
+    }
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return static_cast<uint32_t>(static_cast<uint64_t>(n) * factor >> shift); }
+};
+
+__global__ void __launch_bounds__(kThreads) k_kv_plan(lcml_kv_plan_desc a, PageDivision page_in, int *err) {
     extern __shared__ int32_t smem[];
     __shared__ Scan scan;
     const int batch = a.batch;
@@ -105,7 +117,7 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(lcml_kv_plan_desc a, int *
     bad |= count != listed;
 
     auto columns = [&](int tokens) -> int {  // columns of the table that hold this many (>= 0)
-        return static_cast<int>(min((static_cast<uint32_t>(tokens) + ps - 1) / ps, static_cast<uint32_t>(a.table_cols)));
+        return tokens > 0 ? min(static_cast<int>(page_in(tokens - 1)) + 1, a.table_cols) : 0;
     };
     if (a.ended != nullptr) {
         // The rows are dealt to the cluster's warps, which take their ended ones in turn; a count goes to every CTA.
@@ -125,8 +137,10 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(lcml_kv_plan_desc a, int *
         asm volatile("barrier.cluster.wait.acquire;" ::: "memory");  // every CTA has started
         each_ended([&](int b, int cols) {
             int n = 0;
-#pragma unroll 4
-            for (int c0 = 0; c0 < cols; c0 += 32) n += row_entry(b, c0 + lane, cols) >= 0;
+            for (int c0 = 0; c0 < cols; c0 += 32 * kEntries) {
+#pragma unroll
+                for (int j = 0; j < kEntries; ++j) n += row_entry(b, c0 + 32 * j + lane, cols) >= 0;
+            }
             n = __reduce_add_sync(kAll, n);
             if (lane < ctas) {
                 const uint32_t to = mapa_shared(smem_u32(pages + b), lane);
@@ -146,16 +160,20 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(lcml_kv_plan_desc a, int *
         __syncthreads();
         each_ended([&](int b, int cols) {
             int64_t at = count + pages[b];
-#pragma unroll 4
-            for (int c0 = 0; c0 < cols; c0 += 32) {
-                const int p = row_entry(b, c0 + lane, cols);
-                const uint32_t have = __ballot_sync(kAll, p >= 0);
-                const int64_t to = at + __popc(have & ((1u << lane) - 1));
-                if (p >= 0) {
-                    if (to < capacity) a.free_pages[to] = p;
-                    a.block_table[b * a.table_stride + c0 + lane] = -1;
+            for (int c0 = 0; c0 < cols; c0 += 32 * kEntries) {
+                int p[kEntries];
+#pragma unroll
+                for (int j = 0; j < kEntries; ++j) p[j] = row_entry(b, c0 + 32 * j + lane, cols);
+#pragma unroll
+                for (int j = 0; j < kEntries; ++j) {
+                    const uint32_t have = __ballot_sync(kAll, p[j] >= 0);
+                    const int64_t to = at + __popc(have & ((1u << lane) - 1));
+                    if (p[j] >= 0) {
+                        if (to < capacity) a.free_pages[to] = p[j];
+                        a.block_table[b * a.table_stride + c0 + 32 * j + lane] = -1;
+                    }
+                    at += __popc(have);
                 }
-                at += __popc(have);
             }
         });
         bad |= count + back > capacity;
@@ -215,45 +233,76 @@ __global__ void __launch_bounds__(kThreads) k_kv_plan(lcml_kv_plan_desc a, int *
         const int b = last_at_or_below(pages, batch, i);
         a.block_table[b * a.table_stride + columns(shift[b] + cu[b]) + (i - pages[b])] = page_of(i);
     }
-    // four tokens a thread, so that four pages are looked up at once
+    // A token a thread, or four, most of them of one row and page: 9 rows of 7001 tokens 6.5 us, 7.9 with a row
+    // and a look-up for each (with eight a thread 7.7).
     const int packed = cu[batch];
     const bool vec = aligned(a.positions, 16) && aligned(a.slots, 16);
-    for (int64_t t0 = 4 * static_cast<int64_t>(me); t0 < total; t0 += 4 * static_cast<int64_t>(stride)) {
-        int pos[4], slot[4], b = t0 < packed ? last_at_or_below(cu, batch, static_cast<int>(t0)) : 0;
-        const int32_t *from[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t t = t0 + j;
-            pos[j] = -1;
-            from[j] = nullptr;  // where the token's page is found
-            if (t >= packed) continue;
-            while (cu[b + 1] <= t) ++b;
-            pos[j] = static_cast<int>(min(static_cast<int64_t>(shift[b]) + t, static_cast<int64_t>(0x7fffffff)));
-            if (pos[j] < reach) {
-                const int col = static_cast<int>(static_cast<uint32_t>(pos[j]) / ps), held = columns(shift[b] + cu[b]), i = pages[b] + col - held;
-                if (col < held) from[j] = a.block_table + b * a.table_stride + col;
-                else if (i < count) from[j] = a.free_pages + (count - 1 - i);
+    auto fill = [&](auto width) {
+        constexpr int N = decltype(width)::value;
+        auto store = [&](int64_t t0, const int (&pos)[N], const int (&slot)[N]) {
+            if constexpr (N == 4) {
+                if (vec && t0 + N <= total) {
+                    *reinterpret_cast<int4 *>(a.positions + t0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+                    *reinterpret_cast<int4 *>(a.slots + t0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+                    return;
+                }
             }
-        }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) slot[j] = from[j] != nullptr ? *from[j] : -1;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t s = static_cast<int64_t>(slot[j]) * ps + static_cast<uint32_t>(pos[j]) % ps;
-            slot[j] = slot[j] >= 0 && s <= 0x7fffffff ? static_cast<int>(s) : -1;
-        }
-        if (vec && t0 + 4 <= total) {
-            *reinterpret_cast<int4 *>(a.positions + t0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
-            *reinterpret_cast<int4 *>(a.slots + t0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < N; ++j)
                 if (t0 + j < total) {
                     a.positions[t0 + j] = pos[j];
                     a.slots[t0 + j] = slot[j];
                 }
+        };
+        for (int64_t t0 = N * static_cast<int64_t>(me); t0 < total; t0 += N * static_cast<int64_t>(stride)) {
+            int pos[N], slot[N], b = t0 < packed ? last_at_or_below(cu, batch, static_cast<int>(t0)) : 0;
+            if (N > 1 && ps >= N && t0 + N <= packed && t0 + N <= cu[b + 1] && shift[b] + t0 + N <= 0x7fffffff) {
+                // tokens of one row, in two pages at most
+                const int p0 = shift[b] + static_cast<int>(t0), col = static_cast<int>(page_in(p0)), off = p0 - col * static_cast<int>(ps);
+                const int held = columns(shift[b] + cu[b]), first_new = pages[b];
+                auto page_at = [&](int c) -> int {
+                    if (c >= a.table_cols) return -1;
+                    return c < held ? a.block_table[b * a.table_stride + c] : page_of(first_new + c - held);
+                };
+                const int page0 = page_at(col), page1 = off + N > static_cast<int>(ps) ? page_at(col + 1) : -1;
+                const int64_t slot0 = static_cast<int64_t>(page0) * ps + off, slot1 = static_cast<int64_t>(page1) * ps + off - ps;
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    const bool in1 = off + j >= static_cast<int>(ps);
+                    const int64_t s = (in1 ? slot1 : slot0) + j;
+                    pos[j] = p0 + j;
+                    slot[j] = (in1 ? page1 : page0) >= 0 && s <= 0x7fffffff ? static_cast<int>(s) : -1;
+                }
+                store(t0, pos, slot);
+                continue;
+            }
+            const int32_t *from[N];
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const int64_t t = t0 + j;
+                pos[j] = -1;
+                from[j] = nullptr;  // where the token's page is found
+                if (t >= packed) continue;
+                while (cu[b + 1] <= t) ++b;
+                pos[j] = static_cast<int>(min(static_cast<int64_t>(shift[b]) + t, static_cast<int64_t>(0x7fffffff)));
+                if (pos[j] < reach) {
+                    const int col = static_cast<int>(page_in(pos[j])), held = columns(shift[b] + cu[b]), i = pages[b] + col - held;
+                    if (col < held) from[j] = a.block_table + b * a.table_stride + col;
+                    else if (i < count) from[j] = a.free_pages + (count - 1 - i);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < N; ++j) slot[j] = from[j] != nullptr ? *from[j] : -1;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const int64_t s = static_cast<int64_t>(slot[j]) * ps + (pos[j] - static_cast<int64_t>(page_in(pos[j])) * ps);
+                slot[j] = slot[j] >= 0 && s <= 0x7fffffff ? static_cast<int>(s) : -1;
+            }
+            store(t0, pos, slot);
         }
-    }
+    };
+    if (total <= stride) fill(std::integral_constant<int, 1>{});
+    else fill(std::integral_constant<int, 4>{});
     if (me == 0) {
         *a.free_count_out = static_cast<int32_t>(max(count - taken, static_cast<int64_t>(0)));
         if (taken > count) record_device_error(err, kDevNoPages);
@@ -285,12 +334,13 @@ extern "C" int lcml_kv_plan(const lcml_kv_plan_desc *d, lcml_stream_t stream) {
     const int rc = ensure_max_smem(reinterpret_cast<const void *>(k_kv_plan), (3 * kMaxRows + 2) * 4, "kv_plan");
     if (rc != LCML_OK) return rc;
     cudaLaunchConfig_t cfg = {};
-    // One CTA where it has a few rows and tokens a thread, else a cluster of 512 threads each
-    // (rows of 7001 tokens: 7.5 us, with 256 threads 10.5, with 1024 9.0, as clusters of those start later).
+    // One CTA where it has a few rows and tokens a thread, else a cluster of 512 threads each (9 rows of
+    // 7001 tokens: 6.5 us, with 256 threads 8.1, with 1024 7.0, as clusters of those start later), or of 1024
+    // where more rows than warps may end (26 of 256 rows: 11.7 us, with 512 12.9).
     const int64_t work = d->batch > (d->total_tokens + 3) / 4 ? d->batch : (d->total_tokens + 3) / 4;
     const bool alone = work <= kThreads && d->ended == nullptr;
     cfg.gridDim = dim3(alone ? 1 : kCluster);
-    cfg.blockDim = dim3(alone ? (work <= 128 ? 128 : static_cast<unsigned>((work + 31) / 32 * 32)) : 512);
+    cfg.blockDim = dim3(alone ? (work <= 128 ? 128 : static_cast<unsigned>((work + 31) / 32 * 32)) : (d->ended != nullptr && d->batch > kCluster * 16 ? kThreads : 512));
     cfg.dynamicSmemBytes = static_cast<size_t>(smem);
     cfg.stream = to_cuda(stream);
     cudaLaunchAttribute attr[2];
@@ -301,7 +351,7 @@ extern "C" int lcml_kv_plan(const lcml_kv_plan_desc *d, lcml_stream_t stream) {
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, k_kv_plan, *d, device_error_word());
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, k_kv_plan, *d, PageDivision(d->page_size), device_error_word());
     g_launches.fetch_add(1, std::memory_order_relaxed);
     if (e != cudaSuccess) {
         cudaGetLastError();

@@ -110,6 +110,31 @@ def test_plan_of_the_most_rows(dev):
     _check_plan(dev, [1] * 16384, held, [False] * 16384, 16, 6, spare=16384, in_place=True)
 
 
+@pytest.mark.parametrize("page", [1, 2, 3, 4, 5, 7, 48, 65536])
+def test_plan_of_long_rows(dev, page):
+    """runs of tokens of one row that begin and end inside a page, or span several"""
+    rng = random.Random(page)
+    new, held = [1, 700, 0, 2, 911, 1, 1301, 5], [rng.randint(0, 3 * page) for _ in range(8)]
+    cols = max(-(-(n + h) // page) for n, h in zip(new, held))
+    over = [False, False, True, False, True, False, False, False]
+    _check_plan(dev, new, held, [False] * 8, page, cols, spare=8 * cols, total=sum(new) + 3)
+    _check_plan(dev, new, held, over, page, cols, spare=8 * cols)
+    _check_plan(dev, new, held, over, page, cols, spare=cols)  # the list runs out
+    short = _no_device_error()
+    assert short in (0, 8)
+    _check_plan(dev, new, held, over, page, max(1, cols // 2), spare=8 * cols)  # rows longer than the table
+    assert _no_device_error() in (0, 7)
+
+
+def test_plan_of_pages_past_32_bits(dev):
+    """slots that int32 does not hold are -1"""
+    import luisaml_b200 as lb
+    free = _ints([1, (1 << 31) // 64 - 1, (1 << 31) // 64, 0x7fffffff, 3], dev)
+    p = lb.kv_plan(_ints([700], dev), _ints([0], dev), _ints([[-1] * 11], dev), free, _ints([5], dev), page_size=64, total=700)
+    want = [3 * 64 + i for i in range(64)] + [-1] * 128 + [(1 << 31) - 64 + i for i in range(64)] + [64 + i for i in range(64)] + [-1] * 380
+    assert p.slots.tolist() == want and p.positions.tolist() == list(range(700)) and _no_device_error() == 8
+
+
 def test_plan_of_nothing(dev):
     import luisaml_b200 as lb
     none = _ints([], dev)
