@@ -9,8 +9,7 @@
 // is taken is free_pages[count - 1 - i] for the i-th new entry of the batch, so
 // entry and slots are computed apart, without a second pass over the table.
 //
-// Bound: latency. A step of 64 rows moves 2 KB: 2.8 us. 256 rows of which 26 end, 45,000 tokens: 11.7 us,
-// a tenth of it the start of the cluster, a fifth its barriers.
+// Bound: latency. A step of 64 rows moves 2 KB: 2.8 us. 256 rows of which 26 end, 45,000 tokens: 11.7 us.
 #include <type_traits>
 
 #include "lcml_decoder.cuh"
