@@ -26,6 +26,8 @@ extern "C" {
  *       entries 0 .. ceil(held[b] / page_size) - 1, entries below 0 left out) go
  *       onto the free list in the order of rows and columns and become -1 in the
  *       table; the row then holds nothing, and new_tokens[b] is a new request's.
+ *       Nothing counts who else holds a page: one that two rows share is given back
+ *       by each that ends.
  *   start[b]  = ended[b] ? 0 : held[b]
  *   kv_len[b] = start[b] + new_tokens[b]
  *   cu_tokens = exclusive sums of new_tokens
