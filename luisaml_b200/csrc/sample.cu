@@ -977,7 +977,9 @@ __global__ void __launch_bounds__(NT, NT == 1024 ? 1 : 3) k_sample(SampleArgs a)
         }
         return;
     }
-    const float least = fmaxf(best - 693.147f * temperature, kLowest);  // 2^-1000
+    // 2^-1000. Rounded up: to nearest it may lie half a float's spacing lower, which at a small
+    // temperature is far more than the exponents that a weight has below 2^-1000.
+    const float least = fmaxf(__fsub_ru(best, 693.147f * temperature), kLowest);
     r.weight = Weight{best, per, least};
     const Weight &weight = r.weight;
 
@@ -1083,6 +1085,13 @@ __global__ void __launch_bounds__(NT, NT == 1024 ? 1 : 3) k_sample(SampleArgs a)
     const int from = passing != 0 ? __ffs(passing) - 1 : 31 - __clz(holding);
     owner = __shfl_sync(kAll, owner, from);
     at_warp = __shfl_sync(kAll, at_warp, from);
+    if (owner < 0) {  // no warp holds anything; the largest logit weighs 1, so no row comes here, and none would go without a token
+        if (r.rank == 0 && threadIdx.x == 0) {
+            a.tokens[row] = best_at;
+            if (a.logprob != nullptr) a.logprob[row] = 0.0f;
+        }
+        return;
+    }
     if (owner / kWarps != r.rank) return;
     // The owner's CTA: a warp per step of the owner's tokens finds the one that passes, else the last that holds anything.
     r.warp = owner % kWarps;

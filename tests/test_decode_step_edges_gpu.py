@@ -1,0 +1,61 @@
+"""Edges of the decode step's operators (include/lcml_decode_step.h): temperatures
+small against the spacing of the logits, and calls at the ends of the documented ranges."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from test_decode_step_gpu import _all, _error_word_stays_clear, _kept  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def _expected(x, t, u, top_k=0, top_p=1.0, min_p=0.0):
+    """(token, logprob) of one row, weights below 2^-1000 taken as 0"""
+    (kept,), w = _kept(x, t, top_k, top_p, min_p, (0.0,))
+    w = np.where(w < 2.0 ** -1000, 0.0, w)[kept]
+    c = np.cumsum(w)
+    i = int((c <= u * c[-1]).sum())
+    return int(kept[i]), math.log(w[i] / c[-1])
+
+
+@pytest.mark.parametrize("setting", [{}, {"top_k": 2}, {"top_k": 600}, {"top_p": 0.9}, {"min_p": 0.1}])
+@pytest.mark.parametrize("vocab,at", [(3001, (5, 9)), (3001, (9, 5)), (3001, (5, 2900)), (3001, (2900, 5)), (50001, (7, 8)), (50001, (40000, 7))])
+@pytest.mark.parametrize("top", [20.0, 1000.0, 10000.0, 1e9])
+def test_sample_logits_a_few_floats_apart(dev, top, vocab, at, setting):
+    """The two largest logits lie 1 to 40 floats apart, the temperature is 1/1500 to 1/20 of a
+    float's spacing there: the second one's weight is 0 or next to it, never negative."""
+    import luisaml_b200 as lb
+    step = float(np.spacing(np.float32(top)))
+    rows = [(n, np.float32(step / f), u) for n in (1, 2, 3, 7, 23, 40) for f in (1500, 1000, 800, 650, 347, 100, 20) for u in (0.0, 0.25, 1.0 - 2.0 ** -24)]
+    x = torch.zeros(len(rows), vocab)
+    x[:, at[0]] = top
+    x[:, at[1]] = torch.tensor([top - n * step for n, _, _ in rows])
+    t, u = (torch.tensor([float(r[i]) for r in rows], device=dev) for i in (1, 2))
+    tokens, logprob = torch.full((len(rows),), -7, dtype=torch.int32, device=dev), torch.full((len(rows),), 7.0, device=dev)
+    per_row = {k: _all(dev, len(rows), v, torch.int32 if k == "top_k" else torch.float32) for k, v in setting.items()}
+    lb.sample(x.to(dev), u, temperature=t, out=tokens, logprob=logprob, **per_row)
+    for r, (n, temperature, number) in enumerate(rows):
+        token, want = _expected(x[r].double().numpy(), float(temperature), number, **{k: float(np.float32(v)) if k != "top_k" else v for k, v in setting.items()})
+        assert tokens[r] == token, (n, temperature, number)
+        # a weight's error and the sum's, and half a step of the output
+        assert abs(float(logprob[r]) - want) <= 2.0 ** -24 * abs(want) + 1e-11, (n, temperature, number)
+
+
+@pytest.mark.parametrize("setting", [{}, {"top_k": 30}, {"top_p": 0.7}, {"min_p": 1e-3}])
+def test_sample_many_logits_a_few_floats_apart(dev, setting):
+    """40 neighbouring floats in rows of their own order"""
+    import luisaml_b200 as lb
+    step, rng = float(np.spacing(np.float32(1000.0))), np.random.default_rng(0)
+    rows = [(np.float32(step / f), u) for f in (1500, 800, 300, 30) for u in (0.0, 0.5, 1.0 - 2.0 ** -24)]
+    x = np.zeros((len(rows), 9001), dtype=np.float32)
+    for row in x:
+        row[rng.choice(9001, 40, replace=False)] = 1000.0 - step * np.arange(40)
+    t, u = (torch.tensor([float(r[i]) for r in rows], device=dev) for i in (0, 1))
+    tokens = torch.full((len(rows),), -7, dtype=torch.int32, device=dev)
+    per_row = {k: _all(dev, len(rows), v, torch.int32 if k == "top_k" else torch.float32) for k, v in setting.items()}
+    lb.sample(torch.from_numpy(x).to(dev), u, temperature=t, out=tokens, **per_row)
+    for r, (temperature, number) in enumerate(rows):
+        want = _expected(x[r].astype(np.float64), float(temperature), number, **{k: float(np.float32(v)) if k != "top_k" else v for k, v in setting.items()})
+        assert tokens[r] == want[0], (temperature, number)
