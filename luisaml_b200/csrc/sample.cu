@@ -24,7 +24,7 @@
 // the order of the sum. Where few tokens count they are packed 32 to a warp before
 // they are weighed (Queue).
 //
-// Bound: the instructions of the pass that weighs every token (10 of fp64, 3.7
+// Bound: the instructions of the pass that weighs every token (13 of fp64, 3.7
 // clocks of a scheduler each, and 30 others): of a row of 128001 fp32 logits in one
 // CTA, 128 of them beside each other, 12,000 clocks go to the load, 45,000 to the
 // weights, 14,000 to their bins, 25,000 to the pass for the cut at top_p 0.9 (more
@@ -101,15 +101,15 @@ struct Weight {
     float least;      // logits below it weigh nothing
     // 2^t, t = (x - top) per: t's nearest whole number by addition of 1.5 2^52, 2^f of the rest
     // on [-1/2, 1/2] as 1 + f p(f), p fitted at Chebyshev points with 2^f's relative
-    // error as the weight (8.2e-13), so the largest logit has exactly 1. The terms from f^5
-    // on are summed in fp32: 2^f is off by 5.1e-12 at most (9.1e-13 rms), and an
-    // fp64 instruction takes 3.7 clocks of a scheduler: 10 a token instead of 13.
+    // error as the weight (8.2e-13), so the largest logit has exactly 1.
     __device__ __forceinline__ double operator()(float x) const {
         const double d = static_cast<double>(x) - top, s = fma(d, per, 6755399441055744.0);
         const double f = fma(d, per, 6755399441055744.0 - s);
-        const float g = static_cast<float>(f);
-        const double high = fmaf(fmaf(fmaf(1.3178918944060163e-06f, g, 1.5309155627301653e-05f), g, 0.00015403825519790757f), g, 0.0013333454862616348f);
-        double p = fma(high, f, 0.009618128616057417);
+        double p = 1.3178918944060163e-06;
+        p = fma(p, f, 1.5309155627301653e-05);
+        p = fma(p, f, 0.00015403825519790757);
+        p = fma(p, f, 0.0013333454862616348);
+        p = fma(p, f, 0.009618128616057417);
         p = fma(p, f, 0.055504109352640572);
         p = fma(p, f, 0.24022650698110781);
         p = fma(p, f, 0.69314718054821356);

@@ -59,3 +59,19 @@ def test_sample_many_logits_a_few_floats_apart(dev, setting):
     for r, (temperature, number) in enumerate(rows):
         want = _expected(x[r].astype(np.float64), float(temperature), number, **{k: float(np.float32(v)) if k != "top_k" else v for k, v in setting.items()})
         assert tokens[r] == want[0], (temperature, number)
+
+
+def test_sample_weights_to_twelve_digits(dev):
+    """Two tokens and a number that lies 1.2e-12 to 5e-12 of the first one's weight beside the border
+    between them: the first one's weight decides on which side, to 1e-12."""
+    import luisaml_b200 as lb
+    x = np.arange(np.float32(0.25).view(np.uint32), np.float32(1.0).view(np.uint32), dtype=np.uint32).view(np.float32)  # all floats of [0.25, 1)
+    w = np.exp(-x.astype(np.float64))
+    u = (w / (1 + w)).astype(np.float32)
+    off = 1 - u.astype(np.float64) / (1 - u.astype(np.float64)) / w  # of w, above the border
+    near = np.nonzero((np.abs(off) > 1.2e-12) & (np.abs(off) < 5e-12))[0]
+    assert len(near) > 500
+    logits = torch.zeros(len(near), 2, device=dev)
+    logits[:, 0] = torch.from_numpy(-x[near]).to(dev)
+    got = lb.sample(logits, torch.from_numpy(u[near]).to(dev))
+    assert torch.equal(got.cpu(), torch.from_numpy((off[near] < 0).astype(np.int32)))
