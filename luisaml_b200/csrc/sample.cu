@@ -40,7 +40,7 @@
 namespace lcml {
 namespace {
 
-constexpr int kMaxCluster = 8;
+constexpr int kMaxCluster = 4;  // CTAs a row
 constexpr int kBins = 2048;
 constexpr int kList = 1024;  // tokens whose order is found in one CTA
 constexpr int kPairs = 256;  // of which so many by comparing each with each
@@ -1210,7 +1210,7 @@ int dispatch_sample(SampleArgs a, int64_t rows, cudaStream_t st) {
         a.slice = static_cast<int>(slice(few, 256));
         return launch_sample<T, true, 256>(a, rows, st);
     }
-    while (a.ctas < 4 && fits(2 * a.ctas) && slice(a.ctas, 1024) > 16384) a.ctas *= 2;
+    while (a.ctas < kMaxCluster && fits(2 * a.ctas) && slice(a.ctas, 1024) > 16384) a.ctas *= 2;
     a.slice = static_cast<int>(slice(a.ctas, 1024));
     if (a.slice * static_cast<int64_t>(sizeof(T)) > kStageMost<1024>) return launch_sample<T, false, 1024>(a, rows, st);
     return launch_sample<T, true, 1024>(a, rows, st);

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_decode_step_gpu import _all, _error_word_stays_clear, _kept  # noqa: F401
+from test_decode_step_gpu import _all, _check_sample, _error_word_stays_clear, _kept, _rows  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -75,3 +75,17 @@ def test_sample_weights_to_twelve_digits(dev):
     logits[:, 0] = torch.from_numpy(-x[near]).to(dev)
     got = lb.sample(logits, torch.from_numpy(u[near]).to(dev))
     assert torch.equal(got.cpu(), torch.from_numpy((off[near] < 0).astype(np.int32)))
+
+
+@pytest.mark.parametrize("dtype,least,most,step", [("f32", 39001, 45001, 500), ("bf16", 78001, 90001, 1000)])
+def test_sample_rows_as_long_as_shared_memory(dev, dtype, least, most, step):
+    """A row a CTA, a little shorter and a little longer than what it holds: the draws of the same rows by
+    several CTAs each, which are checked. No number lies within a rounding of a 64-bit sum of a border."""
+    import luisaml_b200 as lb
+    for vocab in range(least, most, step):
+        x, u = _rows(dev, 3, vocab, dtype)
+        for setting in ({}, {"top_p": 0.9}, {"top_k": 700, "min_p": 0.001}):
+            per_row = {k: _all(dev, 81, v, torch.int32 if k == "top_k" else torch.float32) for k, v in setting.items()}
+            want = _check_sample(x, u, **{k: v[:3] for k, v in per_row.items()})
+            got = lb.sample(x.repeat(27, 1), u.repeat(27), **per_row)  # more rows than half the SMs
+            assert torch.equal(got.view(27, 3), want.expand(27, 3)), (vocab, setting)
