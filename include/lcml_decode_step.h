@@ -124,9 +124,13 @@ int lcml_kv_attention_sinks(const lcml_kv_attention_desc *desc, int32_t sinks, l
  * one). logprob: log of the token's share of that sum. temperature <= 0 or NaN: the
  * lowest index of the largest logit, logprob 0. A NaN logit counts as -infinity; a
  * row with +infinity gives the first of those, logprob 0; a row of -infinity alone
- * gives token -1 and logprob NaN. Weights and sums are held in 64 bits, the
- * weights good to 1e-12 of each; w below 2^-1000 are 0. Parameters are device arrays of one value a row; NULL: off
- * (temperature: 1).
+ * gives token -1 and logprob NaN.
+ * Weights and sums are held in 64 bits, a weight good to 1e-12 of itself, but where up
+ * to 256 tokens stay, to 2^-52 of the largest (a lighter one counts as that much). w below
+ * 2^-1000 are 0. Equal calls give equal tokens. The same row in another batch or at
+ * another alignment is summed in another order: there a token may differ whose border
+ * uniform meets to the rounding of a 64-bit sum. Parameters are device arrays of one value
+ * a row; NULL: off (temperature: 1).
  */
 typedef struct lcml_sample_desc {
     int64_t rows, vocab;       /* vocab <= 2^31 - 65537 */

@@ -18,8 +18,8 @@
 // index, per warp, then the CTA that holds uniform * sum goes over that warp's tokens
 // once more. Up to 256 kept tokens are all in the list and drawn from there.
 //
-// Weights and sums are fp64, in an order that the sizes fix (of the list, whose order
-// atomics make, as 64-bit integers or sorted): a token lies within an fp32 rounding
+// Weights and sums are fp64, in an order that the sizes, the number of rows and the row's
+// alignment fix (of the list, whose order atomics make, as 64-bit integers or sorted): a token lies within an fp32 rounding
 // of its neighbours' range once in some thousand rows, and the result would go by
 // the order of the sum. Where few tokens count they are packed 32 to a warp before
 // they are weighed (Queue).

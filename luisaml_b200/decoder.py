@@ -139,8 +139,10 @@ def sample(logits, uniform, *, temperature=None, top_k=None, top_p=None, min_p=N
     Parameters are tensors of one value a row: ``temperature`` (0: the largest logit), ``top_k`` int32 (0: all),
     ``top_p`` of what top_k keeps (1: all), ``min_p`` of the largest probability (0: all). The draw is among the
     tokens that all of them keep, equal logits in the order of their indices, and takes the lowest index at
-    which their probabilities, summed by rising index, pass ``uniform``. Probabilities are held in 64 bits and
-    the order of every sum is fixed: equal inputs give equal tokens. ``logprob``: optional float32 [rows]
+    which their probabilities, summed by rising index, pass ``uniform``. Probabilities are held in 64 bits, good
+    to 1e-12 of each (where up to 256 tokens stay: or to 2^-52 of the largest). Equal calls give equal tokens; the
+    same row in another batch or at another alignment is summed in another order and may give another token where
+    ``uniform`` meets a border to the rounding of a 64-bit sum. ``logprob``: optional float32 [rows]
     output, the log of the token's probability among the kept ones. A row of -infinity alone gives -1.
     """
     return _bind.sample(logits, uniform, temperature, top_k, top_p, min_p, out, logprob)

@@ -89,3 +89,21 @@ def test_sample_rows_as_long_as_shared_memory(dev, dtype, least, most, step):
             want = _check_sample(x, u, **{k: v[:3] for k, v in per_row.items()})
             got = lb.sample(x.repeat(27, 1), u.repeat(27), **per_row)  # more rows than half the SMs
             assert torch.equal(got.view(27, 3), want.expand(27, 3)), (vocab, setting)
+
+
+@pytest.mark.parametrize("setting", [{}, {"temperature": 0.6, "top_p": 0.95}, {"top_k": 50}, {"top_k": 3000, "top_p": 0.8}, {"min_p": 0.02}])
+@pytest.mark.parametrize("vocab", [900, 10007, 128001])
+def test_sample_a_row_alone_in_a_batch_and_at_each_alignment(dev, vocab, setting):
+    """sums in another order, by another number of CTAs: the same tokens but next to a border (none here is)"""
+    import luisaml_b200 as lb
+    x, u = _rows(dev, 4, vocab)
+    per_row = {k: _all(dev, 100, v, torch.int32 if k == "top_k" else torch.float32) for k, v in setting.items()}
+    few = {k: v[:4] for k, v in per_row.items()}
+    want = _check_sample(x, u, **few)
+    for r in range(4):
+        assert lb.sample(x[r:r + 1], u[r:r + 1], **{k: v[:1] for k, v in per_row.items()}).item() == want[r]
+    assert torch.equal(lb.sample(x.repeat(25, 1), u.repeat(25), **per_row).view(25, 4), want.expand(25, 4))
+    for off in range(1, 4):
+        wide = torch.zeros(4, vocab + 5, device=dev)
+        wide[:, off:off + vocab] = x
+        assert torch.equal(lb.sample(wide[:, off:off + vocab], u, **few), want), off
