@@ -50,7 +50,7 @@ extern "C" {
 typedef struct lcml_kv_plan_desc {
     int32_t batch;             /* <= 16384 */
     int32_t page_size;         /* <= 65536 */
-    int32_t table_cols;
+    int32_t table_cols;        /* batch * table_cols <= 2^31 - 65537 */
     int64_t table_stride;
     int32_t *block_table;      /* device [batch, table_cols], changed in place */
     const int32_t *new_tokens; /* device [batch] */

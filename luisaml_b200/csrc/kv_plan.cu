@@ -320,7 +320,8 @@ extern "C" int lcml_kv_plan(const lcml_kv_plan_desc *d, lcml_stream_t stream) {
     LCML_CHECK_ARG(d->page_size > 0 && d->page_size <= 65536, "lcml_kv_plan: page_size %d", d->page_size);
     LCML_CHECK_ARG(d->table_cols >= 0 && d->table_stride >= d->table_cols, "lcml_kv_plan: table_stride is less than table_cols, or negative");
     LCML_CHECK_ARG(d->total_tokens >= 0 && d->total_tokens <= 0x7fffffff, "lcml_kv_plan: total_tokens is not in 0 .. 2^31 - 1");
-    LCML_CHECK_ARG(static_cast<int64_t>(d->batch) * d->table_cols <= 0x7fffffff, "lcml_kv_plan: the table has over 2^31 - 1 entries");
+    // entries and columns are counted in 32 bits, by strides of up to kCluster * kThreads
+    LCML_CHECK_ARG(static_cast<int64_t>(d->batch) * d->table_cols <= 0x7fffffff - 65536, "lcml_kv_plan: the table has over 2^31 - 65537 entries");
     LCML_CHECK_ARG(d->free_capacity >= 0, "lcml_kv_plan: negative free_capacity");
     LCML_CHECK_ARG(d->cu_tokens && d->free_count && d->free_count_out, "lcml_kv_plan: null pointer");
     LCML_CHECK_ARG(d->batch == 0 || (d->new_tokens && d->held && d->start && d->kv_len && (d->block_table || d->table_cols == 0)),
