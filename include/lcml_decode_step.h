@@ -82,7 +82,7 @@ int lcml_kv_plan(const lcml_kv_plan_desc *desc, lcml_stream_t stream);
  */
 typedef struct lcml_qk_norm_rope_desc {
     int64_t tokens;
-    int32_t q_heads, k_heads;  /* >= 0 */
+    int32_t q_heads, k_heads;  /* 0 .. 2^31 - 65537 */
     int32_t head_dim;          /* even, <= 512 */
     int32_t rotary;            /* even, <= head_dim */
     int dtype;                 /* FLOAT, FLOAT16 or BFLOAT16 */

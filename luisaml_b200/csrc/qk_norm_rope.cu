@@ -275,6 +275,8 @@ using namespace lcml;
 extern "C" int lcml_qk_norm_rope(const lcml_qk_norm_rope_desc *d, lcml_stream_t stream) {
     LCML_CHECK_ARG(d != nullptr, "lcml_qk_norm_rope: null descriptor");
     LCML_CHECK_ARG(d->tokens >= 0 && d->q_heads >= 0 && d->k_heads >= 0, "lcml_qk_norm_rope: negative extent");
+    // heads are counted in 32 bits, a group of up to 32 at a time
+    LCML_CHECK_ARG(d->q_heads <= 0x7fffffff - 65536 && d->k_heads <= 0x7fffffff - 65536, "lcml_qk_norm_rope: too many heads");
     LCML_CHECK_ARG(d->head_dim > 0 && d->head_dim % 2 == 0 && d->head_dim <= 512, "lcml_qk_norm_rope: head_dim %d is not even and at most 512", d->head_dim);
     LCML_CHECK_ARG(d->rotary >= 0 && d->rotary % 2 == 0 && d->rotary <= d->head_dim, "lcml_qk_norm_rope: rotary %d is not even and at most head_dim %d",
                    d->rotary, d->head_dim);
