@@ -28,7 +28,7 @@ class Decoder:
         self.hq, self.hk, self.d, self.page, self.window, self.sinks = q_heads, kv_heads, head_dim, page, window, sinks
         width = q_heads * head_dim
         g = torch.Generator(device=device).manual_seed(0)
-        torch.manual_seed(0)
+        torch.manual_seed(2)  # not the embedding's numbers: each token would be followed by itself
         self.embedding = torch.randn(vocab, width, generator=g, device=device).bfloat16()
         self.head = quantized_weight(vocab, width, device)
         self.norms = torch.rand(2 * layers + 1, width, generator=g, device=device) + 0.5

@@ -33,3 +33,21 @@ def test_example_compares_every_step(dev, monkeypatch, wrong):
     monkeypatch.setattr(decode_loop.Decoder, "step", planted)
     same, _, _, _ = decode_loop.run(**SIZES)
     assert len(seen) == SIZES["steps"] and same == (wrong is None)
+
+
+def test_example_draws_by_its_numbers(dev, monkeypatch):
+    """each row's tokens change from step to step: the weights are not such that a token is followed by itself"""
+    sys.path.insert(0, os.path.join(ROOT, "examples"))
+    import decode_loop
+    step, seen = decode_loop.Decoder.step, []
+
+    def kept(self, tokens, new, ended, max_tokens, draw):
+        got = step(self, tokens, new, ended, max_tokens, draw)
+        if not torch.cuda.is_current_stream_capturing():
+            seen.append(got)
+        return got
+
+    monkeypatch.setattr(decode_loop.Decoder, "step", kept)
+    assert decode_loop.run(**SIZES)[0]
+    drawn = torch.stack(seen[:SIZES["steps"] + 1])
+    assert min(drawn[:, b].unique().numel() for b in range(SIZES["batch"])) > SIZES["steps"] // 2
