@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_decode_step_gpu import _all, _check_sample, _error_word_stays_clear, _kept, _rows  # noqa: F401
+from test_decode_step_gpu import _all, _check_plan, _check_sample, _error_word_stays_clear, _kept, _no_device_error, _rows  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -107,3 +107,35 @@ def test_sample_a_row_alone_in_a_batch_and_at_each_alignment(dev, vocab, setting
         wide = torch.zeros(4, vocab + 5, device=dev)
         wide[:, off:off + vocab] = x
         assert torch.equal(lb.sample(wide[:, off:off + vocab], u, **few), want), off
+
+
+@pytest.mark.parametrize("use_ended", [False, True])
+@pytest.mark.parametrize("batch,new,held,page,cols,spare,code", [
+    (8, 700, 50, 16, 60, 8 * 60, 0),
+    (8, 700, 50, 16, 60, 3, 8),  # the list runs out
+    (8, 700, 50, 16, 30, 8 * 60, 7),  # rows longer than the table
+    (300, 9, 20, 16, 2, 300 * 2, 0),
+    (300, 9, 40, 16, 2, 300 * 2, 7),
+    (300, 9, 24, 16, 3, 10, 8),
+    (1, 5000, 0, 1, 5000, 5000, 0),
+    (1, 5000, 0, 1, 5000, 4999, 8),
+    (1, 5000, 1, 1, 5000, 5001, 7)])
+def test_plan_says_what_does_not_fit(dev, batch, new, held, page, cols, spare, code, use_ended):
+    """the error word is 8, 7 or clear, as the lengths say"""
+    _check_plan(dev, [new] * batch, [held] * batch, [False] * batch, page, cols, spare=spare, use_ended=use_ended)
+    assert _no_device_error() == code
+
+
+@pytest.mark.parametrize("case", ["negative new", "negative held", "tokens left out", "list full"])
+def test_plan_says_which_lengths_are_wrong(dev, case):
+    new, held, ended, kw = [3, 4, 5], [20, 0, 33], [False, False, case == "list full"], {}
+    if case == "negative new":
+        new[1] = -1
+    elif case == "negative held":
+        held[1] = -5
+    elif case == "tokens left out":
+        kw["total"] = 11
+    else:
+        kw["capacity"] = 10
+    _check_plan(dev, new, held, ended, 16, 4, spare=8 if case == "list full" else 12, **kw)
+    assert _no_device_error() == 7
