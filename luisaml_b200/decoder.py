@@ -113,7 +113,9 @@ def kv_plan(new_tokens, held, block_table, free_pages, free_count, *, page_size,
     list first and ``new_tokens`` is the row's new request's. ``total``: length of the packed maps, at
     least the batch's new tokens. ``kv_len`` and ``free_count_out``: outputs, which may be ``held`` and
     ``free_count`` themselves, so that a captured step moves on with each replay.
-    Returns a :class:`KvPlan`. An empty free list shows in :func:`luisaml_b200.device_error` as 8,
+    Returns a :class:`KvPlan`. Its tensors that are not given share one allocation, which lives as long as any
+    of them: none may be resized (it would run into the next), and a small one that is kept for long is better
+    cloned. An empty free list shows in :func:`luisaml_b200.device_error` as 8,
     lengths that do not fit as 7; what has no page gets -1 and is never followed.
     """
     return tuple.__new__(KvPlan, _bind.kv_plan(new_tokens, held, block_table, free_pages, free_count, ended, page_size, total, kv_len, free_count_out))
