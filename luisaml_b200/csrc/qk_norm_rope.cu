@@ -19,7 +19,8 @@
 // registers, 32.5 so: 5.2 of a copy's 6.5 TB/s). Below some thousand tokens it is
 // latency: position, angles (fp64), the first heads; one token 2.9 us, 3001 of
 // 24 heads of 96 in fp32 14.2 us (16.4 where neighbouring pairs of a quarter turn: both
-// kinds of chunk share a warp), floor 8.5.
+// kinds of chunk share a warp), floor 8.5. Heads that are not 16-byte aligned go element by
+// element (E = 1): 8191 tokens of 40 heads 93 us, one 2.8.
 #include "lcml_decoder.cuh"
 
 #include "../../include/lcml_decode_step.h"
@@ -237,8 +238,9 @@ int launch_rope(RopeArgs a, bool inter, cudaStream_t st) {
     while (a.lanes < 32 && a.lanes * C < chunks) a.lanes *= 2;
     // A warp per token where there are 24 an SM, as many as it holds; else a token's heads are
     // shared until there are (one token of 40 heads of 128: one warp 8 us, ten 2.9; 300 tokens:
-    // four warps each 5.9, all ten 4.3; 3001 of 24 heads of 96 in fp32: one 20.4, two 16.6; but
-    // 1000 of 40 heads: three, all at once, 7.4, four 9.2).
+    // four warps each 5.9, all ten 4.3; 3001 of 24 heads of 96 in fp32: one 20.4, two 16.6). The
+    // share is rounded up, which may leave a few warps to a second round: 1000 of 40 heads get four, 9.1
+    // us, where three, all at once, take 7.4.
     const int per_warp = 32 / a.lanes;
     const int64_t most = (a.heads[0] + per_warp - 1) / per_warp + (a.heads[1] + per_warp - 1) / per_warp;
     const int64_t want = static_cast<int64_t>(sm_count()) * 24;

@@ -24,13 +24,13 @@
 // the order of the sum. Where few tokens count they are packed 32 to a warp before
 // they are weighed (Queue).
 //
-// Bound: the instructions of the pass that weighs every token (13 of fp64, 3.7
-// clocks of a scheduler each, and 30 others): of a row of 128001 fp32 logits in one
-// CTA, 128 of them beside each other, 12,000 clocks go to the load, 45,000 to the
-// weights, 14,000 to their bins, 25,000 to the pass for the cut at top_p 0.9 (more
-// the more tokens that keeps) and 15,000 to the rest: 74 us, 41 without top_p, 25 with
-// top_k 50 (floor 10). Small calls are a chain of some ten barriers and fp64 sums:
-// 10 us for a row of 2000, 11 to 13 for one of 32000 with top_k.
+// Bound: the phases of a row, one after the other, and their instructions (128 rows of 128001
+// with top_p: 63 % of the issue slots, 18 % of the fp64 pipe). Of a row of 128001 fp32 logits in
+// one CTA, 128 of them beside each other, 12,000 clocks go to the load, 45,000 to the
+// weights (13 fp64 instructions a token and 30 others), 14,000 to their bins, 25,000 to
+// the pass for the cut at top_p 0.9 (more the more tokens that keeps) and 15,000 to the
+// rest: 77 us, 39 without top_p, 23 with top_k 50 (floor 10). Small calls are a chain of some
+// ten barriers and fp64 sums: 14 us for a row of 2000 with top_p, 11 for one of 32000 with top_k.
 #include <type_traits>
 
 #include "lcml_decoder.cuh"
@@ -1198,11 +1198,11 @@ int dispatch_sample(SampleArgs a, int64_t rows, cudaStream_t st) {
         const int64_t unit = static_cast<int64_t>(threads) * E * ctas;
         return (length + unit - 1) / unit * threads * E;
     };
-    // CTAs of 256 threads where they hold few tokens (rows of 2000: 1 of them 13.4 us, 16.0 in CTAs of
-    // 1024; 8 of 10000 with top_k 100 14.1 and 17.3), else of 1024, one an SM.
+    // CTAs of 256 threads where they hold few tokens (a row of 2000 with top_p in two of them 13.8 us, 15.3 in
+    // two of 1024; 8 of 10000 with top_k 100 11.6 and 13.0), else of 1024, one an SM.
     // Several CTAs a row while each finds an SM and keeps 16384 tokens: 16 rows of 128001 with top_p 0.9
-    // take 69 us in one each, 44 in two, 33 in four; in eight 62, as clusters of so many find no
-    // room beside each other. 36 rows 80, 50 and, no longer all at once, 63.
+    // take 74 us in one each, 47 in two, 35 in four; in eight 62, as clusters of so many find no
+    // room beside each other. 36 rows 74, 47 and, no longer all at once, 64.
     auto fits = [&](int ctas) { return rows * ctas <= sm_count() * 7 / 8; };
     const int few = fits(2) ? 2 : 1;
     if (a.vocab <= few * few * 4096) {
